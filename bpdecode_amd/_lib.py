@@ -16,7 +16,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libbpdecode_hip.so"
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 OK, ERR_INVALID, ERR_HIP, ERR_OVERFLOW, ERR_UNSUPPORTED = 0, 1, 2, 3, 4
 DTYPE_F32, DTYPE_F16, DTYPE_BF16, DTYPE_F64 = 0, 1, 2, 3
@@ -24,7 +24,8 @@ INDEX_I32, INDEX_I64, INDEX_I64_LOW32 = 0, 1, 2
 MAX_FUSED_PENDING = 256  # BPD_MAX_FUSED_PENDING
 MAX_INLINE_VALUES = 960  # BPD_MAX_INLINE_VALUES
 MAX_PRIOR_INLINE_VALUES = 320  # BPD_MAX_PRIOR_INLINE_VALUES
-FLAG_STATE_RANGE, FLAG_TOKEN_RANGE = 1, 2
+FLAG_STATE_RANGE, FLAG_TOKEN_RANGE, FLAG_PAGE_RANGE, FLAG_LOGITS = 1, 2, 4, 8
+MAX_DRAFTS = 63  # BPD_MAX_DRAFTS
 PDA_MAX_CONFIGS = 8
 PDA_MAX_DEPTH = 32
 PDA_CONFIG_WORDS = 2 + PDA_MAX_CONFIGS + PDA_MAX_CONFIGS * PDA_MAX_DEPTH
@@ -145,6 +146,23 @@ _SIGNATURES = {
     "bpd_host_soft_prior": (cint, [vp, i64, i64, i64, vp, i32, vp, vp, i32, vp, vp, i32, f32]),
     "bpd_host_soft_build_lookahead": (cint, [vp, i32, i64, vp, vp, i32, i32, vp]),
     "bpd_host_soft_apply": (cint, [vp, cint, i64, i64, i64, vp, i32, vp, vp, f32]),
+    "bpd_verify_workspace_bytes": (sz, [i64, i32, i64]),
+    "bpd_verify": (cint, [vp, cint, i64, i32, i64, i64, i64, vp, cint, i64, vp, vp, cint, i64, i64, vp, i64,
+                          vp, f32, vp, i64, i32, vp, vp, vp, vp, cint, vp, vp, vp, vp, sz, vp, vp]),
+    "bpd_host_verify": (cint, [vp, cint, i64, i32, i64, i64, i64, vp, cint, i64, vp, vp, cint, i64, i64, vp,
+                               i64, vp, f32, vp, i64, i32, vp, vp, vp, vp, cint, vp, vp, vp, vp]),
+    "bpd_kv_append": (cint, [vp, i64, i32, i32, i32, cint, vp, i64, i64, i64, vp, i64, i64, i64, vp, i64, i64,
+                             i64, i32, vp, i64, i32, vp, i64, i32, vp, vp, vp, vp, i64, i32, cint, vp, vp]),
+    "bpd_host_kv_append": (cint, [vp, i64, i32, i32, i32, cint, vp, i64, i64, i64, vp, i64, i64, i64, vp, i64,
+                                  i64, i64, i32, vp, i64, i32, vp, i64, i32, vp, vp, vp, vp, i64, i32, cint,
+                                  vp]),
+    "bpd_kv_read": (cint, [vp, i64, i32, i32, i32, cint, vp, vp, i64, i32, vp, i64, i32, vp, vp, vp, vp]),
+    "bpd_host_kv_read": (cint, [vp, i64, i32, i32, i32, cint, vp, vp, i64, i32, vp, i64, i32, vp, vp, vp]),
+    "bpd_kv_attend_workspace_bytes": (sz, [i64, i32, i32, i32, i32, i64]),
+    "bpd_kv_attend": (cint, [vp, i64, i32, i32, i32, cint, vp, i64, i64, i64, i32, vp, i64, i32, vp, i64, i32,
+                             vp, vp, f32, vp, sz, vp, vp]),
+    "bpd_host_kv_attend": (cint, [vp, i64, i32, i32, i32, cint, vp, i64, i64, i64, i32, vp, i64, i32, vp, i64,
+                                  i32, vp, vp, f32, vp]),
 }
 
 _lib = None

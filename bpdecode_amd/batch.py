@@ -598,6 +598,28 @@ class ConstraintBatch:
         pool[slots] = nxt
         return nxt
 
+    def verify(self, seq_ids: Sequence[Hashable], logits: torch.Tensor, draft_tokens: torch.Tensor,
+               uniforms: torch.Tensor, *, draft_probs: torch.Tensor | None = None,
+               draft_lens: torch.Tensor | None = None,
+               temperature: float | torch.Tensor = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
+        """Verify a block of drafted tokens per sequence against ``logits``
+        [len(seq_ids), drafts + 1, columns] under the grammar, and advance each
+        sequence by the drafts that stand and the token after them
+        (:func:`~bpdecode_amd.ops.verify_draft`).  Returns int32 (accepted,
+        next_token); a sequence whose grammar allows nothing after its accepted
+        drafts yields -1 and is ``BROKEN``."""
+        slots = self._slots(seq_ids)
+        pool = self._state
+        kw = {"draft_probs": draft_probs, "draft_lens": draft_lens, "temperature": temperature, "err": self._err}
+        if self.fsa.tok_next is not None:
+            n, token, _ = ops.dense_verify(logits, draft_tokens, uniforms, tok_next=self.fsa.tok_next,
+                                           allow_bits=self.fsa.ensure_allow_bits(), states=pool, slots=slots,
+                                           write_back=True, **kw)
+            return n, token
+        n, token, state = ops._walked_verify(logits, draft_tokens, uniforms, self.fsa, pool[slots], **kw)
+        pool[slots] = state
+        return n, token
+
     def check_errors(self) -> None:
         """Raise if a device kernel met an out-of-range state or token since
         the last check (synchronises with the device)."""

@@ -824,5 +824,165 @@ def advance_state(fsa: FsaTensors, states: torch.Tensor, token_ids: torch.Tensor
     return dense_advance(rows, idx, token_ids)
 
 
+def dense_verify(logits, draft_tokens, uniforms, *, draft_probs=None, draft_lens=None, temperature=1.0, vocab=None,
+                 tok_next=None, allow_bits=None, bit_rows=None, states=None, slots=None, write_back=False, err=None):
+    """:func:`verify_draft` over the tables themselves: ``allow_bits`` (packed,
+    one row per state) with ``tok_next`` and ``states`` (walked along the
+    drafts; the state of request b is ``states[slots[b]]`` with ``slots``, and
+    ``write_back`` updates it there) or with ``bit_rows`` int32 [batch, drafts
+    + 1], the row of ``allow_bits`` of each position.  ``vocab``: columns that
+    are tokens (all of ``logits``, or of ``tok_next``, without it)."""
+    if logits.dim() != 3 or draft_tokens.dim() != 2 or uniforms.dim() != 2:
+        raise RuntimeError("logits must be [batch, drafts + 1, vocab], draft_tokens [batch, drafts], "
+                           "uniforms [batch, drafts + 1]")
+    B, T = draft_tokens.shape
+    if logits.shape[:2] != (B, T + 1) or uniforms.shape != (B, T + 1):
+        raise RuntimeError(f"{T} drafted tokens of {B} requests need logits and uniforms at {T + 1} positions, "
+                           f"got {list(logits.shape)} and {list(uniforms.shape)}")
+    if T > _lib.MAX_DRAFTS:
+        raise RuntimeError(f"at most {_lib.MAX_DRAFTS} drafted tokens, got {T}")
+    V = vocab if vocab is not None else logits.shape[2] if tok_next is None else tok_next.shape[1]
+    if not 1 <= V <= logits.shape[2]:
+        raise RuntimeError(f"logits have {logits.shape[2]} columns for a vocabulary of {V} tokens")
+    if uniforms.dtype != torch.float32:
+        raise RuntimeError("uniforms must be float32")
+    if tok_next is not None and (tok_next.dim() != 2 or tok_next.shape[1] != V):
+        raise RuntimeError(f"tok_next has {list(tok_next.shape)} entries for a vocabulary of {V} tokens")
+    if (tok_next is None) == (bit_rows is None) and allow_bits is not None:
+        raise RuntimeError("allow_bits needs tok_next or bit_rows")
+    if allow_bits is None and (tok_next is not None or bit_rows is not None):
+        raise RuntimeError("tok_next and bit_rows need allow_bits")
+    temp = temperature if isinstance(temperature, torch.Tensor) else None
+    dev = _same_device(logits, draft_tokens, uniforms, draft_probs, draft_lens, temp, tok_next, allow_bits, bit_rows,
+                       states, slots)
+    code = _lib.dtype_code(logits.dtype)
+    if logits.stride(2) != 1:
+        logits = logits.contiguous()
+    tk = draft_tokens if draft_tokens.dtype in (torch.int32, torch.int64) else draft_tokens.to(torch.int64)
+    if T > 1 and tk.stride(1) != 1:
+        tk = tk.contiguous()
+    if uniforms.stride(1) != 1 and T:
+        uniforms = uniforms.contiguous()
+    probs = (None, 0, 0, 0)
+    if draft_probs is not None:
+        if draft_probs.dim() != 3 or draft_probs.shape[:2] != (B, T) or draft_probs.shape[2] < V:
+            raise RuntimeError(f"draft_probs must be [{B}, {T}, at least {V}], got {list(draft_probs.shape)}")
+        pcode = _lib.dtype_code(draft_probs.dtype)
+        if draft_probs.stride(2) != 1:
+            draft_probs = draft_probs.contiguous()
+        if T:
+            probs = (draft_probs.data_ptr(), pcode, draft_probs.stride(0), draft_probs.stride(1))
+    if draft_lens is not None:
+        if draft_lens.shape != (B,):
+            raise RuntimeError("one draft length per request")
+        draft_lens = _i32(draft_lens)
+    if temp is not None:
+        if temp.shape != (B,):
+            raise RuntimeError("one temperature per request")
+        temp = temp.to(torch.float32).contiguous()
+    S = words = 0
+    if allow_bits is not None:
+        if allow_bits.dim() != 2 or allow_bits.dtype != torch.int32 or allow_bits.shape[1] != (V + 31) // 32:
+            raise RuntimeError(f"allow_bits must be int32 [states, {(V + 31) // 32}]")
+        allow_bits = allow_bits.contiguous()
+        S, words = allow_bits.shape
+    sl = None
+    if tok_next is not None:
+        tok_next = _i32(tok_next)
+        if tok_next.shape[0] != S:
+            raise RuntimeError(f"tok_next has {tok_next.shape[0]} states but allow_bits has {S}")
+        if states is None:
+            raise RuntimeError("tok_next needs the requests' states")
+        if slots is not None:
+            if slots.numel() != B:
+                raise RuntimeError("one slot per request")
+            sl = slots.to(torch.int64).contiguous()
+        elif states.numel() != B:
+            raise RuntimeError(f"one state per request (got {states.numel()} states for {B} requests)")
+        if write_back and (states.dtype != torch.int32 or not states.is_contiguous()):
+            raise RuntimeError("write_back needs a contiguous int32 state pool")
+        states = _i32(states)
+    elif bit_rows is not None:
+        if bit_rows.shape != (B, T + 1):
+            raise RuntimeError(f"bit_rows must be [{B}, {T + 1}]")
+        bit_rows = _i32(bit_rows)
+    if write_back and tok_next is None:
+        raise RuntimeError("states are advanced through tok_next only")
+    out = torch.empty((3, B), dtype=torch.int32, device=dev)
+    n, token, state = out.unbind(0)
+    args = (logits.data_ptr(), code, B, T, V, logits.stride(0), logits.stride(1), tk.data_ptr() if T else None,
+            _lib.index_code(tk.dtype), tk.stride(0), ptr(draft_lens), *probs, uniforms.data_ptr(), uniforms.stride(0),
+            ptr(temp), 0.0 if temp is not None else float(temperature), ptr(allow_bits), words, S, ptr(tok_next),
+            ptr(states) if tok_next is not None else None, ptr(sl), ptr(bit_rows), int(write_back), n.data_ptr(),
+            token.data_ptr(), state.data_ptr() if tok_next is not None else None)
+    if dev.type == "cuda":
+        need = int(lib().bpd_verify_workspace_bytes(B, T, V))
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        check(lib().bpd_verify(*args, ptr(ws), need, ptr(err), _lib.stream_of(dev)))
+    else:
+        check(lib().bpd_host_verify(*args, ptr(err)))
+    return (n, token) if tok_next is None else (n, token, state)
+
+
+def _walked_verify(logits, draft_tokens, uniforms, fsa: FsaTensors, states, err=None, **kw):
+    """:func:`verify_draft` for a bundle without ``tok_next``: the states of
+    the positions walked first, one round of :func:`advance_state` per drafted
+    token, then their rows of the allow-bit table (of masks walked for them,
+    where the bundle has none), and the state after the next token last."""
+    V = fsa.vocab_size
+    B, T = draft_tokens.shape
+    s = [_i32(states)]
+    for i in range(T):
+        x = draft_tokens[:, i]
+        ok = (x >= 0) & (x < V)
+        nxt = advance_state(fsa, s[i], torch.where(ok, x, 0))
+        s.append(torch.where(ok, nxt, -1))
+    rows = torch.stack(s, 1)
+    bits = fsa.allow_bits_or_none()
+    at = rows
+    if bits is None:
+        bits = compute_mask(fsa, rows.view(-1).clone())
+        at = torch.arange(B * (T + 1), dtype=torch.int32, device=rows.device).view(B, T + 1)
+    n, token = dense_verify(logits, draft_tokens, uniforms, vocab=V, allow_bits=bits, bit_rows=at, err=err, **kw)
+    last = rows.gather(1, n.long()[:, None])[:, 0]
+    nxt = advance_state(fsa, last.contiguous(), token.clamp(min=0))
+    return n, token, torch.where(token < 0, -1, nxt)
+
+
+def verify_draft(logits: torch.Tensor, draft_tokens: torch.Tensor, uniforms: torch.Tensor, fsa: FsaTensors | None = None,
+                 states: torch.Tensor | None = None, *, draft_probs: torch.Tensor | None = None,
+                 draft_lens: torch.Tensor | None = None, temperature: float | torch.Tensor = 1.0):
+    """How many drafted tokens of each request stand, and the token after them.
+
+    ``logits`` [batch, drafts + 1, columns] are the target model's after 0, 1,
+    ... drafted tokens ``draft_tokens`` [batch, drafts]; ``draft_probs``
+    [batch, drafts, columns] the probabilities they were sampled from (None:
+    the draft was certain, as a token looked up in the prompt is);
+    ``draft_lens`` the drafts of each request that count.  With p the softmax
+    of ``logits`` at ``temperature`` (one number or one per request; 0: all on
+    the first largest) over the tokens that the grammar ``fsa`` allows after
+    the drafts before, draft i stands while ``uniforms[:, i] * q < p`` at its
+    token, and the next token is drawn by ``uniforms[:, drafts]`` from
+    max(p - q, 0) at the first that does not, or from p after a whole block:
+    what is emitted is distributed as p.  Without drafts ([batch, 0]) this
+    samples one token.  Columns past the grammar's vocabulary never count.
+
+    Returns int32 (accepted, next_token), and with ``fsa`` and ``states`` (one
+    per request) the states after both; a position that allows nothing yields
+    -1 for either."""
+    if fsa is None:
+        if states is not None:
+            raise RuntimeError("states without a grammar")
+        return dense_verify(logits, draft_tokens, uniforms, draft_probs=draft_probs, draft_lens=draft_lens,
+                            temperature=temperature)
+    if states is None:
+        raise RuntimeError("a grammar needs one state per request")
+    kw = {"draft_probs": draft_probs, "draft_lens": draft_lens, "temperature": temperature}
+    if fsa.tok_next is None:
+        return _walked_verify(logits, draft_tokens, uniforms, fsa, states, **kw)
+    return dense_verify(logits, draft_tokens, uniforms, tok_next=fsa.tok_next, allow_bits=fsa.ensure_allow_bits(),
+                        states=states, **kw)
+
+
 # registers torch.ops.bpdecode.* (the reference loads its extension at this point)
 from . import torch_ops as _torch_ops  # noqa: E402,F401

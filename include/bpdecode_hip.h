@@ -63,6 +63,11 @@ extern "C" {
 /* Bits OR-ed into the optional `err` word by kernels (device int32). */
 #define BPD_FLAG_STATE_RANGE 1 /* a state >= num_states was read */
 #define BPD_FLAG_TOKEN_RANGE 2 /* a token outside [-vocab, vocab) was read */
+#define BPD_FLAG_PAGE_RANGE 4  /* a position or page outside a cache, its block table or the rotation's tables */
+#define BPD_FLAG_LOGITS 8      /* an allowed logit was +inf or NaN */
+
+/* Drafted tokens of one request that bpd_verify takes. */
+#define BPD_MAX_DRAFTS 63
 
 #define BPD_PDA_MAX_CONFIGS 8
 #define BPD_PDA_MAX_DEPTH 32
@@ -645,6 +650,133 @@ int bpd_soft_prior_noalloc(float* logits, int64_t rows, int64_t vocab, int64_t l
                            int32_t eos_id, const int32_t* states, const int64_t* slots,
                            const BpdSoftClasses* classes, int32_t k, float alpha, int32_t* err,
                            void* stream);
+
+/* --------------------------------------------------- speculative step --
+ * bpd_verify: how many of a request's drafted tokens stand, and the token that
+ * follows them.  For request b and position i, z = logits + b * ld_row +
+ * i * ld_pos (elements, [rows, drafts + 1, >= vocab]) are the target's logits
+ * after i drafted tokens; p_i is their softmax at the request's temperature
+ * over the allowed tokens (temperature 0, or not positive and finite: all on
+ * the first largest), q_i the draft's probabilities probs + b * probs_row +
+ * i * probs_pos, or with probs NULL all on the drafted token.  With n_b =
+ * draft_lens[b] (cut to 0..drafts; NULL: drafts) draft i < n_b stands while
+ * uniforms[b][i] * q_i(x_i) < p_i(x_i); accepted[b] counts those before the
+ * first that does not.  next_token[b] is the first token whose running sum of
+ * max(p - q, 0) at that position (of p after a whole block, or where that sum
+ * is 0) passes uniforms[b][drafts] times the whole sum; -1 where the position
+ * allows nothing: no allowed token, every allowed logit -inf, or an allowed
+ * logit +inf or NaN (BPD_FLAG_LOGITS).  Sums that decide a token are held in
+ * 64 bits.
+ * Grammar: allow_bits uint32 [num_states, words] with either tok_next and
+ * states (states[slots ? slots[b] : b], walked along the drafted tokens;
+ * next_state[b] (may be NULL) and, with write_back, the pool entry become the
+ * state after next_token, -1 where there is none), or bit_rows int32 [rows,
+ * drafts + 1], the row of allow_bits of each position (-1: allows nothing).
+ * NULL allow_bits: every token is allowed.  A drafted token outside
+ * [0, vocab) does not stand (BPD_FLAG_TOKEN_RANGE); a state at or above
+ * num_states allows nothing (BPD_FLAG_STATE_RANGE).  tokens: int32 or int64,
+ * row stride tokens_ld; temperature float [rows] on the device, or NULL and
+ * temperature_all.  workspace: bpd_verify_workspace_bytes bytes, 16-byte
+ * aligned.  No counterpart in the reference, which samples one token per
+ * step outside itself. */
+size_t bpd_verify_workspace_bytes(int64_t rows, int32_t drafts, int64_t vocab);
+int bpd_verify(const void* logits, int dtype, int64_t rows, int32_t drafts, int64_t vocab,
+               int64_t ld_row, int64_t ld_pos, const void* tokens, int token_dtype,
+               int64_t tokens_ld, const int32_t* draft_lens, const void* probs, int probs_dtype,
+               int64_t probs_row, int64_t probs_pos, const float* uniforms, int64_t uniforms_ld,
+               const float* temperature, float temperature_all, const uint32_t* allow_bits,
+               int64_t words, int32_t num_states, const int32_t* tok_next, int32_t* states,
+               const int64_t* slots, const int32_t* bit_rows, int write_back, int32_t* accepted,
+               int32_t* next_token, int32_t* next_state, void* workspace, size_t workspace_bytes,
+               int32_t* err, void* stream);
+int bpd_host_verify(const void* logits, int dtype, int64_t rows, int32_t drafts, int64_t vocab,
+                    int64_t ld_row, int64_t ld_pos, const void* tokens, int token_dtype,
+                    int64_t tokens_ld, const int32_t* draft_lens, const void* probs,
+                    int probs_dtype, int64_t probs_row, int64_t probs_pos, const float* uniforms,
+                    int64_t uniforms_ld, const float* temperature, float temperature_all,
+                    const uint32_t* allow_bits, int64_t words, int32_t num_states,
+                    const int32_t* tok_next, int32_t* states, const int64_t* slots,
+                    const int32_t* bit_rows, int write_back, int32_t* accepted,
+                    int32_t* next_token, int32_t* next_state, int32_t* err);
+
+/* The paged key/value cache in 4 bits.  pages uint8 [num_pages, kv_heads,
+ * bytes], 16-byte aligned; the block of one page and head holds, for its
+ * page_size tokens in order: key codes [page_size, head_dim / 2], value codes
+ * (the same), key scales [page_size, head_dim / 32], value scales (the same).
+ * Channel 2j of a token is the low half of code byte j.  A code is e2m1 (a
+ * sign and 0, .5, 1, 1.5, 2, 3, 4, 6), a scale byte e stands for 2^(e - 127)
+ * and 32 neighbouring channels: the smallest with max|x| <= 7 * 2^(e - 127)
+ * that the cache's type holds (bfloat16: 2 <= e <= 252, float16: 104 <= e <=
+ * 140); codes are rounded to nearest, ties to the even code, and 255 marks a
+ * group that held an infinity or a NaN and reads as NaN.  page_size: a power
+ * of two from 16 to 256; head_dim: 64, 96, 128, 192 or 256; dtype (of q, k, v
+ * and every output): BPD_DTYPE_F16 or BPD_DTYPE_BF16.  Token p of request b
+ * lies in page block_table[b * table_ld + p / page_size] (int32, table_blocks
+ * per request).  Positions and pages outside their tables are left out and
+ * set BPD_FLAG_PAGE_RANGE in `err`; no memory outside them is touched.
+ *
+ * bpd_kv_append: tokens starts[b] + i, i < counts[b] (NULL: tokens), of k and
+ * v [rows, tokens, kv_heads, head_dim] (strides in elements, channels next to
+ * each other) into the cache; k and q [rows, tokens, heads, head_dim] (heads 0:
+ * none) are rotated first: (x, y) -> (x cos - y sin, y cos + x sin) in float
+ * for channel pairs (j, j + rotary / 2), or (2j, 2j + 1) with `interleaved`,
+ * by cos/sin float [positions, rotary / 2] at the token's position.  q_out
+ * [rows, tokens, heads, head_dim] contiguous, zeros for tokens past counts[b].
+ * Two requests must not append to one page.
+ * bpd_kv_read: tokens starts[b] + i, i < counts[b], back as k_out and v_out
+ * [rows, tokens, kv_heads, head_dim] contiguous; zeros past counts[b] and for
+ * tokens outside the tables. */
+int bpd_kv_append(uint8_t* pages, int64_t num_pages, int32_t page_size, int32_t kv_heads,
+                  int32_t head_dim, int dtype, const void* k, int64_t k_row, int64_t k_token,
+                  int64_t k_head, const void* v, int64_t v_row, int64_t v_token, int64_t v_head,
+                  const void* q, int64_t q_row, int64_t q_token, int64_t q_head, int32_t heads,
+                  void* q_out, int64_t rows, int32_t tokens, const int32_t* block_table,
+                  int64_t table_ld, int32_t table_blocks, const int32_t* starts,
+                  const int32_t* counts, const float* cos, const float* sin, int64_t positions,
+                  int32_t rotary, int interleaved, int32_t* err, void* stream);
+int bpd_host_kv_append(uint8_t* pages, int64_t num_pages, int32_t page_size, int32_t kv_heads,
+                       int32_t head_dim, int dtype, const void* k, int64_t k_row, int64_t k_token,
+                       int64_t k_head, const void* v, int64_t v_row, int64_t v_token,
+                       int64_t v_head, const void* q, int64_t q_row, int64_t q_token,
+                       int64_t q_head, int32_t heads, void* q_out, int64_t rows, int32_t tokens,
+                       const int32_t* block_table, int64_t table_ld, int32_t table_blocks,
+                       const int32_t* starts, const int32_t* counts, const float* cos,
+                       const float* sin, int64_t positions, int32_t rotary, int interleaved,
+                       int32_t* err);
+int bpd_kv_read(const uint8_t* pages, int64_t num_pages, int32_t page_size, int32_t kv_heads,
+                int32_t head_dim, int dtype, void* k_out, void* v_out, int64_t rows,
+                int32_t tokens, const int32_t* block_table, int64_t table_ld,
+                int32_t table_blocks, const int32_t* starts, const int32_t* counts, int32_t* err,
+                void* stream);
+int bpd_host_kv_read(const uint8_t* pages, int64_t num_pages, int32_t page_size, int32_t kv_heads,
+                     int32_t head_dim, int dtype, void* k_out, void* v_out, int64_t rows,
+                     int32_t tokens, const int32_t* block_table, int64_t table_ld,
+                     int32_t table_blocks, const int32_t* starts, const int32_t* counts,
+                     int32_t* err);
+
+/* bpd_kv_attend: out [rows, tokens, heads, head_dim] (contiguous) =
+ * softmax(scale q k^T) v over the cache, for a block of n = query_lens[b] (cut
+ * to tokens; NULL: tokens) queries q [rows, tokens, heads, head_dim] per
+ * request whose own keys are already appended: query i sees the first
+ * lengths[b] - n + 1 + i tokens, lengths[b] counting the block.  Zeros for a
+ * query that sees nothing and for those past n.  Query head h reads key head
+ * h / (heads / kv_heads).  Softmax statistics and sums in float.  workspace:
+ * bpd_kv_attend_workspace_bytes bytes for `longest` = table_blocks *
+ * page_size, 16-byte aligned (NULL where that is 0). */
+size_t bpd_kv_attend_workspace_bytes(int64_t rows, int32_t tokens, int32_t heads,
+                                     int32_t kv_heads, int32_t head_dim, int64_t longest);
+int bpd_kv_attend(const uint8_t* pages, int64_t num_pages, int32_t page_size, int32_t kv_heads,
+                  int32_t head_dim, int dtype, const void* q, int64_t q_row, int64_t q_token,
+                  int64_t q_head, int32_t heads, void* out, int64_t rows, int32_t tokens,
+                  const int32_t* block_table, int64_t table_ld, int32_t table_blocks,
+                  const int32_t* lengths, const int32_t* query_lens, float scale, void* workspace,
+                  size_t workspace_bytes, int32_t* err, void* stream);
+int bpd_host_kv_attend(const uint8_t* pages, int64_t num_pages, int32_t page_size,
+                       int32_t kv_heads, int32_t head_dim, int dtype, const void* q,
+                       int64_t q_row, int64_t q_token, int64_t q_head, int32_t heads, void* out,
+                       int64_t rows, int32_t tokens, const int32_t* block_table, int64_t table_ld,
+                       int32_t table_blocks, const int32_t* lengths, const int32_t* query_lens,
+                       float scale, int32_t* err);
 
 #ifdef __cplusplus
 }
