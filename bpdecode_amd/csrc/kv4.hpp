@@ -91,14 +91,15 @@ __host__ __device__ __forceinline__ uint32_t kv_code(float x, int32_t e) {
   return c | (x < 0.0f ? 8u : 0u);
 }
 
-// Value of a 4-bit code at scale byte e.  2^(e - 127) is a normal float for
-// every byte that kv_scale_byte gives; byte 0 is read as 0.
+// Value of a 4-bit code at scale byte e, as gfx950 converts it: 2^(e - 127) is
+// a normal float for every byte that kv_scale_byte gives, byte 0 a subnormal
+// one.
 __host__ __device__ __forceinline__ float kv_value(uint32_t code, uint32_t e) {
   if (e == kKvBadScale) return bits_float(0x7FC00000u);
   const uint32_t c = code & 7u;
   // levels: 0, then m * 2^k with m = 1 (even codes) or 1.5 (odd ones above 1)
   const float lv = c < 2 ? 0.5f * float(c) : bits_float((126u + (c >> 1)) << 23) * ((c & 1u) ? 1.5f : 1.0f);
-  return (code & 8u ? -lv : lv) * bits_float(e << 23);
+  return (code & 8u ? -lv : lv) * bits_float(e ? e << 23 : 0x400000u);
 }
 
 // The rotation of a pair by its position's angle, each product and each sum
