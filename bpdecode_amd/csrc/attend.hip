@@ -49,16 +49,16 @@ constexpr int kWaves = 4;   // waves of a block
 constexpr int kNever = 0x7FFFFFFF;
 
 // How a call's work is cut.  A unit is one request, one key head and one group
-// of query columns (tokens x heads that share the key head); its tiles are
-// cut into equal splits of at least kWaves tiles, so that all splits of a call
-// are about as long and there are about `target` of them.  The lengths are on
-// the device, so every wave works the cut out for itself.
+// of query columns (tokens x heads that share the key head); all units' tiles
+// stand in one row, request by request, and every block takes an equal run of
+// them.  A run may end one unit and begin others: a unit that lies in one run
+// is finished by its block, the pieces of the others are joined afterwards.
+// The lengths are on the device, so every wave works the cut out for itself.
 struct AttendPlan {
-  int32_t groups;  // column groups
-  int32_t cols;    // columns of a group, at most 16 * NT
-  int32_t target;  // blocks that fill the device
-  int32_t splits;  // at most this many splits over all requests
-  float* partials;
+  int32_t groups;   // column groups
+  int32_t cols;     // columns of a group, at most 16 * NT
+  int32_t blocks;   // runs that fill the device, 0: one block takes one unit
+  float* partials;  // two pieces per run: of its first unit, of its last
 };
 
 __device__ __forceinline__ int32_t queries_of(const AttendArgs& a, int64_t b) {
@@ -71,8 +71,10 @@ __device__ __forceinline__ int64_t length_of(const AttendArgs& a, int64_t b) {
   const int64_t s = a.lengths[b], room = int64_t(a.table.blocks) * a.page.page_size;
   return s < 0 ? 0 : s < room ? s : room;
 }
+// Tiles of one of its units, one at least: someone has to write the zeros.
 __device__ __forceinline__ int32_t tiles_of(const AttendArgs& a, int64_t b) {
-  return queries_of(a, b) > 0 ? int32_t((length_of(a, b) + kTile - 1) / kTile) : 0;
+  const int32_t n = queries_of(a, b) > 0 ? int32_t((length_of(a, b) + kTile - 1) / kTile) : 0;
+  return n < 1 ? 1 : n;
 }
 
 template <class T>
@@ -81,41 +83,61 @@ __device__ __forceinline__ T wave_sum(T x) {
   return x;
 }
 
-// Tiles that a split has at most, by the whole call's tiles.
-__device__ __forceinline__ int32_t split_tiles(const AttendArgs& a, const AttendPlan& p, int lane) {
-  int64_t whole = 0;
-  for (int64_t b = lane; b < a.rows; b += kWave) whole += tiles_of(a, b);
-  whole = wave_sum(whole) * (a.kv_heads * p.groups);
-  const int64_t per = (whole + p.target - 1) / p.target;
-  return per < kWaves ? kWaves : int32_t(per);
+// A value that all lanes share, or lane `from`'s, in scalar registers.
+__device__ __forceinline__ int32_t scalar(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t scalar(int64_t x) {
+  return int64_t(scalar(int32_t(x >> 32))) << 32 | uint32_t(scalar(int32_t(x)));
 }
-__device__ __forceinline__ int32_t splits_of(int32_t tiles, int32_t most) {
-  return tiles <= most ? 1 : (tiles + most - 1) / most;
+__device__ __forceinline__ int64_t scalar(int64_t x, int from) {
+  return int64_t(__builtin_amdgcn_readlane(int32_t(x >> 32), from)) << 32 |
+         uint32_t(__builtin_amdgcn_readlane(int32_t(x), from));
 }
 
-// The request whose splits hold number `at`, the number of its first split,
-// and its splits; false past the last.
-__device__ __forceinline__ bool find_split(const AttendArgs& a, int32_t most, int32_t at, int lane, int64_t* row,
-                                           int32_t* first, int32_t* splits) {
-  int32_t before = 0;
-  for (int64_t b0 = 0; b0 < a.rows; b0 += kWave) {
-    const int32_t mine = b0 + lane < a.rows ? splits_of(tiles_of(a, b0 + lane), most) : 0;
-    int32_t upto = mine;
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {  // of numbers that are not negative
+  if (((x | y) >> 32) == 0) return scalar(int32_t(uint32_t(x) / uint32_t(y)));
+  return scalar(x / y);
+}
+
+// A request's place in the row of tiles.
+struct Place {
+  int64_t first;  // its first tile
+  int64_t whole;  // tiles of the call
+  int64_t row;
+  int32_t tiles;  // of each of its units
+};
+
+// The request that holds tile `at` (row < 0) or request `row`; `run` becomes
+// the tiles of a run, `at` = run number * run.  False past the last tile.
+__device__ __forceinline__ bool find_place(const AttendArgs& a, const AttendPlan& p, int64_t number, int64_t row,
+                                           int lane, int64_t* run, Place* place) {
+  const int32_t units = a.kv_heads * p.groups;
+  const int32_t mine = lane < a.rows ? tiles_of(a, lane) : 0;
+  int64_t whole = mine;
+  for (int64_t b = lane + kWave; b < a.rows; b += kWave) whole += tiles_of(a, b);
+  whole = scalar(wave_sum(whole));
+  const int64_t per = quotient(whole * units + p.blocks - 1, p.blocks);
+  *run = per < kWaves ? kWaves : per;
+  place->whole = whole * units;
+  const int64_t at = number * *run;
+  if (row < 0 && at >= place->whole) return false;
+  int64_t before = 0;
+  for (int64_t b0 = 0;; b0 += kWave) {
+    const int32_t here = b0 == 0 ? mine : b0 + lane < a.rows ? tiles_of(a, b0 + lane) : 0;
+    int64_t upto = here;
     for (int o = 1; o < kWave; o <<= 1) {
-      const int32_t y = __shfl_up(upto, o);
+      const int64_t y = __shfl_up(upto, o);
       if (lane >= o) upto += y;
     }
-    const uint64_t m = __ballot(before + upto > at);
+    const uint64_t m = __ballot(row < 0 ? (before + upto) * units > at : b0 + lane == row);
     if (m) {
       const int hit = __builtin_ctzll(m);
-      *row = b0 + hit;
-      *splits = __builtin_amdgcn_readlane(mine, hit);
-      *first = before + __builtin_amdgcn_readlane(upto, hit) - *splits;
+      place->row = b0 + hit;
+      place->tiles = __builtin_amdgcn_readlane(here, hit);
+      place->first = (before + scalar(upto, hit) - place->tiles) * units;
       return true;
     }
-    before += __builtin_amdgcn_readlane(upto, kWave - 1);
+    before += scalar(upto, kWave - 1);
   }
-  return false;
 }
 
 // A head's channels as one or two parts of 128, 64 or 32: what 16 lanes take
@@ -177,7 +199,39 @@ __device__ __forceinline__ float scale_at(const uint32_t* w, int at, int words, 
   return bits_float(__builtin_amdgcn_perm(hi, w[i], sel + (uint32_t(o) << 24)) >> 1);
 }
 
-// One block per split of a unit, its tiles dealt to the waves in turn.
+// N neighbouring value tiles from v on of one column, times `inv`, to its head:
+// rows 4 g .. 4 g + 3 of each are channels (width / 16) row + tile of a part.
+template <int DT, int D, int N>
+__device__ __forceinline__ void store_columns(uint16_t* out, int v, int g, const f32x4* x, float inv) {
+  using Pt = Parts<D>;
+  const int p = 16 * v < Pt::first ? 0 : 1, per = p ? Pt::second / 16 : Pt::first / 16;
+  uint16_t* to = out + (p ? Pt::first : 0) + 4 * g * per + (v - (p ? Pt::first / 16 : 0));
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+#pragma unroll
+    for (int k = 0; k < N; k += 2) {
+      if (N == 1)
+        to[r * per] = uint16_t(two_rounded<DT>(x[0][r] * inv, 0.0f));
+      else
+        *reinterpret_cast<uint32_t*>(to + r * per + k) = two_rounded<DT>(x[k][r] * inv, x[k + (N > 1)][r] * inv);
+    }
+}
+
+// Blocks that a CU is to hold, by registers (a block puts one wave on each SIMD).
+constexpr int attend_blocks(int dim, int nt) {
+  if (nt == 1) return dim == 64 ? 4 : dim == 128 ? 3 : 2;
+  if (nt == 2) return dim == 64 ? 3 : dim <= 128 ? 2 : 1;
+  return 1;
+}
+
+// A value that the compiler forms anew here instead of keeping it (or what
+// follows from it) in registers across a loop.
+__device__ __forceinline__ int here(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// One block per run, the tiles of each unit in it dealt to the waves in turn.
 //
 // Scores: with keys as the left operand and queries as the right, a lane holds
 // column n = lane % 16 (a query) and, of each 16 tokens, rows 4 g .. 4 g + 3
@@ -191,60 +245,58 @@ __device__ __forceinline__ float scale_at(const uint32_t* w, int at, int words, 
 // The running maximum is followed loosely: weights may grow to 2^8 before the
 // sums are scaled down, so most tiles cost no exchange between lanes.
 template <int DT, int D, int NT>
-__global__ __launch_bounds__(kWaves* kWave) void kv_attend_kernel(AttendArgs a, AttendPlan plan) {
+__global__ __launch_bounds__(kWaves* kWave, attend_blocks(D, NT)) void kv_attend_kernel(AttendArgs a, AttendPlan plan) {
   using Pt = Parts<D>;
   constexpr int G = D / kKvGroup, KW = D / 32, VT = D / 16;  // scales, key words of a lane, value tiles
   constexpr int kScaleWords = 4 * G;                          // of 16 tokens
-  __shared__ float joined[(kWaves / 2) * (2 + 4 * VT) * kWave];
+  constexpr int kJoin = VT <= kWaves ? kWaves : 2 * kWaves;   // value tiles joined at a time
+  __shared__ f32x4 joined[kWaves][kJoin][kWave];
+  __shared__ float tops[kWaves][kWave], sums[kWaves][kWave];
+  __shared__ Frag queries[NT][KW][kWave];  // as the lanes of every wave take them
 
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int m = lane & 15, g = lane >> 4;
-  int64_t x = blockIdx.x;
-  int32_t group = 0;
-  if (plan.groups > 1) {  // a unit's groups read the same keys: blocks 8 apart, on one XCD
-    const int64_t r = x % (8 * plan.groups);
-    group = int32_t(r / 8);
-    x = x / (8 * plan.groups) * 8 + r % 8;
+  const int32_t share = a.heads / a.kv_heads, units = a.kv_heads * plan.groups;
+  int64_t b, pos = 0, stop, begin = 0;
+  int32_t tiles, unit, tile0 = 0;
+  if (plan.blocks == 0) {
+    b = scalar(int32_t(blockIdx.x / uint32_t(units)));
+    unit = int32_t(blockIdx.x) - int32_t(b) * units;
+    stop = tiles = tiles_of(a, b);
+  } else {
+    int64_t run;
+    Place place;
+    if (!find_place(a, plan, blockIdx.x, -1, lane, &run, &place)) return;
+    begin = pos = run * blockIdx.x;
+    stop = pos + run < place.whole ? pos + run : place.whole;
+    b = place.row;
+    tiles = place.tiles;
+    // (a request's tiles are fewer than 2^31, which the host checks)
+    unit = scalar(int32_t(uint32_t(pos - place.first) / uint32_t(tiles)));
+    tile0 = int32_t(pos - place.first) - unit * tiles;
   }
-  const int32_t at = int32_t(x / a.kv_heads), kvh = int32_t(x % a.kv_heads);
-  const int32_t most = split_tiles(a, plan, lane);
-  int64_t b;
-  int32_t first, splits;
-  if (!find_split(a, most, at, lane, &b, &first, &splits)) return;
 
-  const int32_t n_q = queries_of(a, b), share = a.heads / a.kv_heads;
-  const int64_t end = length_of(a, b);
-  const int32_t tiles = tiles_of(a, b), per = (tiles + splits - 1) / splits;
-  const int32_t tile0 = (at - first) * per, tile1 = tile0 + per < tiles ? tile0 + per : tiles;
-  if (a.err && n_q > 0 && a.lengths[b] > end && threadIdx.x == 0) atomicOr(a.err, BPD_FLAG_PAGE_RANGE);
-
-  // this lane's columns: the queries, and how many tokens each sees
-  Frag q[NT][KW];
-  int32_t sees[NT];
-  int32_t least = int32_t(end);
+  // which of 4 neighbouring scales a lane takes: as a key lane, as a value lane
+  uint32_t ksel[Pt::count], vsel[Pt::count];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int32_t c = group * plan.cols + t * 16 + m;
-    const int32_t i = c / share, h = kvh * share + c % share;
-    const bool in = t * 16 + m < plan.cols && i < n_q;
-    const int64_t s = in ? int64_t(a.lengths[b]) - n_q + 1 + i : 0;
-    sees[t] = int32_t(s < 0 ? 0 : s < end ? s : end);
-    if (in) least = min(least, sees[t]);
-    const uint16_t* row = a.q + b * a.q_row + (in ? i : 0) * a.q_token + (in ? h : 0) * a.q_head;
-#pragma unroll
-    for (int p = 0; p < Pt::count; ++p)
-#pragma unroll
-      for (int k = 0; k < Pt::width(p) / 32; ++k) {
-        const uint16_t* from = row + Pt::begin(p) + g * (Pt::width(p) / 4) + 8 * k;
-        Frag f = {{0u, 0u, 0u, 0u}};
-        if (in) __builtin_memcpy(&f, from, 16);  // at any element
-        q[t][Pt::begin(p) / 32 + k] = f;
-      }
+  for (int p = 0; p < Pt::count; ++p) {
+    ksel[p] = uint32_t(g * Pt::width(p) / 128) << 24 | 0x0C0C0C;
+    vsel[p] = uint32_t(m * Pt::width(p) / 512) << 24 | 0x0C0C0C;
   }
-  for (int o = 1; o < 16; o <<= 1) least = min(least, __shfl_xor(least, o));
-
+  // scores times this are exponents of two; a negative scale turns the queries
+  // around and a scale of zero clears them, so that a larger score stays larger
+  const float to_log2 = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * 1.44269504088896340736f;
   const int32_t P = a.page.page_size;
   const int shift = __builtin_ctz(P);
+
+  for (;;) {
+  const int32_t n_here = int32_t(stop - pos < tiles - tile0 ? stop - pos : tiles - tile0);
+  const int32_t kvh = scalar(unit / plan.groups), group = unit - kvh * plan.groups;
+  const int32_t n_q = queries_of(a, b);
+  const int64_t end = n_q > 0 ? length_of(a, b) : 0;
+  const int32_t tile1 = end > 0 ? tile0 + n_here : tile0;
+  if (a.err && n_q > 0 && a.lengths[b] > end && threadIdx.x == 0) atomicOr(a.err, BPD_FLAG_PAGE_RANGE);
+
   const int32_t* table = a.table.block_table + b * a.table.ld;
   // page of the chunk of 16 tokens that starts at t, -1: none
   const auto page_at = [&](int64_t t) -> int32_t { return t < end ? table[t >> shift] : -1; };
@@ -287,13 +339,50 @@ __global__ __launch_bounds__(kWaves* kWave) void kv_attend_kernel(AttendArgs a, 
       vs[4 * k] = w.x, vs[4 * k + 1] = w.y, vs[4 * k + 2] = w.z, vs[4 * k + 3] = w.w;
     }
   };
-  // which of 4 neighbouring scales a lane takes: as a key lane, as a value lane
-  uint32_t ksel[Pt::count], vsel[Pt::count];
+  int32_t tile = tile0 + wave;
+  int32_t kpage = -1, vpage = -1, knext = -1, vnext = -1;
+  if (tile < tile1) kpage = page_at(int64_t(tile) * kTile + (m >> 2) * 16), vpage = page_at(int64_t(tile) * kTile + g * 16);
+  // this lane's columns: the queries, and how many tokens each sees
+  const int ql = here(lane), qm = ql & 15;
+  Frag q[NT][KW];  // every fourth of them
+  int32_t sees[NT];
+  int32_t least = int32_t(end);
 #pragma unroll
-  for (int p = 0; p < Pt::count; ++p) {
-    ksel[p] = uint32_t(g * Pt::width(p) / 128) << 24 | 0x0C0C0C;
-    vsel[p] = uint32_t(m * Pt::width(p) / 512) << 24 | 0x0C0C0C;
+  for (int t = 0; t < NT; ++t) {
+    const int32_t c = group * plan.cols + t * 16 + qm;
+    const int32_t i = c / share, h = kvh * share + c % share;
+    const bool in = t * 16 + qm < plan.cols && i < n_q;
+    const int64_t s = in ? int64_t(a.lengths[b]) - n_q + 1 + i : 0;
+    sees[t] = int32_t(s < 0 ? 0 : s < end ? s : end);
+    if (in) least = min(least, sees[t]);
+    const uint16_t* row = a.q + b * a.q_row + (in ? i : 0) * a.q_token + (in ? h : 0) * a.q_head;
+#pragma unroll
+    for (int p = 0; p < Pt::count; ++p)
+#pragma unroll
+      for (int k = 0; k < Pt::width(p) / 32; ++k) {
+        const uint16_t* from = row + Pt::begin(p) + (ql >> 4) * (Pt::width(p) / 4) + 8 * k;
+        Frag f = {{0u, 0u, 0u, 0u}};
+        if (in && a.scale != 0.0f && (t * KW + Pt::begin(p) / 32 + k) % kWaves == wave) __builtin_memcpy(&f, from, 16);  // at any element
+        if (a.scale < 0.0f)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) f.u[j] ^= 0x80008000u;
+        q[t][Pt::begin(p) / 32 + k] = f;
+      }
   }
+  if (tile < tile1) {
+    const int64_t t0 = int64_t(tile) * kTile;
+    load_keys(block_at(kpage), int32_t((t0 + 4 * m) & (P - 1)));
+    load_values(block_at(vpage), int32_t((t0 + 16 * g) & (P - 1)));
+    const int64_t t1 = t0 + kWaves * kTile;
+    if (tile + kWaves < tile1) knext = page_at(t1 + (m >> 2) * 16), vnext = page_at(t1 + g * 16);
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int k = 0; k < KW; ++k)
+      if ((t * KW + k) % kWaves == wave) queries[t][k][ql] = q[t][k];
+  __syncthreads();
+  for (int o = 1; o < 16; o <<= 1) least = min(least, __shfl_xor(least, o));
 
   f32x4 acc[NT][VT];
   float top[NT], sum[NT];
@@ -306,80 +395,75 @@ __global__ __launch_bounds__(kWaves* kWave) void kv_attend_kernel(AttendArgs a, 
   int32_t nan_at[Pt::count];  // first token of the tail whose value group is bad, as a value lane
 #pragma unroll
   for (int p = 0; p < Pt::count; ++p) nan_at[p] = kNever;
-  const float to_log2 = a.scale * 1.44269504088896340736f;
-
-  int32_t tile = tile0 + wave;
-  int32_t kpage = -1, vpage = -1, knext = -1, vnext = -1;
-  if (tile < tile1) {
-    const int64_t t0 = int64_t(tile) * kTile;
-    kpage = page_at(t0 + (m >> 2) * 16), vpage = page_at(t0 + g * 16);
-    load_keys(block_at(kpage), int32_t((t0 + 4 * m) & (P - 1)));
-    load_values(block_at(vpage), int32_t((t0 + 16 * g) & (P - 1)));
-    const int64_t t1 = int64_t(tile + kWaves) * kTile;
-    if (tile + kWaves < tile1) knext = page_at(t1 + (m >> 2) * 16), vnext = page_at(t1 + g * 16);
-  }
   for (; tile < tile1; tile += kWaves) {
     const int64_t t0 = int64_t(tile) * kTile, t1 = t0 + kWaves * kTile;
     const bool more = tile + kWaves < tile1;
+    // read anew for every tile: the registers hold loads in flight instead
+    const int q_lane = here(lane);
     f32x4 s[NT][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int t = 0; t < NT; ++t) s[t][j] = f32x4{0, 0, 0, 0};
+      for (int j = 0; j < 4; ++j) s[t][j] = f32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int p = 0; p < Pt::count; ++p) {
-        // the scale of this token's group: byte G j + Pt::begin(p) / 32 + (g's share)
-        const float sc = scale_at(ks, G * j + Pt::begin(p) / kKvGroup, G, ksel[p]);
+    for (int p = 0; p < Pt::count; ++p) {
+      float sc[4];  // of the lane's group of channels, by token
 #pragma unroll
-        for (int k = 0; k < Pt::width(p) / 32; ++k) {
+      for (int j = 0; j < 4; ++j) sc[j] = scale_at(ks, G * j + Pt::begin(p) / kKvGroup, G, ksel[p]);
+#pragma unroll
+      for (int k = 0; k < Pt::width(p) / 32; ++k) {
+        Frag q[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) q[t] = queries[t][Pt::begin(p) / 32 + k][q_lane];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
           const uint32_t w = kc[j][Pt::begin(p) / 32 + k];
           Frag f;
-          f.u[0] = two_values<DT, 0>(w, sc);
-          f.u[1] = two_values<DT, 1>(w, sc);
-          f.u[2] = two_values<DT, 2>(w, sc);
-          f.u[3] = two_values<DT, 3>(w, sc);
+          f.u[0] = two_values<DT, 0>(w, sc[j]);
+          f.u[1] = two_values<DT, 1>(w, sc[j]);
+          f.u[2] = two_values<DT, 2>(w, sc[j]);
+          f.u[3] = two_values<DT, 3>(w, sc[j]);
 #pragma unroll
-          for (int t = 0; t < NT; ++t) s[t][j] = mfma<DT>(f, q[t][Pt::begin(p) / 32 + k], s[t][j]);
+          for (int t = 0; t < NT; ++t) s[t][j] = mfma<DT>(f, q[t], s[t][j]);
         }
       }
     }
     if (more) load_keys(block_at(knext), int32_t((t1 + 4 * m) & (P - 1)));
 
-    // scores in units of log 2; token 16 g + 4 i + j of the tile is s[t][j][i]
-    const int64_t mine = t0 + 16 * g;
+    // token 16 g + 4 i + j of the tile is s[t][j][i]
+    const int32_t mine = int32_t(t0) + 16 * g;
     const bool there = vpage >= 0 && vpage < a.table.num_pages;
     const bool tail = t0 + kTile > least;
     const bool masked = __any(!there || tail);
-    uint32_t quiet[Pt::count] = {};  // value groups that are left out: one bit per token
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[t][j][i] *= to_log2;
     if (masked) {
-      if (!there && mine < end && a.err) atomicOr(a.err, BPD_FLAG_PAGE_RANGE);
+      const int32_t present = there ? int32_t(end) - mine : 0;
+      if (!there && mine < int32_t(end) && a.err) atomicOr(a.err, BPD_FLAG_PAGE_RANGE);
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (!there || mine + 4 * i + j >= sees[t]) s[t][j][i] = -INFINITY;
+            if (4 * i + j >= (there ? sees[t] - mine : 0)) s[t][j][i] = -INFINITY;
       // values that no query or not every query sees: nothing where there is
       // no token, and bad groups are noted, so that a weight of 0 meets no NaN
 #pragma unroll
       for (int u = 0; u < 16; ++u) {
-        const bool gone = !there || mine + u >= end;
+        const bool gone = u >= present;
 #pragma unroll
         for (int p = 0; p < Pt::count; ++p) {
           const int byte = G * u + Pt::begin(p) / kKvGroup;
           const uint32_t e = float_bits(scale_at(vs, byte, kScaleWords, vsel[p])) >> 23;
           if (e == kKvBadScale && !gone && tail) {
-            const int32_t tok = int32_t(mine + u);
-            nan_at[p] = tok < nan_at[p] ? tok : nan_at[p];
+            nan_at[p] = min(nan_at[p], mine + u);
           }
-          if (gone || (e == kKvBadScale && tail)) vc[u][p] = 0, quiet[p] |= 1u << u;
+          if (gone || (e == kKvBadScale && tail)) {  // zeros, at a scale of one
+            vc[u][p] = 0;
+            const uint32_t at_byte = byte % 4 + (vsel[p] >> 24), put = 0xFFu << (8 * (at_byte & 3));
+            if (at_byte < 4) vs[byte / 4] = (vs[byte / 4] & ~put) | (put & 0x7F7F7F7Fu);
+            if (at_byte >= 4 && byte / 4 + 1 < kScaleWords)
+              vs[byte / 4 + 1] = (vs[byte / 4 + 1] & ~put) | (put & 0x7F7F7F7Fu);
+          }
         }
       }
     }
@@ -390,6 +474,7 @@ __global__ __launch_bounds__(kWaves* kWave) void kv_attend_kernel(AttendArgs a, 
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) most_here = fmaxf(most_here, s[t][j][i]);
+      most_here *= to_log2;
       if (__any(most_here > top[t] + 8.0f)) {
         float now = fmaxf(top[t], most_here);
         now = fmaxf(now, __shfl_xor(now, 16));
@@ -406,7 +491,7 @@ __global__ __launch_bounds__(kWaves* kWave) void kv_attend_kernel(AttendArgs a, 
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          s[t][j][i] = __builtin_amdgcn_exp2f(s[t][j][i] - top[t]);
+          s[t][j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][i], to_log2, -top[t]));
           sum[t] += s[t][j][i];
         }
     }
@@ -430,10 +515,8 @@ __global__ __launch_bounds__(kWaves* kWave) void kv_attend_kernel(AttendArgs a, 
           const int u = 8 * h + 2 * k;
           float sc[2];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
+          for (int e = 0; e < 2; ++e)
             sc[e] = scale_at(vs, G * (u + e) + Pt::begin(p) / kKvGroup, kScaleWords, vsel[p]);
-            if (masked) sc[e] = quiet[p] >> (u + e) & 1u ? 1.0f : sc[e];
-          }
           const auto pair = [&](auto byte) {
             constexpr int B = decltype(byte)::value;
             if constexpr (2 * B < kMost) {
@@ -476,129 +559,154 @@ __global__ __launch_bounds__(kWaves* kWave) void kv_attend_kernel(AttendArgs a, 
           for (int i = 0; i < 4; ++i) acc[c][Pt::begin(p) / 16 + v][i] = bits_float(0x7FC00000u);
   }
 
+  // join the waves: each takes its share of the value tiles
+  const int el = here(lane);
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     sum[t] += __shfl_xor(sum[t], 16);
     sum[t] += __shfl_xor(sum[t], 32);
-    // join the waves, the upper half to the lower
-    for (int half = kWaves / 2; half; half /= 2) {
-      float* to = joined + (wave % half) * ((2 + 4 * VT) * kWave) + lane;
+#pragma unroll
+    for (int v0 = 0; v0 < VT; v0 += kJoin) {
+      constexpr int kMine = kJoin / kWaves;
       __syncthreads();
-      if (wave >= half && wave < 2 * half) {
-        to[0] = top[t], to[kWave] = sum[t];
+      if (v0 == 0) tops[wave][el] = top[t], sums[wave][el] = sum[t];
 #pragma unroll
-        for (int v = 0; v < VT; ++v)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) to[(2 + 4 * v + i) * kWave] = acc[t][v][i];
+      for (int v = 0; v < kJoin; ++v) {
+        if (v0 + v < VT) joined[wave][v][el] = acc[t][v0 + v];
       }
       __syncthreads();
-      if (wave < half) {
-        const float other = to[0], now = fmaxf(top[t], other);
-        const float f0 = __builtin_amdgcn_exp2f(top[t] - now), f1 = __builtin_amdgcn_exp2f(other - now);
-        top[t] = now;
-        sum[t] = sum[t] * f0 + to[kWave] * f1;
+      float now = tops[0][el], whole = 0.0f, f[kWaves];
 #pragma unroll
-        for (int v = 0; v < VT; ++v)
+      for (int w = 1; w < kWaves; ++w) now = fmaxf(now, tops[w][el]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[t][v][i] = acc[t][v][i] * f0 + to[(2 + 4 * v + i) * kWave] * f1;
+      for (int w = 0; w < kWaves; ++w) {
+        f[w] = __builtin_amdgcn_exp2f(tops[w][el] - now);
+        whole += sums[w][el] * f[w];
       }
-    }
-    if (wave) continue;
-    if (splits == 1) {
-      const int32_t c = group * plan.cols + t * 16 + m;
-      const int32_t i = c / share, h = kvh * share + c % share;
-      if (t * 16 + m >= plan.cols || i >= a.tokens) continue;
-      uint16_t* out = a.out + ((b * a.tokens + i) * a.heads + h) * D;
-      const float inv = sum[t] == 0.0f ? 0.0f : 1.0f / sum[t];
+      f32x4 mine[kMine];
 #pragma unroll
-      for (int p = 0; p < Pt::count; ++p)
+      for (int k = 0; k < kMine; ++k) {
+        mine[k] = f32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          uint16_t* at_row = out + Pt::begin(p) + (4 * g + r) * (Pt::width(p) / 16);
+        for (int w = 0; w < kWaves; ++w) {
+          const f32x4 y = joined[w][wave * kMine + k][el];
 #pragma unroll
-          for (int v = 0; v < Pt::width(p) / 16; v += 2)
-            *reinterpret_cast<uint32_t*>(at_row + v) =
-                two_rounded<DT>(acc[t][Pt::begin(p) / 16 + v][r] * inv, acc[t][Pt::begin(p) / 16 + v + 1][r] * inv);
+          for (int i = 0; i < 4; ++i) mine[k][i] += y[i] * f[w];
         }
-    } else {
-      float* to = plan.partials + ((int64_t(at) * a.kv_heads + kvh) * plan.groups + group) * (NT * (2 + 4 * VT) * kWave) +
-                  t * ((2 + 4 * VT) * kWave);
-      to[lane] = top[t], to[kWave + lane] = sum[t];
+      }
+      const int v = v0 + wave * kMine;  // the first of the wave's value tiles
+      if (v >= VT) continue;
+      const int32_t column = t * 16 + (el & 15);
+      if (n_here == tiles) {
+        const int32_t c = group * plan.cols + column;
+        const int32_t i = c / share, h = kvh * share + c % share;
+        if (column >= plan.cols || i >= a.tokens) continue;
+        store_columns<DT, D, kMine>(a.out + ((b * a.tokens + i) * a.heads + h) * D, v, el >> 4, mine,
+                                    whole == 0.0f ? 0.0f : 1.0f / whole);
+      } else {
+        const int64_t piece = 2 * int64_t(blockIdx.x) + (pos == begin ? 0 : 1);
+        float* to = plan.partials + (piece * NT + t) * ((2 + 4 * VT) * kWave);
+        if (v == 0) to[el] = now, to[kWave + el] = whole;
 #pragma unroll
-      for (int v = 0; v < VT; ++v)
-        *reinterpret_cast<f32x4*>(to + 2 * kWave + (v * kWave + lane) * 4) = acc[t][v];
+        for (int k = 0; k < kMine; ++k)
+          if (v + k < VT) *reinterpret_cast<f32x4*>(to + 2 * kWave + ((v + k) * kWave + el) * 4) = mine[k];
+      }
     }
+  }
+  pos += n_here;
+  if (pos >= stop) break;
+  tile0 = 0;
+  if (++unit == units) unit = 0, tiles = tiles_of(a, ++b);
+  __syncthreads();
   }
 }
 
-// Joins a unit's splits: one block per unit, column tile and pair of value
-// tiles, its waves over the splits.
+// Joins the pieces of a unit that lies in several runs: one block per unit,
+// column tile and pair of value tiles, its waves over the pieces.
 template <int DT, int D, int NT>
 __global__ __launch_bounds__(kWaves* kWave) void kv_attend_join_kernel(AttendArgs a, AttendPlan plan) {
-  using Pt = Parts<D>;
-  constexpr int VT = D / 16, kPiece = (2 + 4 * VT) * kWave;
-  __shared__ float joined[kWaves][10][kWave];
-  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int m = lane & 15, g = lane >> 4;
-  int64_t x = blockIdx.x;
+  constexpr int VT = D / 16, kPiece = (2 + 4 * VT) * kWave, kAtOnce = 4;
+  __shared__ f32x4 joined[kWaves][2][kWave];
+  __shared__ float tops[kWaves][kWave], sums[kWaves][kWave];
+  const int lane = threadIdx.x % kWave, wave = scalar(int32_t(threadIdx.x / kWave));
+  uint32_t x = blockIdx.x;
   const int v0 = int(x % (VT / 2)) * 2;
   x /= VT / 2;
   const int t = int(x % NT);
   x /= NT;
-  const int32_t group = int32_t(x % plan.groups);
-  x /= plan.groups;
-  const int32_t kvh = int32_t(x % a.kv_heads);
-  const int64_t b = x / a.kv_heads;
-  const int32_t most = split_tiles(a, plan, lane);
-  const int32_t splits = splits_of(tiles_of(a, b), most);
-  if (splits == 1) return;
-  int32_t first = 0;
-  for (int64_t r = lane; r < b; r += kWave) first += splits_of(tiles_of(a, r), most);
-  first = wave_sum(first);
-  const float* from = plan.partials + ((int64_t(first) * a.kv_heads + kvh) * plan.groups + group) * (NT * kPiece) + t * kPiece;
-  const int64_t step = int64_t(a.kv_heads) * plan.groups * (NT * kPiece);
+  const int32_t units = a.kv_heads * plan.groups;
+  const int32_t unit = scalar(int32_t(x % uint32_t(units)));
+  const int64_t b = scalar(int32_t(x / uint32_t(units)));
+  int64_t run;
+  Place place;
+  find_place(a, plan, 0, b, lane, &run, &place);
+  const int64_t begin = place.first + int64_t(unit) * place.tiles;
+  const int64_t run0 = quotient(begin, run), run1 = quotient(begin + place.tiles - 1, run);
+  if (run0 == run1) return;
   float top = -3e38f, sum = 0.0f;
   f32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-  for (int32_t i = wave; i < splits; i += kWaves) {
-    const float* p = from + i * step;
-    const float other = p[lane], now = fmaxf(top, other);
-    const float f0 = __builtin_amdgcn_exp2f(top - now), f1 = __builtin_amdgcn_exp2f(other - now);
+  for (int64_t i0 = run0 + wave; i0 <= run1; i0 += kWaves * kAtOnce) {
+    float m[kAtOnce], l[kAtOnce];
+    f32x4 y[kAtOnce][2];
+#pragma unroll
+    for (int n = 0; n < kAtOnce; ++n) {
+      const int64_t i = i0 + n * kWaves;
+      m[n] = -3e38f, l[n] = 0.0f, y[n][0] = y[n][1] = f32x4{0, 0, 0, 0};
+      if (i > run1) continue;
+      const float* p = plan.partials + ((2 * i + (i == run0 && begin != run0 * run ? 1 : 0)) * NT + t) * kPiece;
+      m[n] = p[lane], l[n] = p[kWave + lane];
+#pragma unroll
+      for (int v = 0; v < 2; ++v) y[n][v] = *reinterpret_cast<const f32x4*>(p + 2 * kWave + ((v0 + v) * kWave + lane) * 4);
+    }
+    float now = top;
+#pragma unroll
+    for (int n = 0; n < kAtOnce; ++n) now = fmaxf(now, m[n]);
+    const float keep = __builtin_amdgcn_exp2f(top - now);
     top = now;
-    sum = sum * f0 + p[kWave + lane] * f1;
+    sum *= keep;
 #pragma unroll
-    for (int v = 0; v < 2; ++v) {
-      const f32x4 y = *reinterpret_cast<const f32x4*>(p + 2 * kWave + ((v0 + v) * kWave + lane) * 4);
+    for (int v = 0; v < 2; ++v)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) acc[v][k] = acc[v][k] * f0 + y[k] * f1;
+      for (int k = 0; k < 4; ++k) acc[v][k] *= keep;
+#pragma unroll
+    for (int n = 0; n < kAtOnce; ++n) {
+      const float f = __builtin_amdgcn_exp2f(m[n] - now);
+      sum += l[n] * f;
+#pragma unroll
+      for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[v][k] += y[n][v][k] * f;
     }
   }
-  joined[wave][0][lane] = top, joined[wave][1][lane] = sum;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) joined[wave][2 + k][lane] = acc[0][k], joined[wave][6 + k][lane] = acc[1][k];
+  tops[wave][lane] = top, sums[wave][lane] = sum, joined[wave][0][lane] = acc[0], joined[wave][1][lane] = acc[1];
   __syncthreads();
   if (wave) return;
+  float now = top;
+#pragma unroll
+  for (int w = 1; w < kWaves; ++w) now = fmaxf(now, tops[w][lane]);
+  const float keep = __builtin_amdgcn_exp2f(top - now);
+  sum *= keep;
+#pragma unroll
+  for (int v = 0; v < 2; ++v)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[v][k] *= keep;
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) {
-    const float other = joined[w][0][lane], now = fmaxf(top, other);
-    const float f0 = __builtin_amdgcn_exp2f(top - now), f1 = __builtin_amdgcn_exp2f(other - now);
-    top = now;
-    sum = sum * f0 + joined[w][1][lane] * f1;
+    const float f = __builtin_amdgcn_exp2f(tops[w][lane] - now);
+    sum += sums[w][lane] * f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      acc[0][k] = acc[0][k] * f0 + joined[w][2 + k][lane] * f1;
-      acc[1][k] = acc[1][k] * f0 + joined[w][6 + k][lane] * f1;
+    for (int v = 0; v < 2; ++v) {
+      const f32x4 y = joined[w][v][lane];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[v][k] += y[k] * f;
     }
   }
-  const int32_t share = a.heads / a.kv_heads, c = group * plan.cols + t * 16 + m;
-  const int32_t i = c / share, h = kvh * share + c % share;
-  if (t * 16 + m >= plan.cols || i >= a.tokens) return;
-  uint16_t* out = a.out + ((b * a.tokens + i) * a.heads + h) * D;
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  const int p = v0 * 16 < Pt::first ? 0 : 1;
-#pragma unroll
-  for (int r = 0; r < 4; ++r)
-    *reinterpret_cast<uint32_t*>(out + Pt::begin(p) + (4 * g + r) * (Pt::width(p) / 16) + v0 - Pt::begin(p) / 16) =
-        two_rounded<DT>(acc[0][r] * inv, acc[1][r] * inv);
+  const int32_t share = a.heads / a.kv_heads, column = t * 16 + (lane & 15);
+  const int32_t c = unit % plan.groups * plan.cols + column;
+  const int32_t i = c / share, h = unit / plan.groups * share + c % share;
+  if (column >= plan.cols || i >= a.tokens) return;
+  store_columns<DT, D, 2>(a.out + ((b * a.tokens + i) * a.heads + h) * D, v0, lane >> 4, acc,
+                          sum == 0.0f ? 0.0f : 1.0f / sum);
 }
 
 // Column tiles of a wave: every query column of a key head where they fit.
@@ -609,34 +717,45 @@ constexpr int most_tiles(int dim) { return dim > 128 ? 2 : 4; }
 struct AttendSizes {
   AttendPlan plan;
   int32_t nt;
-  size_t piece;  // floats of one split's partial result
+  int64_t tiles;  // at most, over all units
+  int32_t blocks;  // that the device holds at a time
+  size_t piece;   // floats of a unit's piece
 };
+
+constexpr int kCus = 256;
+constexpr int kShort = 16, kMiddling = 64;  // tiles of a unit
 
 AttendSizes attend_sizes(int64_t rows, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t dim, int64_t longest) {
   AttendSizes z{};
   const int64_t cols = int64_t(tokens) * (heads / kv_heads);
-  const int64_t tiles = (cols + 15) / 16, most = most_tiles(dim);
-  z.nt = tiles <= 1 ? 1 : tiles <= 2 || most == 2 ? 2 : 4;
-  z.plan.groups = int32_t((tiles + z.nt - 1) / z.nt);
+  const int64_t col_tiles = (cols + 15) / 16, most = most_tiles(dim);
+  z.nt = col_tiles <= 1 ? 1 : col_tiles <= 2 || most == 2 ? 2 : 4;
+  z.plan.groups = int32_t((col_tiles + z.nt - 1) / z.nt);
   z.plan.cols = int32_t((cols + z.plan.groups - 1) / z.plan.groups);
-  z.plan.target = 2048;
-  const int64_t units = int64_t(kv_heads) * z.plan.groups;
-  // at least kWaves tiles each, and about `target` over all units
-  const int64_t per_row = ((longest + kTile - 1) / kTile + kWaves - 1) / kWaves;
-  const int64_t by_length = rows * (per_row < 1 ? 1 : per_row), by_target = z.plan.target / units + 1 + rows;
-  z.plan.splits = int32_t(std::min(by_length, by_target));
+  const int64_t per_unit = std::max<int64_t>(1, (std::min<int64_t>(longest, 0x7FFFFFFF) + kTile - 1) / kTile);
+  z.tiles = per_unit * kv_heads * z.plan.groups;
+  z.blocks = kCus * attend_blocks(dim, z.nt);
+  // one block per unit where that fills half the device with units of a
+  // middling length, or where units are short: nothing is searched or joined
+  const int64_t units = rows * kv_heads * z.plan.groups;
+  z.plan.blocks = per_unit <= kShort || (per_unit <= kMiddling && 2 * units >= z.blocks) ? 0 : z.blocks;
   z.piece = size_t(z.nt) * (2 + dim / 4) * kWave;
   return z;
 }
 
+// Runs that a call can have: each of kWaves tiles at least.
+int64_t attend_runs(const AttendSizes& z, int64_t rows) {
+  const int64_t runs = (z.tiles + kWaves - 1) / kWaves * rows;
+  return runs < z.plan.blocks ? runs : z.plan.blocks;
+}
+
 template <int DT, int D, int NT>
 int launch_attend(const AttendArgs& a, const AttendSizes& z, hipStream_t s) {
-  const int64_t units = int64_t(z.plan.splits) * a.kv_heads;
-  const int64_t blocks = z.plan.groups == 1 ? units : (units + 7) / 8 * 8 * z.plan.groups;
   const int64_t joins = a.rows * a.kv_heads * z.plan.groups * NT * (D / 32);
-  BPD_REQUIRE(blocks < (int64_t(1) << 31) && joins < (int64_t(1) << 31), "too many queries in one call");
+  BPD_REQUIRE(z.tiles < (int64_t(1) << 31) && joins < (int64_t(1) << 31), "too many queries or tokens in one call");
+  const int64_t blocks = z.plan.blocks ? attend_runs(z, a.rows) : a.rows * a.kv_heads * z.plan.groups;
   kv_attend_kernel<DT, D, NT><<<uint32_t(blocks), kWaves * kWave, 0, s>>>(a, z.plan);
-  if (z.plan.splits > a.rows) kv_attend_join_kernel<DT, D, NT><<<uint32_t(joins), kWaves * kWave, 0, s>>>(a, z.plan);
+  if (z.plan.blocks) kv_attend_join_kernel<DT, D, NT><<<uint32_t(joins), kWaves * kWave, 0, s>>>(a, z.plan);
   BPD_LAUNCHED();
   return BPD_OK;
 }
@@ -719,6 +838,7 @@ int check_attend(const AttendArgs& a, int dtype) {
   BPD_REQUIRE(std::isfinite(a.scale), "the scale must be finite");
   BPD_REQUIRE(a.rows * int64_t(a.tokens) == 0 || (a.q && a.out && a.lengths), "null pointer argument");
   BPD_REQUIRE(a.table.block_table || a.table.blocks == 0 || a.rows == 0, "null block table");
+  BPD_REQUIRE((reinterpret_cast<uintptr_t>(a.out) & 3u) == 0, "the output must lie at a multiple of 4 bytes");
   BPD_REQUIRE(a.rows * int64_t(a.tokens) * a.heads < (int64_t(1) << 31), "too many queries in one call");
   return BPD_OK;
 }
@@ -739,7 +859,7 @@ extern "C" size_t bpd_kv_attend_workspace_bytes(int64_t rows, int32_t tokens, in
                                                 int32_t head_dim, int64_t longest) {
   if (rows <= 0 || tokens <= 0 || kv_heads <= 0 || heads < kv_heads) return 0;
   const AttendSizes z = attend_sizes(rows, tokens, heads, kv_heads, head_dim, longest);
-  return z.plan.splits > rows ? size_t(z.plan.splits) * kv_heads * z.plan.groups * z.piece * sizeof(float) : 0;
+  return 2 * size_t(attend_runs(z, rows)) * z.piece * sizeof(float);
 }
 
 extern "C" int bpd_kv_attend(const uint8_t* pages, int64_t num_pages, int32_t page_size, int32_t kv_heads,
@@ -755,7 +875,7 @@ extern "C" int bpd_kv_attend(const uint8_t* pages, int64_t num_pages, int32_t pa
   const int64_t longest = int64_t(table_blocks) * page_size;
   AttendSizes z = attend_sizes(rows, tokens, heads, kv_heads, head_dim, longest);
   BPD_REQUIRE(workspace_bytes >= bpd_kv_attend_workspace_bytes(rows, tokens, heads, kv_heads, head_dim, longest) &&
-                  (workspace || z.plan.splits <= rows),
+                  (workspace || z.plan.blocks == 0),
               "the workspace is smaller than bpd_kv_attend_workspace_bytes");
   z.plan.partials = static_cast<float*>(workspace);
   return dtype == BPD_DTYPE_BF16 ? launch_attend_dim<BPD_DTYPE_BF16>(a, z, as_stream(stream))
