@@ -169,28 +169,6 @@ __device__ __forceinline__ f32x4 mfma(const Frag& x, const Frag& y, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(x.h, y.h, c, 0, 0, 0);
 }
 
-// Two codes (byte B of w) times a scale, as two elements of the type: exact.
-template <int DT, int B>
-__device__ __forceinline__ uint32_t two_values(uint32_t w, float s) {
-  if constexpr (DT == BPD_DTYPE_BF16)
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, B));
-  else
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, B));
-}
-
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-template <int DT>
-__device__ __forceinline__ uint32_t two_rounded(float x, float y) {
-  if constexpr (DT == BPD_DTYPE_BF16) {
-    const bf16x2 r = {static_cast<__bf16>(x), static_cast<__bf16>(y)};
-    return __builtin_bit_cast(uint32_t, r);
-  } else {
-    const f16x2 r = {static_cast<_Float16>(x), static_cast<_Float16>(y)};
-    return __builtin_bit_cast(uint32_t, r);
-  }
-}
-
 // Byte `at` + `lane_at` of an array of words as a power of two (the float
 // whose exponent it is); lane_at < 4 differs between lanes.
 __device__ __forceinline__ float scale_at(const uint32_t* w, int at, int words, uint32_t sel) {

@@ -102,6 +102,29 @@ __host__ __device__ __forceinline__ float kv_value(uint32_t code, uint32_t e) {
   return (code & 8u ? -lv : lv) * bits_float(e ? e << 23 : 0x400000u);
 }
 
+// Two codes (byte B of w) times a scale, as two elements of the type: exact.
+template <int DT, int B>
+__device__ __forceinline__ uint32_t two_values(uint32_t w, float s) {
+  if constexpr (DT == BPD_DTYPE_BF16)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, B));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, B));
+}
+
+// Two floats as two elements, rounded to nearest even.
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+template <int DT>
+__device__ __forceinline__ uint32_t two_rounded(float x, float y) {
+  if constexpr (DT == BPD_DTYPE_BF16) {
+    const bf16x2 r = {static_cast<__bf16>(x), static_cast<__bf16>(y)};
+    return __builtin_bit_cast(uint32_t, r);
+  } else {
+    const f16x2 r = {static_cast<_Float16>(x), static_cast<_Float16>(y)};
+    return __builtin_bit_cast(uint32_t, r);
+  }
+}
+
 // The rotation of a pair by its position's angle, each product and each sum
 // rounded by itself (no fused multiply-add), so that the codes that follow
 // from it do not depend on how a compiler joins them.
@@ -141,7 +164,7 @@ struct KvTable {
   int64_t num_pages;
   __host__ __device__ __forceinline__ int64_t page_of(int64_t row, int64_t pos, int32_t page_size) const {
     if (pos < 0 || pos >= int64_t(blocks) * page_size) return -1;
-    const int32_t page = block_table[row * ld + pos / page_size];
+    const int32_t page = block_table[row * ld + (pos >> __builtin_ctz(uint32_t(page_size)))];
     return page >= 0 && page < num_pages ? page : -1;
   }
 };
