@@ -18,8 +18,6 @@ stands, so a block whose drafts were refused is overwritten by the next one.
 
 from __future__ import annotations
 
-import math
-
 import torch
 
 from . import _lib
@@ -34,10 +32,6 @@ _CODES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16}
 def block_bytes(page_size: int, head_dim: int) -> int:
     """Bytes of one page of one key/value head."""
     return page_size * (head_dim + 2 * (head_dim // GROUP))
-
-
-def _unit_channels(x: torch.Tensor) -> torch.Tensor:
-    return x if x.stride(3) == 1 else x.contiguous()
 
 
 class PagedKV4:
@@ -82,30 +76,39 @@ class PagedKV4:
         return cls(pages, page_size, head_dim, dtype, torch.zeros(1, dtype=torch.int32, device=pages.device))
 
     # --- arguments ---------------------------------------------------------
-    def _block(self, x: torch.Tensor, name: str, heads: int | None = None) -> torch.Tensor:
-        if x.dim() != 4 or x.shape[3] != self.head_dim or (heads is not None and x.shape[2] != heads):
+    def _block(self, x: torch.Tensor, name: str, heads: int | None = None) -> tuple[torch.Tensor, tuple]:
+        """``x`` with its channels next to each other, and its address and strides."""
+        shape = x.shape
+        if len(shape) != 4 or shape[3] != self.head_dim or (heads is not None and shape[2] != heads):
             raise RuntimeError(f"{name} must be [requests, tokens, {heads or 'heads'}, {self.head_dim}], "
-                               f"got {list(x.shape)}")
-        if x.dtype != self.dtype or x.device != self.device:
+                               f"got {list(shape)}")
+        if x.dtype is not self.dtype or x.device != self.device:
             raise RuntimeError(f"{name} must be {self.dtype} on {self.device}, got {x.dtype} on {x.device}")
-        return _unit_channels(x)
+        a, b, c, d = x.stride()
+        if d != 1:
+            x = x.contiguous()
+            a, b, c, d = x.stride()
+        return x, (x.data_ptr(), a, b, c)
 
     def _table(self, block_table: torch.Tensor, rows: int) -> tuple[torch.Tensor, tuple]:
-        if block_table.dim() != 2 or block_table.shape[0] != rows:
-            raise RuntimeError(f"block_table must be [{rows}, blocks], got {list(block_table.shape)}")
-        if block_table.dtype != torch.int32 or block_table.device != self.device:
+        shape = block_table.shape
+        if len(shape) != 2 or shape[0] != rows:
+            raise RuntimeError(f"block_table must be [{rows}, blocks], got {list(shape)}")
+        if block_table.dtype is not torch.int32 or block_table.device != self.device:
             raise RuntimeError(f"block_table must be int32 on {self.device}")
-        n = block_table.shape[1]
-        if n > 1 and block_table.stride(1) != 1 or rows > 1 and block_table.stride(0) < n:
+        n = shape[1]
+        ld, unit = block_table.stride()
+        if n > 1 and unit != 1 or rows > 1 and ld < n:
             block_table = block_table.contiguous()
-        return block_table, (block_table.data_ptr(), block_table.stride(0) if rows > 1 else n, n)
+            ld = n
+        return block_table, (block_table.data_ptr(), ld if rows > 1 else n, n)
 
     def _per_request(self, x: torch.Tensor | None, name: str, rows: int) -> torch.Tensor | None:
         if x is None:
             return None
-        if x.shape != (rows,) or x.dtype != torch.int32 or x.device != self.device:
+        if x.dtype is not torch.int32 or x.dim() != 1 or x.shape[0] != rows or x.device != self.device:
             raise RuntimeError(f"{name} must be int32 [{rows}] on {self.device}")
-        return x if x.stride(0) == 1 or rows <= 1 else x.contiguous()
+        return x if rows <= 1 or x.stride(0) == 1 else x.contiguous()
 
     # --- operators -----------------------------------------------------------
     def append(self, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, starts: torch.Tensor, *,
@@ -120,8 +123,9 @@ class PagedKV4:
         (2j, 2j + 1) with ``interleaved``.  Returns the rotated ``q`` (zeros
         past ``counts[b]``), None without ``q``.  Two requests must not append
         to one page in one call."""
-        k, v = self._block(k, "k", self.kv_heads), self._block(v, "v", self.kv_heads)
-        B, T = k.shape[:2]
+        k, ks = self._block(k, "k", self.kv_heads)
+        v, vs = self._block(v, "v", self.kv_heads)
+        B, T, _, _ = k.shape
         if v.shape != k.shape:
             raise RuntimeError(f"k and v differ in shape: {list(k.shape)} and {list(v.shape)}")
         block_table, table = self._table(block_table, B)
@@ -130,24 +134,23 @@ class PagedKV4:
         if (cos is None) != (sin is None):
             raise RuntimeError("the rotation needs both cos and sin")
         if cos is not None:
-            if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32 \
-                    or cos.device != self.device or sin.device != self.device:
+            if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype is not torch.float32 \
+                    or sin.dtype is not torch.float32 or cos.device != self.device or sin.device != self.device:
                 raise RuntimeError(f"cos and sin must be float32 [positions, R / 2] on {self.device}")
             cos, sin = cos.contiguous(), sin.contiguous()
-            positions, rotary = cos.shape[0], 2 * cos.shape[1]
+            positions, rotary = cos.shape
+            rotary *= 2
             if rotary > self.head_dim:
                 raise RuntimeError(f"{rotary} rotated channels in heads of {self.head_dim}")
         out, heads, qs = None, 0, (None, 0, 0, 0)
         if q is not None:
-            q = self._block(q, "q")
-            heads = q.shape[2]
-            if q.shape[:2] != k.shape[:2]:
+            q, qs = self._block(q, "q")
+            rows, tokens, heads, _ = q.shape
+            if rows != B or tokens != T:
                 raise RuntimeError(f"q and k differ in requests or tokens: {list(q.shape)} and {list(k.shape)}")
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            qs = (q.data_ptr(), q.stride(0), q.stride(1), q.stride(2))
-        args = (*self._head, k.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
-                v.data_ptr(), v.stride(0), v.stride(1), v.stride(2), *qs, heads, ptr(out), B, T, *table,
-                ptr(starts), ptr(counts), ptr(cos), ptr(sin), positions, rotary, int(interleaved), ptr(self.err))
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        args = (*self._head, *ks, *vs, *qs, heads, ptr(out), B, T, *table, ptr(starts), ptr(counts), ptr(cos), ptr(sin),
+                positions, rotary, int(interleaved), ptr(self.err))
         if self._on_dev:
             check(lib().bpd_kv_append(*args, _lib.stream_of(self.device)))
         else:
@@ -162,7 +165,7 @@ class PagedKV4:
         B = starts.shape[0] if starts.dim() == 1 else -1
         block_table, table = self._table(block_table, B)
         starts, counts = self._per_request(starts, "starts", B), self._per_request(counts, "counts", B)
-        k = torch.empty((B, tokens, self.kv_heads, self.head_dim), dtype=self.dtype, device=self.device)
+        k = self.pages.new_empty((B, tokens, self.kv_heads, self.head_dim), dtype=self.dtype)
         v = torch.empty_like(k)
         args = (*self._head, k.data_ptr(), v.data_ptr(), B, tokens, *table, ptr(starts), ptr(counts), ptr(self.err))
         if self._on_dev:
@@ -180,18 +183,18 @@ class PagedKV4:
         ``lengths`` counting the block itself.  Query head h reads key head
         ``h // (heads // kv_heads)``; ``scale`` defaults to 1 / sqrt(head_dim).
         Zeros where a query sees nothing and past n."""
-        q = self._block(q, "q")
+        q, qs = self._block(q, "q")
         B, T, H, D = q.shape
         if H < 1 or H % self.kv_heads:
             raise RuntimeError(f"query heads ({H}) must be a multiple of the cache's heads ({self.kv_heads})")
         block_table, table = self._table(block_table, B)
         lengths, query_lens = self._per_request(lengths, "lengths", B), self._per_request(query_lens, "query_lens", B)
-        out = torch.empty((B, T, H, D), dtype=q.dtype, device=q.device)
-        args = (*self._head, q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), H, out.data_ptr(), B, T, *table,
-                ptr(lengths), ptr(query_lens), 1.0 / math.sqrt(D) if scale is None else float(scale))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        args = (*self._head, *qs, H, out.data_ptr(), B, T, *table, ptr(lengths), ptr(query_lens),
+                D ** -0.5 if scale is None else float(scale))
         if self._on_dev:
-            need = int(lib().bpd_kv_attend_workspace_bytes(B, T, H, self.kv_heads, D, table[2] * self.page_size))
-            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+            need = lib().bpd_kv_attend_workspace_bytes(B, T, H, self.kv_heads, D, table[2] * self.page_size)
+            ws = self.pages.new_empty(need) if need else None
             check(lib().bpd_kv_attend(*args, ptr(ws), need, ptr(self.err), _lib.stream_of(self.device)))
         else:
             check(lib().bpd_host_kv_attend(*args, ptr(self.err)))

@@ -836,14 +836,15 @@ def dense_verify(logits, draft_tokens, uniforms, *, draft_probs=None, draft_lens
         raise RuntimeError("logits must be [batch, drafts + 1, vocab], draft_tokens [batch, drafts], "
                            "uniforms [batch, drafts + 1]")
     B, T = draft_tokens.shape
-    if logits.shape[:2] != (B, T + 1) or uniforms.shape != (B, T + 1):
+    rows, positions, columns = logits.shape
+    if rows != B or positions != T + 1 or uniforms.shape != (B, T + 1):
         raise RuntimeError(f"{T} drafted tokens of {B} requests need logits and uniforms at {T + 1} positions, "
                            f"got {list(logits.shape)} and {list(uniforms.shape)}")
     if T > _lib.MAX_DRAFTS:
         raise RuntimeError(f"at most {_lib.MAX_DRAFTS} drafted tokens, got {T}")
-    V = vocab if vocab is not None else logits.shape[2] if tok_next is None else tok_next.shape[1]
-    if not 1 <= V <= logits.shape[2]:
-        raise RuntimeError(f"logits have {logits.shape[2]} columns for a vocabulary of {V} tokens")
+    V = vocab if vocab is not None else columns if tok_next is None else tok_next.shape[1]
+    if not 1 <= V <= columns:
+        raise RuntimeError(f"logits have {columns} columns for a vocabulary of {V} tokens")
     if uniforms.dtype != torch.float32:
         raise RuntimeError("uniforms must be float32")
     if tok_next is not None and (tok_next.dim() != 2 or tok_next.shape[1] != V):
@@ -856,8 +857,10 @@ def dense_verify(logits, draft_tokens, uniforms, *, draft_probs=None, draft_lens
     dev = _same_device(logits, draft_tokens, uniforms, draft_probs, draft_lens, temp, tok_next, allow_bits, bit_rows,
                        states, slots)
     code = _lib.dtype_code(logits.dtype)
-    if logits.stride(2) != 1:
+    z_row, z_pos, unit = logits.stride()
+    if unit != 1:
         logits = logits.contiguous()
+        z_row, z_pos, _ = logits.stride()
     tk = draft_tokens if draft_tokens.dtype in (torch.int32, torch.int64) else draft_tokens.to(torch.int64)
     if T > 1 and tk.stride(1) != 1:
         tk = tk.contiguous()
@@ -868,10 +871,12 @@ def dense_verify(logits, draft_tokens, uniforms, *, draft_probs=None, draft_lens
         if draft_probs.dim() != 3 or draft_probs.shape[:2] != (B, T) or draft_probs.shape[2] < V:
             raise RuntimeError(f"draft_probs must be [{B}, {T}, at least {V}], got {list(draft_probs.shape)}")
         pcode = _lib.dtype_code(draft_probs.dtype)
-        if draft_probs.stride(2) != 1:
+        q_row, q_pos, unit = draft_probs.stride()
+        if unit != 1:
             draft_probs = draft_probs.contiguous()
+            q_row, q_pos, _ = draft_probs.stride()
         if T:
-            probs = (draft_probs.data_ptr(), pcode, draft_probs.stride(0), draft_probs.stride(1))
+            probs = (draft_probs.data_ptr(), pcode, q_row, q_pos)
     if draft_lens is not None:
         if draft_lens.shape != (B,):
             raise RuntimeError("one draft length per request")
@@ -908,16 +913,15 @@ def dense_verify(logits, draft_tokens, uniforms, *, draft_probs=None, draft_lens
         bit_rows = _i32(bit_rows)
     if write_back and tok_next is None:
         raise RuntimeError("states are advanced through tok_next only")
-    out = torch.empty((3, B), dtype=torch.int32, device=dev)
-    n, token, state = out.unbind(0)
-    args = (logits.data_ptr(), code, B, T, V, logits.stride(0), logits.stride(1), tk.data_ptr() if T else None,
+    n, token, state = logits.new_empty((3, B), dtype=torch.int32).unbind(0)
+    args = (logits.data_ptr(), code, B, T, V, z_row, z_pos, tk.data_ptr() if T else None,
             _lib.index_code(tk.dtype), tk.stride(0), ptr(draft_lens), *probs, uniforms.data_ptr(), uniforms.stride(0),
             ptr(temp), 0.0 if temp is not None else float(temperature), ptr(allow_bits), words, S, ptr(tok_next),
             ptr(states) if tok_next is not None else None, ptr(sl), ptr(bit_rows), int(write_back), n.data_ptr(),
             token.data_ptr(), state.data_ptr() if tok_next is not None else None)
     if dev.type == "cuda":
-        need = int(lib().bpd_verify_workspace_bytes(B, T, V))
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        need = lib().bpd_verify_workspace_bytes(B, T, V)
+        ws = logits.new_empty(need, dtype=torch.uint8)
         check(lib().bpd_verify(*args, ptr(ws), need, ptr(err), _lib.stream_of(dev)))
     else:
         check(lib().bpd_host_verify(*args, ptr(err)))
