@@ -187,7 +187,8 @@ constexpr int kLongRuns = 4, kShortRuns = 1;
 constexpr double kLog2E = 1.4426950408889634;
 // Of the 32-bit sum: an exponent y is off by 3 * 2^-24 |y| (the difference, the
 // factor and their product rounded), and at least half of the mass lies at
-// y > -18, the share of one of 2^18 tokens; 38 roundings of the sum add 2^-19.
+// y > -18, the share of one of 2^18 tokens; a lane's 128 terms and their joining
+// add 2^-18 at most, if every rounding goes the same way.
 constexpr double kSumError = 5e-6;
 // What tokens near their border may move of the whole, if all of them lie on
 // the wrong side by all of kSumError.
@@ -261,20 +262,22 @@ __device__ __forceinline__ double exp2_down(double y) {
 
 typedef uint32_t words4 __attribute__((ext_vector_type(4), aligned(2)));
 
-// kRun neighbouring elements; any alignment of the type's own.
+// kRun neighbouring elements as they lie in memory; any alignment of the type's
+// own.
 template <int DT>
-__device__ __forceinline__ void load_run(const void* from, int64_t t, float (&z)[kRun]) {
-  if constexpr (DT == BPD_DTYPE_F32) {
-    __builtin_memcpy(z, static_cast<const float*>(from) + t, sizeof(z));
-  } else {
-    const words4 w = *reinterpret_cast<const words4*>(static_cast<const uint16_t*>(from) + t);
+struct Raw {
+  words4 w[DT == BPD_DTYPE_F32 ? 2 : 1];
+};
+template <int DT>
+__device__ __forceinline__ void unpack(const Raw<DT>& x, float (&z)[kRun]) {
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      if constexpr (DT == BPD_DTYPE_BF16)
-        z[j] = __builtin_bit_cast(float, j & 1 ? w[j / 2] & 0xFFFF0000u : w[j / 2] << 16);
-      else
-        z[j] = float(__builtin_bit_cast(_Float16, uint16_t(w[j / 2] >> (16 * (j & 1)))));
-    }
+  for (int j = 0; j < kRun; ++j) {
+    if constexpr (DT == BPD_DTYPE_F32)
+      z[j] = __builtin_bit_cast(float, uint32_t(x.w[j / 4][j % 4]));
+    else if constexpr (DT == BPD_DTYPE_BF16)
+      z[j] = __builtin_bit_cast(float, j & 1 ? x.w[0][j / 2] & 0xFFFF0000u : x.w[0][j / 2] << 16);
+    else
+      z[j] = float(__builtin_bit_cast(_Float16, uint16_t(x.w[0][j / 2] >> (16 * (j & 1)))));
   }
 }
 
@@ -295,10 +298,26 @@ __device__ __forceinline__ Run run_at(int64_t t, int64_t vocab) {
   return Run{t - shift, 0xFFu << shift & 0xFFu, shift};
 }
 template <int DT>
-__device__ __forceinline__ void load_run(const void* from, const Run& run, int64_t vocab, float (&z)[kRun]) {
-  if (vocab >= kRun) return load_run<DT>(from, run.t, z);
+__device__ __forceinline__ Raw<DT> load_raw(const void* from, const Run& run, int64_t vocab) {
+  Raw<DT> x;
+  if (vocab >= kRun) {
+    const char* p = static_cast<const char*>(from) + run.t * (DT == BPD_DTYPE_F32 ? 4 : 2);
+    __builtin_memcpy(&x, __builtin_assume_aligned(p, DT == BPD_DTYPE_F32 ? 4 : 2), sizeof(x));
+    return x;
+  }
 #pragma unroll
-  for (int j = 0; j < kRun; ++j) z[j] = load_elem(from, DT, j < vocab ? j : 0);
+  for (int j = 0; j < kRun; ++j) {
+    const int64_t t = j < vocab ? j : 0;
+    if constexpr (DT == BPD_DTYPE_F32)
+      x.w[j / 4][j % 4] = static_cast<const uint32_t*>(from)[t];
+    else
+      x.w[0][j / 2] = (j & 1 ? uint32_t(x.w[0][j / 2]) : 0u) | uint32_t(static_cast<const uint16_t*>(from)[t]) << (16 * (j & 1));
+  }
+  return x;
+}
+template <int DT>
+__device__ __forceinline__ void load_run(const void* from, const Run& run, int64_t vocab, float (&z)[kRun]) {
+  unpack<DT>(load_raw<DT>(from, run, vocab), z);
 }
 template <int DT, int N>
 __device__ __forceinline__ void load_runs(const void* from, const Run (&runs)[N], int64_t vocab, float (&z)[N][kRun]) {
@@ -334,7 +353,10 @@ __device__ __forceinline__ float wave_max(float x) {
 }
 
 // One wave per part, position (`count` from `from` on) and request, in this
-// order.  The positions before `from` have been judged.
+// order.  The positions before `from` have been judged.  A lane keeps its own
+// largest logit and the sum relative to it; all its runs are on their way before
+// the first is summed.  (Two or four such sets per wave, the next on its way
+// while one is summed: 23 -> 26 us for the first position of 256 rows.)
 template <int DT, int Runs>
 __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs a, Space w, int32_t from, int32_t count) {
   const int lane = threadIdx.x % kWave;
@@ -346,48 +368,59 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs a, Spa
   const int32_t i = from + int32_t(at - uint32_t(b) * uint32_t(count));
   if (i > draft_len(a, b) || (from > 0 && w.decided[b] >= 0)) return;
   int32_t* states = w.states + b * (a.drafts + 1);
+  const char* row = row_of(a, b, i);
+  Raw<DT> raw[Runs];
+  uint32_t bits[Runs];
+  const auto run_of = [&](int k) { return run_at((int64_t(part) * Runs + k) * (kWave * kRun) + lane * kRun, a.vocab); };
   // the logits, before the walk to this position's state is waited for
-  Run runs[Runs];
-  float z[Runs][kRun];
 #pragma unroll
-  for (int k = 0; k < Runs; ++k) runs[k] = run_at((int64_t(part) * Runs + k) * (kWave * kRun) + lane * kRun, a.vocab);
-  load_runs<DT>(row_of(a, b, i), runs, a.vocab, z);
+  for (int k = 0; k < Runs; ++k) raw[k] = load_raw<DT>(row, run_of(k), a.vocab);
   int32_t state = from > 0 ? states[from - 1] : 0;
   for (int32_t k = a.bit_rows ? i : from; k <= i; ++k) state = state_at(a, b, k, state);
   if (part == 0 && lane == 0) states[i] = state;
+#pragma unroll
+  for (int k = 0; k < Runs; ++k) bits[k] = run_bits(a, state, run_of(k));
+  const double temp = temperature_of(a, b);
+  // half the difference does not pass the type's range; a factor past it would
+  // only make a zero of the largest logit's difference a NaN
+  const float to_log2 = temp > 0.0 ? float(fmin(2.0 * kLog2E / temp, 1e38)) : 0.0f;
   bool bad = false;
-  float top = -INFINITY;
+  float top = -INFINITY, sum = 0.0f;
+  int32_t first = 0x7FFFFFFF;
 #pragma unroll
   for (int k = 0; k < Runs; ++k) {
-    const uint32_t bits = run_bits(a, state, runs[k]);
+    if (!__any(bits[k] != 0)) continue;
+    float z[kRun], here = -INFINITY;
+    unpack<DT>(raw[k], z);
 #pragma unroll
     for (int j = 0; j < kRun; ++j) {
-      z[k][j] = masked(z[k][j], bits, j);
-      bad |= !(z[k][j] < INFINITY);
-      top = fmaxf(top, z[k][j]);
+      z[j] = masked(z[j], bits[k], j);
+      bad |= !(z[j] < INFINITY);
+      here = fmaxf(here, z[j]);
     }
-  }
-  top = wave_max(top);
-  Part p{__any(bad) ? NAN : top, 0.0f};
-  const double temp = temperature_of(a, b);
-  if (!(p.top > -INFINITY)) {
-    // nothing allowed, or nothing that has a softmax
-  } else if (temp > 0.0) {
-    // half the difference does not pass the type's range; a factor past it
-    // would only make a zero of the largest logit's difference a NaN
-    const float to_log2 = float(fmin(2.0 * kLog2E / temp, 1e38)), half = -0.5f * top;
+    if (temp > 0.0) {
+      if (__any(here > top)) {
+        const float now = fmaxf(top, here);
+        sum *= top > -INFINITY ? __builtin_amdgcn_exp2f(__builtin_fmaf(top, 0.5f, -0.5f * now) * to_log2) : 0.0f;
+        top = now;
+      }
+      const float half = -0.5f * (top > -INFINITY ? top : 0.0f);
 #pragma unroll
-    for (int k = 0; k < Runs; ++k)
-#pragma unroll
-      for (int j = 0; j < kRun; ++j) p.sum += __builtin_amdgcn_exp2f(__builtin_fmaf(z[k][j], 0.5f, half) * to_log2);
-    p.sum = wave_sum(p.sum);
-  } else {
-    int32_t first = 0x7FFFFFFF;
-#pragma unroll
-    for (int k = Runs - 1; k >= 0; --k)
+      for (int j = 0; j < kRun; ++j) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(z[j], 0.5f, half) * to_log2);
+    } else if (here > top) {
+      top = here;
 #pragma unroll
       for (int j = kRun - 1; j >= 0; --j)
-        if (z[k][j] == top) first = int32_t(runs[k].t) + j;
+        if (z[j] == top) first = int32_t(run_of(k).t) + j;
+    }
+  }
+  // the lanes' parts as one
+  const float whole = wave_max(top);
+  Part p{__any(bad) ? NAN : whole, 0.0f};
+  if (p.top > -INFINITY && temp > 0.0) {
+    p.sum = wave_sum(sum * __builtin_amdgcn_exp2f(__builtin_fmaf(top, 0.5f, -0.5f * whole) * to_log2));
+  } else if (p.top > -INFINITY) {
+    if (top != whole) first = 0x7FFFFFFF;
     for (int o = 32; o; o >>= 1) first = min(first, __shfl_xor(first, o));
     p.sum = __builtin_bit_cast(float, first);
   }
@@ -575,25 +608,34 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a, Spa
   if (st.empty || !(temperature_of(a, b) > 0.0)) return;
   const Deciding d = deciding(a, b, n, st);
   const bool less = n < draft_len(a, b);
-  Run runs[Runs];
-  float z[Runs][kRun], q[Runs][kRun];
-#pragma unroll
-  for (int k = 0; k < Runs; ++k) runs[k] = run_at((int64_t(chunk) * Runs + k) * (kThreads * kRun) + tid * kRun, a.vocab);
-  load_runs<DT>(d.row, runs, a.vocab, z);
-  draft_runs(a, d, runs, q);
+  // One run at a time leaves seven waves on a SIMD, which hide its loads better
+  // than two or four runs in flight do (57, 60 and 66 us: 256 rows of 151,936
+  // bf16 with bf16 probabilities).
+  constexpr int kAtOnce = 1;
   double s[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll 1
+  for (int k0 = 0; k0 < Runs; k0 += kAtOnce) {
+    Run runs[kAtOnce];
+    float z[kAtOnce][kRun], q[kAtOnce][kRun];
 #pragma unroll
-  for (int k = 0; k < Runs; ++k) {
-    const uint32_t bits = run_bits(a, d.state, runs[k]);
+    for (int k = 0; k < kAtOnce; ++k)
+      runs[k] = run_at((int64_t(chunk) * Runs + k0 + k) * (kThreads * kRun) + tid * kRun, a.vocab);
+    load_runs<DT>(d.row, runs, a.vocab, z);
+    draft_runs(a, d, runs, q);
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      const double x = exp2_down((double(masked(z[k][j], bits, j)) - d.top) * d.to_log2);
-      s[0] += x;
-      if (!less) continue;
-      const double p = q[k][j], y = x - p * st.sum;
-      s[1] += y > 0.0 ? x : 0.0;
-      s[2] += y > 0.0 ? p : 0.0;
-      s[3] += fabs(y) <= kSumError * x ? x : 0.0;
+    for (int k = 0; k < kAtOnce; ++k) {
+      const uint32_t bits = run_bits(a, d.state, runs[k]);
+      if (!__any(bits != 0)) continue;
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
+        const double x = exp2_down((double(masked(z[k][j], bits, j)) - d.top) * d.to_log2);
+        s[0] += x;
+        if (!less) continue;
+        const double p = q[k][j], y = x - p * st.sum;
+        s[1] += y > 0.0 ? x : 0.0;
+        s[2] += y > 0.0 ? p : 0.0;
+        s[3] += fabs(y) <= kSumError * x ? x : 0.0;
+      }
     }
   }
 #pragma unroll
