@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "kv4.hpp"
+#include "wave.hpp"
 
 namespace bpd {
 namespace {
@@ -77,21 +78,9 @@ __device__ __forceinline__ int32_t tiles_of(const AttendArgs& a, int64_t b) {
   return n < 1 ? 1 : n;
 }
 
-template <class T>
-__device__ __forceinline__ T wave_sum(T x) {
-  for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
-  return x;
-}
-
-// A value that all lanes share, or lane `from`'s, in scalar registers.
+// A value that all lanes share, in scalar registers.
 __device__ __forceinline__ int32_t scalar(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ int64_t scalar(int64_t x) {
-  return int64_t(scalar(int32_t(x >> 32))) << 32 | uint32_t(scalar(int32_t(x)));
-}
-__device__ __forceinline__ int64_t scalar(int64_t x, int from) {
-  return int64_t(__builtin_amdgcn_readlane(int32_t(x >> 32), from)) << 32 |
-         uint32_t(__builtin_amdgcn_readlane(int32_t(x), from));
-}
+__device__ __forceinline__ int64_t scalar(int64_t x) { return of_lane(x, 0); }
 
 __device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {  // of numbers that are not negative
   if (((x | y) >> 32) == 0) return scalar(int32_t(uint32_t(x) / uint32_t(y)));
@@ -114,7 +103,7 @@ __device__ __forceinline__ bool find_place(const AttendArgs& a, const AttendPlan
   const int32_t mine = lane < a.rows ? tiles_of(a, lane) : 0;
   int64_t whole = mine;
   for (int64_t b = lane + kWave; b < a.rows; b += kWave) whole += tiles_of(a, b);
-  whole = scalar(wave_sum(whole));
+  whole = wave_sum(whole);
   const int64_t per = quotient(whole * units + p.blocks - 1, p.blocks);
   *run = per < kWaves ? kWaves : per;
   place->whole = whole * units;
@@ -123,20 +112,16 @@ __device__ __forceinline__ bool find_place(const AttendArgs& a, const AttendPlan
   int64_t before = 0;
   for (int64_t b0 = 0;; b0 += kWave) {
     const int32_t here = b0 == 0 ? mine : b0 + lane < a.rows ? tiles_of(a, b0 + lane) : 0;
-    int64_t upto = here;
-    for (int o = 1; o < kWave; o <<= 1) {
-      const int64_t y = __shfl_up(upto, o);
-      if (lane >= o) upto += y;
-    }
+    const int64_t upto = wave_scan_sum(int64_t(here));
     const uint64_t m = __ballot(row < 0 ? (before + upto) * units > at : b0 + lane == row);
     if (m) {
       const int hit = __builtin_ctzll(m);
       place->row = b0 + hit;
       place->tiles = __builtin_amdgcn_readlane(here, hit);
-      place->first = (before + scalar(upto, hit) - place->tiles) * units;
+      place->first = (before + of_lane(upto, hit) - place->tiles) * units;
       return true;
     }
-    before += scalar(upto, kWave - 1);
+    before += of_lane(upto, kWave - 1);
   }
 }
 
@@ -360,7 +345,7 @@ __global__ __launch_bounds__(kWaves* kWave, attend_blocks(D, NT)) void kv_attend
     for (int k = 0; k < KW; ++k)
       if ((t * KW + k) % kWaves == wave) queries[t][k][ql] = q[t][k];
   __syncthreads();
-  for (int o = 1; o < 16; o <<= 1) least = min(least, __shfl_xor(least, o));
+  least = wave_min(least);
 
   f32x4 acc[NT][VT];
   float top[NT], sum[NT];

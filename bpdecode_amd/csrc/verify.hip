@@ -14,6 +14,7 @@
 #include <cmath>
 
 #include "bpd_common.hpp"
+#include "wave.hpp"
 
 namespace bpd {
 namespace {
@@ -342,16 +343,6 @@ __device__ __forceinline__ const char* row_of(const VerifyArgs& a, int64_t b, in
   return static_cast<const char*>(a.logits) + row_at(a, b, i) * (a.dtype == BPD_DTYPE_F32 ? 4 : 2);
 }
 
-template <class T>
-__device__ __forceinline__ T wave_sum(T x) {
-  for (int o = 32; o; o >>= 1) x += __shfl_xor(x, o);
-  return x;
-}
-__device__ __forceinline__ float wave_max(float x) {
-  for (int o = 32; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
-  return x;
-}
-
 // One wave per part, position (`count` from `from` on) and request, in this
 // order.  The positions before `from` have been judged.  A lane keeps its own
 // largest logit and the sum relative to it; all its runs are on their way before
@@ -421,8 +412,7 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs a, Spa
     p.sum = wave_sum(sum * __builtin_amdgcn_exp2f(__builtin_fmaf(top, 0.5f, -0.5f * whole) * to_log2));
   } else if (p.top > -INFINITY) {
     if (top != whole) first = 0x7FFFFFFF;
-    for (int o = 32; o; o >>= 1) first = min(first, __shfl_xor(first, o));
-    p.sum = __builtin_bit_cast(float, first);
+    p.sum = __builtin_bit_cast(float, wave_min(first));
   }
   if (lane == 0) w.parts[(b * (a.drafts + 1) + i) * w.row_parts + part] = p;
 }
@@ -452,7 +442,7 @@ __device__ __forceinline__ RowStat whole_row(const VerifyArgs& a, const Space& w
   }
   for (int32_t c = lane; c < w.row_parts; c += kWave)
     if (parts[c].top == st.top) st.first = min(st.first, __builtin_bit_cast(int32_t, parts[c].sum));
-  for (int o = 32; o; o >>= 1) st.first = min(st.first, __shfl_xor(st.first, o));
+  st.first = wave_min(st.first);
   st.sum = 1.0;
   return st;
 }
@@ -718,18 +708,13 @@ __global__ __launch_bounds__(kThreads* Runs) void verify_pick_kernel(VerifyArgs 
             mine = off ? y.over - y.take * s.all : y.all;
             mine = mine > 0.0 ? mine : 0.0;
           }
-          double upto = mine;
-          for (int o = 1; o < kWave; o <<= 1) {
-            const double y = __shfl_up(upto, o);
-            if (lane >= o) upto += y;
-          }
-          upto += run;
-          run = __shfl(upto, kWave - 1);
+          const double upto = run + wave_scan_sum(mine);
+          run = of_lane(upto, kWave - 1);
           const uint64_t any = pass == 0 ? 0 : __ballot(mine > 0.0), past = __ballot(mine > 0.0 && upto > u * whole);
           if (any) {
             past_it = (any & past) != 0;
             const int l = past_it ? __builtin_ctzll(past) : 63 - __builtin_clzll(any);
-            hit = c0 + l, at = __shfl(upto - mine, l);
+            hit = c0 + l, at = of_lane(upto - mine, l);
           }
         }
         if (pass == 0) whole = run;
@@ -742,11 +727,7 @@ __global__ __launch_bounds__(kThreads* Runs) void verify_pick_kernel(VerifyArgs 
       const int64_t t = shares(where, take_off != 0, row_sum, x);
 #pragma unroll
       for (int j = 0; j < kRun; ++j) own += x[j];
-      double upto = own;
-      for (int o = 1; o < kWave; o <<= 1) {
-        const double y = __shfl_up(upto, o);
-        if (lane >= o) upto += y;
-      }
+      const double upto = wave_scan_sum(own);
       if (lane == kWave - 1) sums[wave] = upto;
       __syncthreads();
       double at = before + (upto - own);
