@@ -47,6 +47,7 @@ __host__ __device__ __forceinline__ int64_t seen_tokens(const AttendArgs& a, int
 constexpr int kWave = 64;
 constexpr int kTile = 64;   // cache tokens that a wave takes at a time
 constexpr int kWaves = 4;   // waves of a block
+constexpr int kManyWaves = 16, kManyPieces = 16;  // of a join of that many pieces a unit
 constexpr int kNever = 0x7FFFFFFF;
 
 // How a call's work is cut.  A unit is one request, one key head and one group
@@ -586,11 +587,11 @@ __global__ __launch_bounds__(kWaves* kWave, attend_blocks(D, NT)) void kv_attend
 
 // Joins the pieces of a unit that lies in several runs: one block per unit,
 // column tile and pair of value tiles, its waves over the pieces.
-template <int DT, int D, int NT>
-__global__ __launch_bounds__(kWaves* kWave) void kv_attend_join_kernel(AttendArgs a, AttendPlan plan) {
+template <int DT, int D, int NT, int W>
+__global__ __launch_bounds__(W* kWave) void kv_attend_join_kernel(AttendArgs a, AttendPlan plan) {
   constexpr int VT = D / 16, kPiece = (2 + 4 * VT) * kWave, kAtOnce = 4;
-  __shared__ f32x4 joined[kWaves][2][kWave];
-  __shared__ float tops[kWaves][kWave], sums[kWaves][kWave];
+  __shared__ f32x4 joined[W][2][kWave];
+  __shared__ float tops[W][kWave], sums[W][kWave];
   const int lane = threadIdx.x % kWave, wave = scalar(int32_t(threadIdx.x / kWave));
   uint32_t x = blockIdx.x;
   const int v0 = int(x % (VT / 2)) * 2;
@@ -608,12 +609,12 @@ __global__ __launch_bounds__(kWaves* kWave) void kv_attend_join_kernel(AttendArg
   if (run0 == run1) return;
   float top = -3e38f, sum = 0.0f;
   f32x4 acc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-  for (int64_t i0 = run0 + wave; i0 <= run1; i0 += kWaves * kAtOnce) {
+  for (int64_t i0 = run0 + wave; i0 <= run1; i0 += W * kAtOnce) {
     float m[kAtOnce], l[kAtOnce];
     f32x4 y[kAtOnce][2];
 #pragma unroll
     for (int n = 0; n < kAtOnce; ++n) {
-      const int64_t i = i0 + n * kWaves;
+      const int64_t i = i0 + n * W;
       m[n] = -3e38f, l[n] = 0.0f, y[n][0] = y[n][1] = f32x4{0, 0, 0, 0};
       if (i > run1) continue;
       const float* p = plan.partials + ((2 * i + (i == run0 && begin != run0 * run ? 1 : 0)) * NT + t) * kPiece;
@@ -646,7 +647,7 @@ __global__ __launch_bounds__(kWaves* kWave) void kv_attend_join_kernel(AttendArg
   if (wave) return;
   float now = top;
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) now = fmaxf(now, tops[w][lane]);
+  for (int w = 1; w < W; ++w) now = fmaxf(now, tops[w][lane]);
   const float keep = __builtin_amdgcn_exp2f(top - now);
   sum *= keep;
 #pragma unroll
@@ -654,7 +655,7 @@ __global__ __launch_bounds__(kWaves* kWave) void kv_attend_join_kernel(AttendArg
 #pragma unroll
     for (int k = 0; k < 4; ++k) acc[v][k] *= keep;
 #pragma unroll
-  for (int w = 1; w < kWaves; ++w) {
+  for (int w = 1; w < W; ++w) {
     const float f = __builtin_amdgcn_exp2f(tops[w][lane] - now);
     sum += sums[w][lane] * f;
 #pragma unroll
@@ -718,7 +719,11 @@ int launch_attend(const AttendArgs& a, const AttendSizes& z, hipStream_t s) {
   BPD_REQUIRE(z.tiles < (int64_t(1) << 31) && joins < (int64_t(1) << 31), "too many queries or tokens in one call");
   const int64_t blocks = z.plan.blocks ? attend_runs(z, a.rows) : a.rows * a.kv_heads * z.plan.groups;
   kv_attend_kernel<DT, D, NT><<<uint32_t(blocks), kWaves * kWave, 0, s>>>(a, z.plan);
-  if (z.plan.blocks) kv_attend_join_kernel<DT, D, NT><<<uint32_t(joins), kWaves * kWave, 0, s>>>(a, z.plan);
+  // few units have many pieces each: more waves to a unit's join
+  if (z.plan.blocks >= kManyPieces * a.rows * a.kv_heads * z.plan.groups)
+    kv_attend_join_kernel<DT, D, NT, kManyWaves><<<uint32_t(joins), kManyWaves * kWave, 0, s>>>(a, z.plan);
+  else if (z.plan.blocks)
+    kv_attend_join_kernel<DT, D, NT, kWaves><<<uint32_t(joins), kWaves * kWave, 0, s>>>(a, z.plan);
   BPD_LAUNCHED();
   return BPD_OK;
 }
