@@ -611,20 +611,28 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a, Spa
     for (int k = 0; k < kAtOnce; ++k)
       runs[k] = run_at((int64_t(chunk) * Runs + k0 + k) * (kThreads * kRun) + tid * kRun, a.vocab);
     load_runs<DT>(d.row, runs, a.vocab, z);
-    draft_runs(a, d, runs, q);
+    if (d.probs) draft_runs(a, d, runs, q);
 #pragma unroll
     for (int k = 0; k < kAtOnce; ++k) {
       const uint32_t bits = run_bits(a, d.state, runs[k]);
       if (!__any(bits != 0)) continue;
+      double x[kRun];
 #pragma unroll
       for (int j = 0; j < kRun; ++j) {
-        const double x = exp2_down((double(masked(z[k][j], bits, j)) - d.top) * d.to_log2);
-        s[0] += x;
-        if (!less) continue;
-        const double p = q[k][j], y = x - p * st.sum;
-        s[1] += y > 0.0 ? x : 0.0;
-        s[2] += y > 0.0 ? p : 0.0;
-        s[3] += fabs(y) <= kSumError * x ? x : 0.0;
+        x[j] = exp2_down((double(masked(z[k][j], bits, j)) - d.top) * d.to_log2);
+        s[0] += x[j];
+      }
+      if (d.probs) {
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) {
+          const double p = q[k][j], y = x[j] - p * st.sum;
+          s[1] += y > 0.0 ? x[j] : 0.0;
+          s[2] += y > 0.0 ? p : 0.0;
+          s[3] += fabs(y) <= kSumError * x[j] ? x[j] : 0.0;
+        }
+      } else if (less) {  // all but the drafted token
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) s[1] += runs[k].t + j == d.drafted ? 0.0 : x[j];
       }
     }
   }
