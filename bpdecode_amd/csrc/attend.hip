@@ -184,8 +184,7 @@ __device__ __forceinline__ void store_columns(uint16_t* out, int v, int g, const
 // Blocks that a CU is to hold, by registers (a block puts one wave on each SIMD).
 constexpr int attend_blocks(int dim, int nt) {
   if (nt == 1) return dim == 64 ? 4 : dim == 128 ? 3 : 2;
-  if (nt == 2) return dim == 64 ? 3 : dim <= 128 ? 2 : 1;
-  return 1;
+  return dim == 64 ? 3 : dim <= 128 ? 2 : 1;
 }
 
 // A value that the compiler forms anew here instead of keeping it (or what
@@ -673,11 +672,6 @@ __global__ __launch_bounds__(W* kWave) void kv_attend_join_kernel(AttendArgs a, 
                           sum == 0.0f ? 0.0f : 1.0f / sum);
 }
 
-// Column tiles of a wave: every query column of a key head where they fit.
-// More share the conversions of keys and values, but the registers of four
-// (of two from 192 channels on) are the most that leave waves to hide loads.
-constexpr int most_tiles(int dim) { return dim > 128 ? 2 : 4; }
-
 struct AttendSizes {
   AttendPlan plan;
   int32_t nt;
@@ -687,13 +681,21 @@ struct AttendSizes {
 };
 
 constexpr int kCus = 256;
-constexpr int kShort = 16, kMiddling = 64;  // tiles of a unit
+// Tiles of a unit up to which it is short, or of a middling length.  Eight
+// units of 1,000 tokens: 10.9 us, cut in runs 14.9; of 2,000: 15.9 and 14.6.
+// 512 units of 4,000 tokens: 50 and 59, of 8,000: 92 and 99; 128 units of
+// 4,000 (a sixth of the device): 30 and 26.
+constexpr int kShort = 16, kMiddling = 128;
 
 AttendSizes attend_sizes(int64_t rows, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t dim, int64_t longest) {
   AttendSizes z{};
   const int64_t cols = int64_t(tokens) * (heads / kv_heads);
-  const int64_t col_tiles = (cols + 15) / 16, most = most_tiles(dim);
-  z.nt = col_tiles <= 1 ? 1 : col_tiles <= 2 || most == 2 ? 2 : 4;
+  // Two column tiles to a wave share the conversions of keys and values; four
+  // leave one wave to a SIMD, and groups of two are read again from L2 instead
+  // (72 columns of 128 channels, 64 requests of 4,000 tokens: one tile 91 us,
+  // two 83, four 114; 40 columns of 64 channels: 40, 37 and 46).
+  const int64_t col_tiles = (cols + 15) / 16;
+  z.nt = col_tiles <= 1 ? 1 : 2;
   z.plan.groups = int32_t((col_tiles + z.nt - 1) / z.nt);
   z.plan.cols = int32_t((cols + z.plan.groups - 1) / z.plan.groups);
   const int64_t per_unit = std::max<int64_t>(1, (std::min<int64_t>(longest, 0x7FFFFFFF) + kTile - 1) / kTile);
@@ -731,8 +733,6 @@ int launch_attend(const AttendArgs& a, const AttendSizes& z, hipStream_t s) {
 template <int DT, int D>
 int launch_attend_tiles(const AttendArgs& a, const AttendSizes& z, hipStream_t s) {
   if (z.nt == 1) return launch_attend<DT, D, 1>(a, z, s);
-  if constexpr (most_tiles(D) == 4)
-    if (z.nt == 4) return launch_attend<DT, D, 4>(a, z, s);
   return launch_attend<DT, D, 2>(a, z, s);
 }
 

@@ -217,9 +217,11 @@ struct Space {
   size_t bytes;
 };
 
-// Long runs share out what a wave does besides its tokens, short ones spread
-// a small call over more of the device.
-constexpr int64_t kLongFrom = int64_t(4) << 20;  // tokens of all positions
+// Long runs share out what a wave does besides its tokens, short ones spread a
+// small call over more of the device and need no launch of their own for the
+// verdicts (five positions of 151,936 bf16: one request 30 us with long runs,
+// 25 with short ones; 8: 33.3 and 32.6; 12: 35 and 37; 32: 45 and 62).
+constexpr int64_t kLongFrom = int64_t(8) << 20;  // tokens of all positions
 
 Space verify_space(int64_t rows, int32_t drafts, int64_t vocab, void* at = nullptr) {
   Space w{};
@@ -770,7 +772,8 @@ __global__ __launch_bounds__(kThreads* Runs) void verify_pick_kernel(VerifyArgs 
 
 // Bytes of one position of every request from which the positions are read in
 // three steps (the first, the second, the others), each for the requests whose
-// drafts stand so far.
+// drafts stand so far (half of them at each; five positions of 151,936 bf16:
+// 128 requests 96 us in steps, 92 at once; 160: 108 and 106; 256: 178 and 188).
 constexpr int64_t kStepBytes = int64_t(48) << 20;
 
 template <int DT, int Runs>

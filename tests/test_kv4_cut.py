@@ -20,9 +20,9 @@ CUTS = [  # tokens, kv heads, heads, dim, page, dtype, lengths
     (1, 1, 2, 64, 16, BF16, [5_000, 1, 0, 17, 4_999, 64]),      # long and short ones, equal runs
     (2, 2, 4, 128, 64, FP16, [4_500, 300, 2, 4_400]),
     (1, 2, 2, 96, 32, BF16, [4_200, 63, 64, 65]),
-    (3, 1, 24, 128, 16, BF16, [4_300, 70]),                      # 72 columns: two groups
+    (3, 1, 24, 128, 16, BF16, [4_300, 70]),                      # 72 columns: groups of two tiles
     (9, 1, 8, 64, 32, FP16, [5_100, 9, 8]),
-    (20, 1, 7, 128, 32, BF16, [500, 21]),                        # 140 columns: three groups
+    (20, 1, 7, 128, 32, BF16, [500, 21]),                        # 140 columns
     (5, 1, 8, 256, 16, BF16, [4_200, 33]),                       # 40 columns of 256 channels
     (7, 2, 8, 192, 64, FP16, [4_120, 200]),
     (1, 1, 1, 256, 256, BF16, [4_600, 255, 257]),
