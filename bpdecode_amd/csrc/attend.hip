@@ -206,7 +206,22 @@ __device__ __forceinline__ int here(int x) {
 // of row m, next to each other, of the tokens from 16 g, converts two codes
 // of a token at a time and swaps halves with the next token's.
 // The running maximum is followed loosely: weights may grow to 2^8 before the
-// sums are scaled down, so most tiles cost no exchange between lanes.
+// sums are scaled down, so most tiles cost no exchange between lanes.  Scores,
+// maximum, sums and the accumulated values are floats; the weights are rounded
+// to the cache's type for the second product, half a step of which is all that
+// is lost (the values themselves are exact in it).
+//
+// (The product that takes codes and scales as they are, fp4 by fp8, was left:
+// of 8 neighbouring products it keeps bits down to 2^-13 of the largest, and
+// queries would need two or three fp8 terms each.)
+//
+// What bounds it: the cache's bytes for long contexts (32 requests of up to
+// 32,768 tokens, 64/8 heads of 128, two tokens: 866 MB in 173 us, 5.0 TB/s of
+// the 5.8 that a plain read reaches), and before that the conversions: a tile
+// of 64 tokens takes about 360 vector instructions, 430 with two column tiles,
+// which two or three waves on a SIMD issue one in five cycles (64 blocks of 5
+// drafts over up to 4,096 tokens: 220 MB in 57 us).  A block that finds
+// nothing to do takes 5 us, each of its first tiles 1.4.
 template <int DT, int D, int NT>
 __global__ __launch_bounds__(kWaves* kWave, attend_blocks(D, NT)) void kv_attend_kernel(AttendArgs a, AttendPlan plan) {
   using Pt = Parts<D>;
@@ -253,334 +268,338 @@ __global__ __launch_bounds__(kWaves* kWave, attend_blocks(D, NT)) void kv_attend
   const int shift = __builtin_ctz(P);
 
   for (;;) {
-  const int32_t n_here = int32_t(stop - pos < tiles - tile0 ? stop - pos : tiles - tile0);
-  const int32_t kvh = scalar(unit / plan.groups), group = unit - kvh * plan.groups;
-  const int32_t n_q = queries_of(a, b);
-  const int64_t end = n_q > 0 ? length_of(a, b) : 0;
-  const int32_t tile1 = end > 0 ? tile0 + n_here : tile0;
-  if (a.err && n_q > 0 && a.lengths[b] > end && threadIdx.x == 0) atomicOr(a.err, BPD_FLAG_PAGE_RANGE);
+    const int32_t n_here = int32_t(stop - pos < tiles - tile0 ? stop - pos : tiles - tile0);
+    const int32_t kvh = scalar(unit / plan.groups), group = unit - kvh * plan.groups;
+    const int32_t n_q = queries_of(a, b);
+    const int64_t end = n_q > 0 ? length_of(a, b) : 0;
+    const int32_t tile1 = end > 0 ? tile0 + n_here : tile0;
+    if (a.err && n_q > 0 && a.lengths[b] > end && threadIdx.x == 0) atomicOr(a.err, BPD_FLAG_PAGE_RANGE);
 
-  const int32_t* table = a.table.block_table + b * a.table.ld;
-  // page of the chunk of 16 tokens that starts at t, -1: none
-  const auto page_at = [&](int64_t t) -> int32_t { return t < end ? table[t >> shift] : -1; };
-  const auto block_at = [&](int32_t page) -> const uint8_t* {
-    const int64_t ok = page >= 0 && page < a.table.num_pages ? page : 0;  // a page outside the pool is masked below
-    return a.pages + (ok * a.kv_heads + kvh) * int64_t(a.page.bytes());
-  };
+    const int32_t* table = a.table.block_table + b * a.table.ld;
+    // page of the chunk of 16 tokens that starts at t, -1: none
+    const auto page_at = [&](int64_t t) -> int32_t { return t < end ? table[t >> shift] : -1; };
+    const auto block_at = [&](int32_t page) -> const uint8_t* {
+      // a page outside the pool is masked below
+      const int64_t ok = page >= 0 && page < a.table.num_pages ? page : 0;
+      return a.pages + (ok * a.kv_heads + kvh) * int64_t(a.page.bytes());
+    };
 
-  uint32_t kc[4][KW], ks[G], vc[16][Pt::count], vs[kScaleWords];
-  const auto load_keys = [&](const uint8_t* block, int32_t slot) {  // tokens 4 m + j of a tile
-    const uint8_t* codes = block + slot * (D / 2);
+    uint32_t kc[4][KW], ks[G], vc[16][Pt::count], vs[kScaleWords];
+    const auto load_keys = [&](const uint8_t* block, int32_t slot) {  // tokens 4 m + j of a tile
+      const uint8_t* codes = block + slot * (D / 2);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int p = 0; p < Pt::count; ++p) {
-        const uint32_t* from =
-            reinterpret_cast<const uint32_t*>(codes + j * (D / 2) + Pt::begin(p) / 2 + g * (Pt::width(p) / 8));
+        for (int p = 0; p < Pt::count; ++p) {
+          const uint32_t* from =
+              reinterpret_cast<const uint32_t*>(codes + j * (D / 2) + Pt::begin(p) / 2 + g * (Pt::width(p) / 8));
 #pragma unroll
-        for (int k = 0; k < Pt::width(p) / 32; ++k) kc[j][Pt::begin(p) / 32 + k] = from[k];
+          for (int k = 0; k < Pt::width(p) / 32; ++k) kc[j][Pt::begin(p) / 32 + k] = from[k];
+        }
+      const uint32_t* scales = reinterpret_cast<const uint32_t*>(block + a.page.k_scales() + slot * G);
+#pragma unroll
+      for (int k = 0; k < G; ++k) ks[k] = scales[k];
+    };
+    const auto load_values = [&](const uint8_t* block, int32_t slot) {  // tokens 16 g + u of a tile
+      const uint8_t* codes = block + a.page.v_codes() + slot * (D / 2);
+#pragma unroll
+      for (int u = 0; u < 16; ++u)
+#pragma unroll
+        for (int p = 0; p < Pt::count; ++p) {
+          const uint8_t* from = codes + u * (D / 2) + Pt::begin(p) / 2 + m * (Pt::width(p) / 32);
+          if (Pt::width(p) == 128) vc[u][p] = *reinterpret_cast<const uint32_t*>(from);
+          if (Pt::width(p) == 64) vc[u][p] = *reinterpret_cast<const uint16_t*>(from);
+          if (Pt::width(p) == 32) vc[u][p] = *from;
+        }
+      const uint4* scales = reinterpret_cast<const uint4*>(block + a.page.v_scales() + slot * G);
+#pragma unroll
+      for (int k = 0; k < kScaleWords / 4; ++k) {
+        const uint4 w = scales[k];
+        vs[4 * k] = w.x, vs[4 * k + 1] = w.y, vs[4 * k + 2] = w.z, vs[4 * k + 3] = w.w;
       }
-    const uint32_t* scales = reinterpret_cast<const uint32_t*>(block + a.page.k_scales() + slot * G);
-#pragma unroll
-    for (int k = 0; k < G; ++k) ks[k] = scales[k];
-  };
-  const auto load_values = [&](const uint8_t* block, int32_t slot) {  // tokens 16 g + u of a tile
-    const uint8_t* codes = block + a.page.v_codes() + slot * (D / 2);
-#pragma unroll
-    for (int u = 0; u < 16; ++u)
-#pragma unroll
-      for (int p = 0; p < Pt::count; ++p) {
-        const uint8_t* from = codes + u * (D / 2) + Pt::begin(p) / 2 + m * (Pt::width(p) / 32);
-        if (Pt::width(p) == 128) vc[u][p] = *reinterpret_cast<const uint32_t*>(from);
-        if (Pt::width(p) == 64) vc[u][p] = *reinterpret_cast<const uint16_t*>(from);
-        if (Pt::width(p) == 32) vc[u][p] = *from;
-      }
-    const uint4* scales = reinterpret_cast<const uint4*>(block + a.page.v_scales() + slot * G);
-#pragma unroll
-    for (int k = 0; k < kScaleWords / 4; ++k) {
-      const uint4 w = scales[k];
-      vs[4 * k] = w.x, vs[4 * k + 1] = w.y, vs[4 * k + 2] = w.z, vs[4 * k + 3] = w.w;
+    };
+    int32_t tile = tile0 + wave;
+    int32_t kpage = -1, vpage = -1, knext = -1, vnext = -1;
+    if (tile < tile1) {
+      kpage = page_at(int64_t(tile) * kTile + (m >> 2) * 16);
+      vpage = page_at(int64_t(tile) * kTile + g * 16);
     }
-  };
-  int32_t tile = tile0 + wave;
-  int32_t kpage = -1, vpage = -1, knext = -1, vnext = -1;
-  if (tile < tile1) kpage = page_at(int64_t(tile) * kTile + (m >> 2) * 16), vpage = page_at(int64_t(tile) * kTile + g * 16);
-  // this lane's columns: the queries, and how many tokens each sees
-  const int ql = here(lane), qm = ql & 15;
-  Frag q[NT][KW];  // every fourth of them
-  int32_t sees[NT];
-  int32_t least = int32_t(end);
+    // this lane's columns: the queries, and how many tokens each sees
+    const int ql = here(lane), qm = ql & 15;
+    Frag q[NT][KW];  // every fourth of them
+    int32_t sees[NT];
+    int32_t least = int32_t(end);
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int32_t c = group * plan.cols + t * 16 + qm;
-    const int32_t i = c / share, h = kvh * share + c % share;
-    const bool in = t * 16 + qm < plan.cols && i < n_q;
-    const int64_t s = in ? int64_t(a.lengths[b]) - n_q + 1 + i : 0;
-    sees[t] = int32_t(s < 0 ? 0 : s < end ? s : end);
-    if (in) least = min(least, sees[t]);
-    const uint16_t* row = a.q + b * a.q_row + (in ? i : 0) * a.q_token + (in ? h : 0) * a.q_head;
+    for (int t = 0; t < NT; ++t) {
+      const int32_t c = group * plan.cols + t * 16 + qm;
+      const int32_t i = c / share, h = kvh * share + c % share;
+      const bool in = t * 16 + qm < plan.cols && i < n_q;
+      const int64_t s = in ? int64_t(a.lengths[b]) - n_q + 1 + i : 0;
+      sees[t] = int32_t(s < 0 ? 0 : s < end ? s : end);
+      if (in) least = min(least, sees[t]);
+      const uint16_t* row = a.q + b * a.q_row + (in ? i : 0) * a.q_token + (in ? h : 0) * a.q_head;
 #pragma unroll
-    for (int p = 0; p < Pt::count; ++p)
+      for (int p = 0; p < Pt::count; ++p)
 #pragma unroll
-      for (int k = 0; k < Pt::width(p) / 32; ++k) {
-        const uint16_t* from = row + Pt::begin(p) + (ql >> 4) * (Pt::width(p) / 4) + 8 * k;
-        Frag f = {{0u, 0u, 0u, 0u}};
-        if (in && a.scale != 0.0f && (t * KW + Pt::begin(p) / 32 + k) % kWaves == wave) __builtin_memcpy(&f, from, 16);  // at any element
-        if (a.scale < 0.0f)
+        for (int k = 0; k < Pt::width(p) / 32; ++k) {
+          const uint16_t* from = row + Pt::begin(p) + (ql >> 4) * (Pt::width(p) / 4) + 8 * k;
+          Frag f = {{0u, 0u, 0u, 0u}};
+          if (in && a.scale != 0.0f && (t * KW + Pt::begin(p) / 32 + k) % kWaves == wave) __builtin_memcpy(&f, from, 16);  // at any element
+          if (a.scale < 0.0f)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) f.u[j] ^= 0x80008000u;
-        q[t][Pt::begin(p) / 32 + k] = f;
-      }
-  }
-  if (tile < tile1) {
-    const int64_t t0 = int64_t(tile) * kTile;
-    load_keys(block_at(kpage), int32_t((t0 + 4 * m) & (P - 1)));
-    load_values(block_at(vpage), int32_t((t0 + 16 * g) & (P - 1)));
-    const int64_t t1 = t0 + kWaves * kTile;
-    if (tile + kWaves < tile1) knext = page_at(t1 + (m >> 2) * 16), vnext = page_at(t1 + g * 16);
-  }
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int k = 0; k < KW; ++k)
-      if ((t * KW + k) % kWaves == wave) queries[t][k][ql] = q[t][k];
-  __syncthreads();
-  least = wave_min(least);
-
-  f32x4 acc[NT][VT];
-  float top[NT], sum[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    top[t] = -3e38f, sum[t] = 0.0f;
-#pragma unroll
-    for (int v = 0; v < VT; ++v) acc[t][v] = f32x4{0, 0, 0, 0};
-  }
-  int32_t nan_at[Pt::count];  // first token of the tail whose value group is bad, as a value lane
-#pragma unroll
-  for (int p = 0; p < Pt::count; ++p) nan_at[p] = kNever;
-  for (; tile < tile1; tile += kWaves) {
-    const int64_t t0 = int64_t(tile) * kTile, t1 = t0 + kWaves * kTile;
-    const bool more = tile + kWaves < tile1;
-    // read anew for every tile: the registers hold loads in flight instead
-    const int q_lane = here(lane);
-    f32x4 s[NT][4];
+            for (int j = 0; j < 4; ++j) f.u[j] ^= 0x80008000u;
+          q[t][Pt::begin(p) / 32 + k] = f;
+        }
+    }
+    if (tile < tile1) {
+      const int64_t t0 = int64_t(tile) * kTile;
+      load_keys(block_at(kpage), int32_t((t0 + 4 * m) & (P - 1)));
+      load_values(block_at(vpage), int32_t((t0 + 16 * g) & (P - 1)));
+      const int64_t t1 = t0 + kWaves * kTile;
+      if (tile + kWaves < tile1) knext = page_at(t1 + (m >> 2) * 16), vnext = page_at(t1 + g * 16);
+    }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[t][j] = f32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int p = 0; p < Pt::count; ++p) {
-      float sc[4];  // of the lane's group of channels, by token
-#pragma unroll
-      for (int j = 0; j < 4; ++j) sc[j] = scale_at(ks, G * j + Pt::begin(p) / kKvGroup, G, ksel[p]);
-#pragma unroll
-      for (int k = 0; k < Pt::width(p) / 32; ++k) {
-        Frag q[NT];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) q[t] = queries[t][Pt::begin(p) / 32 + k][q_lane];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t w = kc[j][Pt::begin(p) / 32 + k];
-          Frag f;
-          f.u[0] = two_values<DT, 0>(w, sc[j]);
-          f.u[1] = two_values<DT, 1>(w, sc[j]);
-          f.u[2] = two_values<DT, 2>(w, sc[j]);
-          f.u[3] = two_values<DT, 3>(w, sc[j]);
-#pragma unroll
-          for (int t = 0; t < NT; ++t) s[t][j] = mfma<DT>(f, q[t], s[t][j]);
-        }
-      }
-    }
-    if (more) load_keys(block_at(knext), int32_t((t1 + 4 * m) & (P - 1)));
+      for (int k = 0; k < KW; ++k)
+        if ((t * KW + k) % kWaves == wave) queries[t][k][ql] = q[t][k];
+    __syncthreads();
+    least = wave_min(least);
 
-    // token 16 g + 4 i + j of the tile is s[t][j][i]
-    const int32_t mine = int32_t(t0) + 16 * g;
-    const bool there = vpage >= 0 && vpage < a.table.num_pages;
-    const bool tail = t0 + kTile > least;
-    const bool masked = __any(!there || tail);
-    if (masked) {
-      const int32_t present = there ? int32_t(end) - mine : 0;
-      if (!there && mine < int32_t(end) && a.err) atomicOr(a.err, BPD_FLAG_PAGE_RANGE);
+    f32x4 acc[NT][VT];
+    float top[NT], sum[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      top[t] = -3e38f, sum[t] = 0.0f;
+#pragma unroll
+      for (int v = 0; v < VT; ++v) acc[t][v] = f32x4{0, 0, 0, 0};
+    }
+    int32_t nan_at[Pt::count];  // first token of the tail whose value group is bad, as a value lane
+#pragma unroll
+    for (int p = 0; p < Pt::count; ++p) nan_at[p] = kNever;
+    for (; tile < tile1; tile += kWaves) {
+      const int64_t t0 = int64_t(tile) * kTile, t1 = t0 + kWaves * kTile;
+      const bool more = tile + kWaves < tile1;
+      // read anew for every tile: the registers hold loads in flight instead
+      const int q_lane = here(lane);
+      f32x4 s[NT][4];
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
+        for (int j = 0; j < 4; ++j) s[t][j] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int p = 0; p < Pt::count; ++p) {
+        float sc[4];  // of the lane's group of channels, by token
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sc[j] = scale_at(ks, G * j + Pt::begin(p) / kKvGroup, G, ksel[p]);
+#pragma unroll
+        for (int k = 0; k < Pt::width(p) / 32; ++k) {
+          Frag q[NT];
+#pragma unroll
+          for (int t = 0; t < NT; ++t) q[t] = queries[t][Pt::begin(p) / 32 + k][q_lane];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t w = kc[j][Pt::begin(p) / 32 + k];
+            Frag f;
+            f.u[0] = two_values<DT, 0>(w, sc[j]);
+            f.u[1] = two_values<DT, 1>(w, sc[j]);
+            f.u[2] = two_values<DT, 2>(w, sc[j]);
+            f.u[3] = two_values<DT, 3>(w, sc[j]);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) s[t][j] = mfma<DT>(f, q[t], s[t][j]);
+          }
+        }
+      }
+      if (more) load_keys(block_at(knext), int32_t((t1 + 4 * m) & (P - 1)));
+
+      // token 16 g + 4 i + j of the tile is s[t][j][i]
+      const int32_t mine = int32_t(t0) + 16 * g;
+      const bool there = vpage >= 0 && vpage < a.table.num_pages;
+      const bool tail = t0 + kTile > least;
+      const bool masked = __any(!there || tail);
+      if (masked) {
+        const int32_t present = there ? int32_t(end) - mine : 0;
+        if (!there && mine < int32_t(end) && a.err) atomicOr(a.err, BPD_FLAG_PAGE_RANGE);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (4 * i + j >= (there ? sees[t] - mine : 0)) s[t][j][i] = -INFINITY;
+        // values that no query or not every query sees: nothing where there is
+        // no token, and bad groups are noted, so that a weight of 0 meets no NaN
+#pragma unroll
+        for (int u = 0; u < 16; ++u) {
+          const bool gone = u >= present;
+#pragma unroll
+          for (int p = 0; p < Pt::count; ++p) {
+            const int byte = G * u + Pt::begin(p) / kKvGroup;
+            const uint32_t e = float_bits(scale_at(vs, byte, kScaleWords, vsel[p])) >> 23;
+            if (e == kKvBadScale && !gone && tail) {
+              nan_at[p] = min(nan_at[p], mine + u);
+            }
+            if (gone || (e == kKvBadScale && tail)) {  // zeros, at a scale of one
+              vc[u][p] = 0;
+              const uint32_t at_byte = byte % 4 + (vsel[p] >> 24), put = 0xFFu << (8 * (at_byte & 3));
+              if (at_byte < 4) vs[byte / 4] = (vs[byte / 4] & ~put) | (put & 0x7F7F7F7Fu);
+              if (at_byte >= 4 && byte / 4 + 1 < kScaleWords)
+                vs[byte / 4 + 1] = (vs[byte / 4 + 1] & ~put) | (put & 0x7F7F7F7Fu);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float most_here = s[t][0][0];
+#pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (4 * i + j >= (there ? sees[t] - mine : 0)) s[t][j][i] = -INFINITY;
-      // values that no query or not every query sees: nothing where there is
-      // no token, and bad groups are noted, so that a weight of 0 meets no NaN
+          for (int i = 0; i < 4; ++i) most_here = fmaxf(most_here, s[t][j][i]);
+        most_here *= to_log2;
+        if (__any(most_here > top[t] + 8.0f)) {
+          float now = fmaxf(top[t], most_here);
+          now = fmaxf(now, __shfl_xor(now, 16));
+          now = fmaxf(now, __shfl_xor(now, 32));
+          const float keep = __builtin_amdgcn_exp2f(top[t] - now);
+          top[t] = now;
+          sum[t] *= keep;
 #pragma unroll
-      for (int u = 0; u < 16; ++u) {
-        const bool gone = u >= present;
+          for (int v = 0; v < VT; ++v)
 #pragma unroll
-        for (int p = 0; p < Pt::count; ++p) {
-          const int byte = G * u + Pt::begin(p) / kKvGroup;
-          const uint32_t e = float_bits(scale_at(vs, byte, kScaleWords, vsel[p])) >> 23;
-          if (e == kKvBadScale && !gone && tail) {
-            nan_at[p] = min(nan_at[p], mine + u);
-          }
-          if (gone || (e == kKvBadScale && tail)) {  // zeros, at a scale of one
-            vc[u][p] = 0;
-            const uint32_t at_byte = byte % 4 + (vsel[p] >> 24), put = 0xFFu << (8 * (at_byte & 3));
-            if (at_byte < 4) vs[byte / 4] = (vs[byte / 4] & ~put) | (put & 0x7F7F7F7Fu);
-            if (at_byte >= 4 && byte / 4 + 1 < kScaleWords)
-              vs[byte / 4 + 1] = (vs[byte / 4 + 1] & ~put) | (put & 0x7F7F7F7Fu);
-          }
+            for (int i = 0; i < 4; ++i) acc[t][v][i] *= keep;
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s[t][j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][i], to_log2, -top[t]));
+            sum[t] += s[t][j][i];
+          }
       }
-    }
+      // the weights, rounded to the type: tokens 8 h .. 8 h + 7 of the lane's 16
+      Frag w[NT][2];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      float most_here = s[t][0][0];
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) most_here = fmaxf(most_here, s[t][j][i]);
-      most_here *= to_log2;
-      if (__any(most_here > top[t] + 8.0f)) {
-        float now = fmaxf(top[t], most_here);
-        now = fmaxf(now, __shfl_xor(now, 16));
-        now = fmaxf(now, __shfl_xor(now, 32));
-        const float keep = __builtin_amdgcn_exp2f(top[t] - now);
-        top[t] = now;
-        sum[t] *= keep;
-#pragma unroll
-        for (int v = 0; v < VT; ++v)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[t][v][i] *= keep;
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[t][j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][i], to_log2, -top[t]));
-          sum[t] += s[t][j][i];
-        }
-    }
-    // the weights, rounded to the type: tokens 8 h .. 8 h + 7 of the lane's 16
-    Frag w[NT][2];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
+          for (int k = 0; k < 4; ++k)
+            w[t][h].u[k] = two_rounded<DT>(s[t][2 * (k & 1)][2 * h + (k >> 1)], s[t][2 * (k & 1) + 1][2 * h + (k >> 1)]);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          w[t][h].u[k] = two_rounded<DT>(s[t][2 * (k & 1)][2 * h + (k >> 1)], s[t][2 * (k & 1) + 1][2 * h + (k >> 1)]);
+        for (int p = 0; p < Pt::count; ++p) {
+          constexpr int kMost = 8;
+          Frag f[kMost];  // one value tile each: channels Pt::begin + row * (width / 16) + tile
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+          for (int k = 0; k < 4; ++k) {
+            const int u = 8 * h + 2 * k;
+            float sc[2];
 #pragma unroll
-      for (int p = 0; p < Pt::count; ++p) {
-        constexpr int kMost = 8;
-        Frag f[kMost];  // one value tile each: channels Pt::begin + row * (width / 16) + tile
+            for (int e = 0; e < 2; ++e)
+              sc[e] = scale_at(vs, G * (u + e) + Pt::begin(p) / kKvGroup, kScaleWords, vsel[p]);
+            const auto pair = [&](auto byte) {
+              constexpr int B = decltype(byte)::value;
+              if constexpr (2 * B < kMost) {
+                const uint32_t x0 = two_values<DT, B>(vc[u][p], sc[0]), x1 = two_values<DT, B>(vc[u + 1][p], sc[1]);
+                f[2 * B].u[k] = __builtin_amdgcn_perm(x1, x0, 0x05040100);
+                f[2 * B + 1].u[k] = __builtin_amdgcn_perm(x1, x0, 0x07060302);
+              }
+            };
+            pair(std::integral_constant<int, 0>());
+            if (Pt::width(p) >= 64) pair(std::integral_constant<int, 1>());
+            if (Pt::width(p) >= 128) pair(std::integral_constant<int, 2>()), pair(std::integral_constant<int, 3>());
+          }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int u = 8 * h + 2 * k;
-          float sc[2];
+          for (int v = 0; v < Pt::width(p) / 16; ++v)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            sc[e] = scale_at(vs, G * (u + e) + Pt::begin(p) / kKvGroup, kScaleWords, vsel[p]);
-          const auto pair = [&](auto byte) {
-            constexpr int B = decltype(byte)::value;
-            if constexpr (2 * B < kMost) {
-              const uint32_t x0 = two_values<DT, B>(vc[u][p], sc[0]), x1 = two_values<DT, B>(vc[u + 1][p], sc[1]);
-              f[2 * B].u[k] = __builtin_amdgcn_perm(x1, x0, 0x05040100);
-              f[2 * B + 1].u[k] = __builtin_amdgcn_perm(x1, x0, 0x07060302);
-            }
-          };
-          pair(std::integral_constant<int, 0>());
-          if (Pt::width(p) >= 64) pair(std::integral_constant<int, 1>());
-          if (Pt::width(p) >= 128) pair(std::integral_constant<int, 2>()), pair(std::integral_constant<int, 3>());
+            for (int t = 0; t < NT; ++t)
+              acc[t][Pt::begin(p) / 16 + v] = mfma<DT>(f[v], w[t][h], acc[t][Pt::begin(p) / 16 + v]);
         }
-#pragma unroll
-        for (int v = 0; v < Pt::width(p) / 16; ++v)
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-            acc[t][Pt::begin(p) / 16 + v] = mfma<DT>(f[v], w[t][h], acc[t][Pt::begin(p) / 16 + v]);
-      }
-    vpage = vnext;
-    if (more) load_values(block_at(vpage), int32_t((t1 + 16 * g) & (P - 1)));
-    const int64_t t2 = t1 + kWaves * kTile;
-    if (tile + 2 * kWaves < tile1) knext = page_at(t2 + (m >> 2) * 16), vnext = page_at(t2 + g * 16);
-  }
+      vpage = vnext;
+      if (more) load_values(block_at(vpage), int32_t((t1 + 16 * g) & (P - 1)));
+      const int64_t t2 = t1 + kWaves * kTile;
+      if (tile + 2 * kWaves < tile1) knext = page_at(t2 + (m >> 2) * 16), vnext = page_at(t2 + g * 16);
+    }
 
-  // bad value groups among the tokens that not every query sees
+    // bad value groups among the tokens that not every query sees
 #pragma unroll
-  for (int p = 0; p < Pt::count; ++p) {
-    if (!__any(nan_at[p] != kNever)) continue;
-    int32_t t = nan_at[p];
-    t = min(t, __shfl_xor(t, 16));
-    t = min(t, __shfl_xor(t, 32));
-    // rows 4 g .. 4 g + 3 of a value tile lie in one group: that of value lane 4 g
-    t = __shfl(t, 4 * g);
+    for (int p = 0; p < Pt::count; ++p) {
+      if (!__any(nan_at[p] != kNever)) continue;
+      int32_t t = nan_at[p];
+      t = min(t, __shfl_xor(t, 16));
+      t = min(t, __shfl_xor(t, 32));
+      // rows 4 g .. 4 g + 3 of a value tile lie in one group: that of value lane 4 g
+      t = __shfl(t, 4 * g);
 #pragma unroll
-    for (int c = 0; c < NT; ++c)
-      if (t < sees[c])
+      for (int c = 0; c < NT; ++c)
+        if (t < sees[c])
 #pragma unroll
-        for (int v = 0; v < Pt::width(p) / 16; ++v)
+          for (int v = 0; v < Pt::width(p) / 16; ++v)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[c][Pt::begin(p) / 16 + v][i] = bits_float(0x7FC00000u);
-  }
+            for (int i = 0; i < 4; ++i) acc[c][Pt::begin(p) / 16 + v][i] = bits_float(0x7FC00000u);
+    }
 
-  // join the waves: each takes its share of the value tiles
-  const int el = here(lane);
+    // join the waves: each takes its share of the value tiles
+    const int el = here(lane);
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    sum[t] += __shfl_xor(sum[t], 16);
-    sum[t] += __shfl_xor(sum[t], 32);
+    for (int t = 0; t < NT; ++t) {
+      sum[t] += __shfl_xor(sum[t], 16);
+      sum[t] += __shfl_xor(sum[t], 32);
 #pragma unroll
-    for (int v0 = 0; v0 < VT; v0 += kJoin) {
-      constexpr int kMine = kJoin / kWaves;
-      __syncthreads();
-      if (v0 == 0) tops[wave][el] = top[t], sums[wave][el] = sum[t];
+      for (int v0 = 0; v0 < VT; v0 += kJoin) {
+        constexpr int kMine = kJoin / kWaves;
+        __syncthreads();
+        if (v0 == 0) tops[wave][el] = top[t], sums[wave][el] = sum[t];
 #pragma unroll
-      for (int v = 0; v < kJoin; ++v) {
-        if (v0 + v < VT) joined[wave][v][el] = acc[t][v0 + v];
-      }
-      __syncthreads();
-      float now = tops[0][el], whole = 0.0f, f[kWaves];
+        for (int v = 0; v < kJoin; ++v) {
+          if (v0 + v < VT) joined[wave][v][el] = acc[t][v0 + v];
+        }
+        __syncthreads();
+        float now = tops[0][el], whole = 0.0f, f[kWaves];
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) now = fmaxf(now, tops[w][el]);
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        f[w] = __builtin_amdgcn_exp2f(tops[w][el] - now);
-        whole += sums[w][el] * f[w];
-      }
-      f32x4 mine[kMine];
-#pragma unroll
-      for (int k = 0; k < kMine; ++k) {
-        mine[k] = f32x4{0, 0, 0, 0};
+        for (int w = 1; w < kWaves; ++w) now = fmaxf(now, tops[w][el]);
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-          const f32x4 y = joined[w][wave * kMine + k][el];
+          f[w] = __builtin_amdgcn_exp2f(tops[w][el] - now);
+          whole += sums[w][el] * f[w];
+        }
+        f32x4 mine[kMine];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mine[k][i] += y[i] * f[w];
+        for (int k = 0; k < kMine; ++k) {
+          mine[k] = f32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int w = 0; w < kWaves; ++w) {
+            const f32x4 y = joined[w][wave * kMine + k][el];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mine[k][i] += y[i] * f[w];
+          }
+        }
+        const int v = v0 + wave * kMine;  // the first of the wave's value tiles
+        if (v >= VT) continue;
+        const int32_t column = t * 16 + (el & 15);
+        if (n_here == tiles) {
+          const int32_t c = group * plan.cols + column;
+          const int32_t i = c / share, h = kvh * share + c % share;
+          if (column >= plan.cols || i >= a.tokens) continue;
+          store_columns<DT, D, kMine>(a.out + ((b * a.tokens + i) * a.heads + h) * D, v, el >> 4, mine,
+                                      whole == 0.0f ? 0.0f : 1.0f / whole);
+        } else {
+          const int64_t piece = 2 * int64_t(blockIdx.x) + (pos == begin ? 0 : 1);
+          float* to = plan.partials + (piece * NT + t) * ((2 + 4 * VT) * kWave);
+          if (v == 0) to[el] = now, to[kWave + el] = whole;
+#pragma unroll
+          for (int k = 0; k < kMine; ++k)
+            if (v + k < VT) *reinterpret_cast<f32x4*>(to + 2 * kWave + ((v + k) * kWave + el) * 4) = mine[k];
         }
       }
-      const int v = v0 + wave * kMine;  // the first of the wave's value tiles
-      if (v >= VT) continue;
-      const int32_t column = t * 16 + (el & 15);
-      if (n_here == tiles) {
-        const int32_t c = group * plan.cols + column;
-        const int32_t i = c / share, h = kvh * share + c % share;
-        if (column >= plan.cols || i >= a.tokens) continue;
-        store_columns<DT, D, kMine>(a.out + ((b * a.tokens + i) * a.heads + h) * D, v, el >> 4, mine,
-                                    whole == 0.0f ? 0.0f : 1.0f / whole);
-      } else {
-        const int64_t piece = 2 * int64_t(blockIdx.x) + (pos == begin ? 0 : 1);
-        float* to = plan.partials + (piece * NT + t) * ((2 + 4 * VT) * kWave);
-        if (v == 0) to[el] = now, to[kWave + el] = whole;
-#pragma unroll
-        for (int k = 0; k < kMine; ++k)
-          if (v + k < VT) *reinterpret_cast<f32x4*>(to + 2 * kWave + ((v + k) * kWave + el) * 4) = mine[k];
-      }
     }
-  }
-  pos += n_here;
-  if (pos >= stop) break;
-  tile0 = 0;
-  if (++unit == units) unit = 0, tiles = tiles_of(a, ++b);
-  __syncthreads();
+    pos += n_here;
+    if (pos >= stop) break;
+    tile0 = 0;
+    if (++unit == units) unit = 0, tiles = tiles_of(a, ++b);
+    __syncthreads();
   }
 }
 

@@ -674,7 +674,9 @@ int bpd_soft_prior_noalloc(float* logits, int64_t rows, int64_t vocab, int64_t l
  * drafts + 1], the row of allow_bits of each position (-1: allows nothing).
  * NULL allow_bits: every token is allowed.  A drafted token outside
  * [0, vocab) does not stand (BPD_FLAG_TOKEN_RANGE); a state at or above
- * num_states allows nothing (BPD_FLAG_STATE_RANGE).  tokens: int32 or int64,
+ * num_states allows nothing (BPD_FLAG_STATE_RANGE).  Flags are those of the
+ * position that decides the block; what follows it is not looked at.  Rows may
+ * lie at any element.  tokens: int32 or int64,
  * row stride tokens_ld; temperature float [rows] on the device, or NULL and
  * temperature_all.  workspace: bpd_verify_workspace_bytes bytes, 16-byte
  * aligned.  No counterpart in the reference, which samples one token per
@@ -725,7 +727,8 @@ int bpd_host_verify(const void* logits, int dtype, int64_t rows, int32_t drafts,
  * Two requests must not append to one page.
  * bpd_kv_read: tokens starts[b] + i, i < counts[b], back as k_out and v_out
  * [rows, tokens, kv_heads, head_dim] contiguous; zeros past counts[b] and for
- * tokens outside the tables. */
+ * tokens outside the tables.  q_out, k_out and v_out lie at multiples of 16
+ * bytes; k, v and q at any element. */
 int bpd_kv_append(uint8_t* pages, int64_t num_pages, int32_t page_size, int32_t kv_heads,
                   int32_t head_dim, int dtype, const void* k, int64_t k_row, int64_t k_token,
                   int64_t k_head, const void* v, int64_t v_row, int64_t v_token, int64_t v_head,
@@ -760,7 +763,9 @@ int bpd_host_kv_read(const uint8_t* pages, int64_t num_pages, int32_t page_size,
  * request whose own keys are already appended: query i sees the first
  * lengths[b] - n + 1 + i tokens, lengths[b] counting the block.  Zeros for a
  * query that sees nothing and for those past n.  Query head h reads key head
- * h / (heads / kv_heads).  Softmax statistics and sums in float.  workspace:
+ * h / (heads / kv_heads).  Softmax statistics and sums in float, weights
+ * rounded to the cache's type once.  out lies at a multiple of 4 bytes.
+ * workspace:
  * bpd_kv_attend_workspace_bytes bytes for `longest` = table_blocks *
  * page_size, 16-byte aligned (NULL where that is 0). */
 size_t bpd_kv_attend_workspace_bytes(int64_t rows, int32_t tokens, int32_t heads,
