@@ -755,8 +755,10 @@ __global__ __launch_bounds__(kThreads* Runs) void verify_pick_kernel(VerifyArgs 
         end = int32_t(t) + j;
         if (at > target && hit == 0x7FFFFFFF) hit = end;
       }
-      if (hit != 0x7FFFFFFF) atomicMin(&found, hit);
-      if (end >= 0) atomicMax(&last, end);
+      // tokens rise with the lanes: one of a wave speaks for it
+      const uint64_t hits = __ballot(hit != 0x7FFFFFFF), some = __ballot(end >= 0);
+      if (hits && lane == __builtin_ctzll(hits)) atomicMin(&found, hit);
+      if (some && lane == 63 - __builtin_clzll(some)) atomicMax(&last, end);
       __syncthreads();
       if (last >= 0) break;
     }
