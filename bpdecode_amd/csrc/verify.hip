@@ -580,10 +580,12 @@ __device__ __forceinline__ Deciding deciding(const VerifyArgs& a, int64_t b, int
 }
 
 // The sums of a chunk of a request's deciding row, one block each: about 40
-// vector instructions a token, most of them in 64 bits, which is its bound (256
-// rows of 151,936 bf16 with bf16 probabilities: 52 us).  With few
-// requests (kShortRuns) every block forms the verdicts for itself: a launch
-// less.
+// vector instructions a token, most of them in 64 bits, which is its bound.
+// Where a grammar leaves every lane of a wave at most a quarter of its tokens,
+// these alone are loaded, all at once, and summed one by one (256 rows of 151,936
+// bf16 with bf16 probabilities under grammars that allow 0.0002 to 0.95 of the
+// tokens: 39 us, and 53 where every lane sums all of them).  With few requests
+// (kShortRuns) every block forms the verdicts for itself: a launch less.
 template <int DT, int Runs>
 __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a, Space w) {
   __shared__ double sums[kWaves][4];
@@ -604,42 +606,66 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a, Spa
   if (st.empty || !(temperature_of(a, b) > 0.0)) return;
   const Deciding d = deciding(a, b, n, st);
   const bool less = n < draft_len(a, b);
+  double s[4] = {0.0, 0.0, 0.0, 0.0};
+  // a token's weight, and where the draft's probabilities come off, its p
+  const auto add = [&](double x, double p) {
+    const double y = x - p * st.sum;
+    s[1] += y > 0.0 ? x : 0.0;
+    s[2] += y > 0.0 ? p : 0.0;
+    s[3] += fabs(y) <= kSumError * x ? x : 0.0;
+  };
+  uint32_t all_bits = 0;  // of the runs, eight each
+#pragma unroll
+  for (int k = 0; k < Runs; ++k)
+    all_bits |= run_bits(a, d.state, run_at((int64_t(chunk) * Runs + k) * (kThreads * kRun) + tid * kRun, a.vocab))
+                << (8 * k);
+  constexpr int kFew = 2 * Runs;
+  const int allowed_here = __popc(all_bits);
+  const bool few = a.allow_bits && !__any(allowed_here > kFew);
+  if (few && __any(allowed_here > 0)) {
+    float z[kFew], q[kFew];
+#pragma unroll
+    for (int k = 0; k < kFew; ++k) {
+      const bool on = all_bits != 0;
+      const int bit = on ? __builtin_ctz(all_bits) : 0;
+      all_bits &= all_bits - 1;
+      const int64_t t = run_at((int64_t(chunk) * Runs + bit / 8) * (kThreads * kRun) + tid * kRun, a.vocab).t + bit % 8;
+      z[k] = on ? load_elem(d.row, DT, t) : -INFINITY;
+      q[k] = !on ? 0.0f : d.probs ? load_elem(d.probs, a.probs_dtype, t) : t == d.drafted ? 2.0f : 0.0f;
+    }
+#pragma unroll 1
+    for (int k = 0; k < kFew; ++k) {
+      if (!__any(k < allowed_here)) break;
+      const double x = exp2_down((double(z[0]) - d.top) * d.to_log2);
+      s[0] += x;
+      if (less) add(x, q[0]);
+#pragma unroll
+      for (int l = 1; l < kFew; ++l) z[l - 1] = z[l], q[l - 1] = q[l];
+    }
+  }
   // One run at a time leaves seven waves on a SIMD, which hide its loads better
   // than two or four runs in flight do (57, 60 and 66 us: 256 rows of 151,936
-  // bf16 with bf16 probabilities).
-  constexpr int kAtOnce = 1;
-  double s[4] = {0.0, 0.0, 0.0, 0.0};
+  // bf16 with bf16 probabilities, every token summed).
 #pragma unroll 1
-  for (int k0 = 0; k0 < Runs; k0 += kAtOnce) {
-    Run runs[kAtOnce];
-    float z[kAtOnce][kRun], q[kAtOnce][kRun];
+  for (int k0 = 0; k0 < Runs && !few; ++k0, all_bits >>= 8) {
+    const Run run[1] = {run_at((int64_t(chunk) * Runs + k0) * (kThreads * kRun) + tid * kRun, a.vocab)};
+    const uint32_t bits = all_bits & 0xFFu;
+    if (!__any(bits != 0)) continue;
+    float z[1][kRun], q[1][kRun];
+    load_runs<DT>(d.row, run, a.vocab, z);
+    if (d.probs) draft_runs(a, d, run, q);
+    double x[kRun];
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k)
-      runs[k] = run_at((int64_t(chunk) * Runs + k0 + k) * (kThreads * kRun) + tid * kRun, a.vocab);
-    load_runs<DT>(d.row, runs, a.vocab, z);
-    if (d.probs) draft_runs(a, d, runs, q);
+    for (int j = 0; j < kRun; ++j) {
+      x[j] = exp2_down((double(masked(z[0][j], bits, j)) - d.top) * d.to_log2);
+      s[0] += x[j];
+    }
+    if (d.probs) {
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      const uint32_t bits = run_bits(a, d.state, runs[k]);
-      if (!__any(bits != 0)) continue;
-      double x[kRun];
+      for (int j = 0; j < kRun; ++j) add(x[j], q[0][j]);
+    } else if (less) {  // all but the drafted token
 #pragma unroll
-      for (int j = 0; j < kRun; ++j) {
-        x[j] = exp2_down((double(masked(z[k][j], bits, j)) - d.top) * d.to_log2);
-        s[0] += x[j];
-      }
-      if (d.probs) {
-#pragma unroll
-        for (int j = 0; j < kRun; ++j) {
-          const double p = q[k][j], y = x[j] - p * st.sum;
-          s[1] += y > 0.0 ? x[j] : 0.0;
-          s[2] += y > 0.0 ? p : 0.0;
-          s[3] += fabs(y) <= kSumError * x[j] ? x[j] : 0.0;
-        }
-      } else if (less) {  // all but the drafted token
-#pragma unroll
-        for (int j = 0; j < kRun; ++j) s[1] += runs[k].t + j == d.drafted ? 0.0 : x[j];
-      }
+      for (int j = 0; j < kRun; ++j) s[1] += run[0].t + j == d.drafted ? 0.0 : x[j];
     }
   }
 #pragma unroll
@@ -657,7 +683,7 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a, Spa
 }
 
 // The next token, one block per request, a run of the chunk per thread: a chain
-// of loads that wait for each other (9 us for a short chunk, 14 for a long one).
+// of loads that wait for each other (5 us for a short chunk, 8 to 10 for a long one).
 template <int DT, int Runs>
 __global__ __launch_bounds__(kThreads* Runs) void verify_pick_kernel(VerifyArgs a, Space w) {
   constexpr int N = kWaves * Runs;

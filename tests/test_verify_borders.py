@@ -69,7 +69,7 @@ def test_vocabularies_about_the_width_of_a_run_and_a_chunk(V, device):
 
 @pytest.mark.parametrize("device", DEVICES)
 def test_long_chunks_with_odd_rows_and_a_grammar(device):
-    """More than 4 Mi tokens of positions: the verdicts take a launch."""
+    """Rows that begin at any element, with and without probabilities."""
     V = 70_001
     st = inputs(17, 3, V, V, torch.float16, torch.bfloat16, 33, True)
     st["uniforms"][:, 0] *= 0.3
@@ -94,6 +94,26 @@ def test_temperatures_at_the_ends_of_their_range(device):
     st["tokens"][:, 0] = 8
     check(call(st, V, device), reference(st, V))
     st["logits"] = torch.where(torch.arange(V) % 3 == 0, torch.finfo(torch.float32).min, -3.0e38).expand(6, 3, V).contiguous()
+    check(call(st, V, device), reference(st, V))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("B, V", [(5, 5_001), (21, 100_003)])  # the verdicts in the sums' launch, in their own
+def test_grammars_that_leave_few_tokens(B, V, device):
+    """Two of eight tokens, of which the first weighs nothing; then wider masks
+    here and there, and stretches without any token."""
+    st = inputs(B, 3, V, V, torch.bfloat16, torch.bfloat16, 36, True)
+    st["uniforms"][:, 0] *= 0.3
+    t = torch.arange(V)
+    every = st["tok_next"].clamp(min=0)
+    two = (t % 8 == 1) | (t % 8 == 4)
+    st["logits"][:, :, 1::8] = -float("inf")
+    st["tok_next"] = torch.where(two, every, -1)
+    check(call(st, V, device), reference(st, V))
+    mixed = torch.where(t % 3_000 < 40, True, two) & (t // 2_500 % 2 == 1)
+    st["tok_next"] = torch.where(mixed, every, -1)
+    check(call(st, V, device), reference(st, V))
+    st["probs"] = None
     check(call(st, V, device), reference(st, V))
 
 
