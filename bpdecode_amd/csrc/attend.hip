@@ -46,7 +46,7 @@ __host__ __device__ __forceinline__ int64_t seen_tokens(const AttendArgs& a, int
 
 constexpr int kWave = 64;
 constexpr int kTile = 64;   // cache tokens that a wave takes at a time
-constexpr int kWaves = 4;   // waves of a block
+constexpr int kWaves = 4;   // waves of a block, but for blocks that have a CU to themselves
 constexpr int kManyWaves = 16, kManyPieces = 16;  // of a join of that many pieces a unit
 constexpr int kNever = 0x7FFFFFFF;
 
@@ -222,14 +222,15 @@ __device__ __forceinline__ int here(int x) {
 // which two or three waves on a SIMD issue one in five cycles (64 blocks of 5
 // drafts over up to 4,096 tokens: 220 MB in 57 us).  A block that finds
 // nothing to do takes 5 us, each of its first tiles 1.4.
-template <int DT, int D, int NT>
-__global__ __launch_bounds__(kWaves* kWave, attend_blocks(D, NT)) void kv_attend_kernel(AttendArgs a, AttendPlan plan) {
+template <int DT, int D, int NT, int W>
+__global__ __launch_bounds__(W* kWave, W == kWaves ? attend_blocks(D, NT) : 1) void kv_attend_kernel(AttendArgs a,
+                                                                                                 AttendPlan plan) {
   using Pt = Parts<D>;
   constexpr int G = D / kKvGroup, KW = D / 32, VT = D / 16;  // scales, key words of a lane, value tiles
   constexpr int kScaleWords = 4 * G;                          // of 16 tokens
-  constexpr int kJoin = VT <= kWaves ? kWaves : 2 * kWaves;   // value tiles joined at a time
-  __shared__ f32x4 joined[kWaves][kJoin][kWave];
-  __shared__ float tops[kWaves][kWave], sums[kWaves][kWave];
+  constexpr int kJoin = VT <= W ? VT : W == kWaves ? 2 * W : W;  // value tiles joined at a time
+  __shared__ f32x4 joined[W][kJoin][kWave];
+  __shared__ float tops[W][kWave], sums[W][kWave];
   __shared__ Frag queries[NT][KW][kWave];  // as the lanes of every wave take them
 
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -344,7 +345,7 @@ __global__ __launch_bounds__(kWaves* kWave, attend_blocks(D, NT)) void kv_attend
         for (int k = 0; k < Pt::width(p) / 32; ++k) {
           const uint16_t* from = row + Pt::begin(p) + (ql >> 4) * (Pt::width(p) / 4) + 8 * k;
           Frag f = {{0u, 0u, 0u, 0u}};
-          if (in && a.scale != 0.0f && (t * KW + Pt::begin(p) / 32 + k) % kWaves == wave) __builtin_memcpy(&f, from, 16);  // at any element
+          if (in && a.scale != 0.0f && (t * KW + Pt::begin(p) / 32 + k) % W == wave) __builtin_memcpy(&f, from, 16);  // at any element
           if (a.scale < 0.0f)
 #pragma unroll
             for (int j = 0; j < 4; ++j) f.u[j] ^= 0x80008000u;
@@ -355,14 +356,14 @@ __global__ __launch_bounds__(kWaves* kWave, attend_blocks(D, NT)) void kv_attend
       const int64_t t0 = int64_t(tile) * kTile;
       load_keys(block_at(kpage), int32_t((t0 + 4 * m) & (P - 1)));
       load_values(block_at(vpage), int32_t((t0 + 16 * g) & (P - 1)));
-      const int64_t t1 = t0 + kWaves * kTile;
-      if (tile + kWaves < tile1) knext = page_at(t1 + (m >> 2) * 16), vnext = page_at(t1 + g * 16);
+      const int64_t t1 = t0 + W * kTile;
+      if (tile + W < tile1) knext = page_at(t1 + (m >> 2) * 16), vnext = page_at(t1 + g * 16);
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int k = 0; k < KW; ++k)
-        if ((t * KW + k) % kWaves == wave) queries[t][k][ql] = q[t][k];
+        if ((t * KW + k) % W == wave) queries[t][k][ql] = q[t][k];
     __syncthreads();
     least = wave_min(least);
 
@@ -377,9 +378,9 @@ __global__ __launch_bounds__(kWaves* kWave, attend_blocks(D, NT)) void kv_attend
     int32_t nan_at[Pt::count];  // first token of the tail whose value group is bad, as a value lane
 #pragma unroll
     for (int p = 0; p < Pt::count; ++p) nan_at[p] = kNever;
-    for (; tile < tile1; tile += kWaves) {
-      const int64_t t0 = int64_t(tile) * kTile, t1 = t0 + kWaves * kTile;
-      const bool more = tile + kWaves < tile1;
+    for (; tile < tile1; tile += W) {
+      const int64_t t0 = int64_t(tile) * kTile, t1 = t0 + W * kTile;
+      const bool more = tile + W < tile1;
       // read anew for every tile: the registers hold loads in flight instead
       const int q_lane = here(lane);
       f32x4 s[NT][4];
@@ -519,8 +520,8 @@ __global__ __launch_bounds__(kWaves* kWave, attend_blocks(D, NT)) void kv_attend
         }
       vpage = vnext;
       if (more) load_values(block_at(vpage), int32_t((t1 + 16 * g) & (P - 1)));
-      const int64_t t2 = t1 + kWaves * kTile;
-      if (tile + 2 * kWaves < tile1) knext = page_at(t2 + (m >> 2) * 16), vnext = page_at(t2 + g * 16);
+      const int64_t t2 = t1 + W * kTile;
+      if (tile + 2 * W < tile1) knext = page_at(t2 + (m >> 2) * 16), vnext = page_at(t2 + g * 16);
     }
 
     // bad value groups among the tokens that not every query sees
@@ -549,7 +550,7 @@ __global__ __launch_bounds__(kWaves* kWave, attend_blocks(D, NT)) void kv_attend
       sum[t] += __shfl_xor(sum[t], 32);
 #pragma unroll
       for (int v0 = 0; v0 < VT; v0 += kJoin) {
-        constexpr int kMine = kJoin / kWaves;
+        constexpr int kMine = kJoin > W ? kJoin / W : 1;
         __syncthreads();
         if (v0 == 0) tops[wave][el] = top[t], sums[wave][el] = sum[t];
 #pragma unroll
@@ -557,11 +558,13 @@ __global__ __launch_bounds__(kWaves* kWave, attend_blocks(D, NT)) void kv_attend
           if (v0 + v < VT) joined[wave][v][el] = acc[t][v0 + v];
         }
         __syncthreads();
-        float now = tops[0][el], whole = 0.0f, f[kWaves];
+        const int v = v0 + wave * kMine;  // the first of the wave's value tiles
+        if (wave * kMine >= kJoin || v >= VT) continue;
+        float now = tops[0][el], whole = 0.0f, f[W];
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) now = fmaxf(now, tops[w][el]);
+        for (int w = 1; w < W; ++w) now = fmaxf(now, tops[w][el]);
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = 0; w < W; ++w) {
           f[w] = __builtin_amdgcn_exp2f(tops[w][el] - now);
           whole += sums[w][el] * f[w];
         }
@@ -570,14 +573,12 @@ __global__ __launch_bounds__(kWaves* kWave, attend_blocks(D, NT)) void kv_attend
         for (int k = 0; k < kMine; ++k) {
           mine[k] = f32x4{0, 0, 0, 0};
 #pragma unroll
-          for (int w = 0; w < kWaves; ++w) {
+          for (int w = 0; w < W; ++w) {
             const f32x4 y = joined[w][wave * kMine + k][el];
 #pragma unroll
             for (int i = 0; i < 4; ++i) mine[k][i] += y[i] * f[w];
           }
         }
-        const int v = v0 + wave * kMine;  // the first of the wave's value tiles
-        if (v >= VT) continue;
         const int32_t column = t * 16 + (el & 15);
         if (n_here == tiles) {
           const int32_t c = group * plan.cols + column;
@@ -693,7 +694,7 @@ __global__ __launch_bounds__(W* kWave) void kv_attend_join_kernel(AttendArgs a, 
 
 struct AttendSizes {
   AttendPlan plan;
-  int32_t nt;
+  int32_t nt, waves;
   int64_t tiles;  // at most, over all units
   int32_t blocks;  // that the device holds at a time
   size_t piece;   // floats of a unit's piece
@@ -705,6 +706,15 @@ constexpr int kCus = 256;
 // 512 units of 4,000 tokens: 50 and 59, of 8,000: 92 and 99; 128 units of
 // 4,000 (a sixth of the device): 30 and 26.
 constexpr int kShort = 16, kMiddling = 128;
+// Waves of a block that has a CU to itself: units no more than CUs, and no more
+// than a fourth as many tiles as there are units, for which runs with their
+// join take longer.  One token, 32 heads of 128, lengths down to a half, runs and
+// this: 9 requests of 1,100 tokens 16.0 and 11.6 us, 16 of 2,000 21.9 and 16.4, 32 of
+// 4,000 32.4 and 26.2 (one of them 4,000 and the others 500: 17.1 and 24.0), 4 of
+// 4,000 (not taken) 18.7 and 23.2; five tokens: 28.7 and 21.3, 39.1 and 34.2 for
+// 16 and 32; heads of 64: 17.9 and 12.9, 25.3 and 20.0.  Up to kShort tiles four waves
+// do as well (16 of 1,000: 12.2 and 11.6, five tokens 15.3 and 16.0).
+constexpr int kUnitWaves = 8;
 
 AttendSizes attend_sizes(int64_t rows, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t dim, int64_t longest) {
   AttendSizes z{};
@@ -723,7 +733,10 @@ AttendSizes attend_sizes(int64_t rows, int32_t tokens, int32_t heads, int32_t kv
   // one block per unit where that fills half the device with units of a
   // middling length, or where units are short: nothing is searched or joined
   const int64_t units = rows * kv_heads * z.plan.groups;
-  z.plan.blocks = per_unit <= kShort || (per_unit <= kMiddling && 2 * units >= z.blocks) ? 0 : z.blocks;
+  const bool alone =
+      units <= kCus && per_unit > kShort && 4 * per_unit <= units && attend_blocks(dim, z.nt) >= kUnitWaves / kWaves;
+  z.waves = alone ? kUnitWaves : kWaves;
+  z.plan.blocks = alone || per_unit <= kShort || (per_unit <= kMiddling && 2 * units >= z.blocks) ? 0 : z.blocks;
   z.piece = size_t(z.nt) * (2 + dim / 4) * kWave;
   return z;
 }
@@ -739,7 +752,11 @@ int launch_attend(const AttendArgs& a, const AttendSizes& z, hipStream_t s) {
   const int64_t joins = a.rows * a.kv_heads * z.plan.groups * NT * (D / 32);
   BPD_REQUIRE(z.tiles < (int64_t(1) << 31) && joins < (int64_t(1) << 31), "too many queries or tokens in one call");
   const int64_t blocks = z.plan.blocks ? attend_runs(z, a.rows) : a.rows * a.kv_heads * z.plan.groups;
-  kv_attend_kernel<DT, D, NT><<<uint32_t(blocks), kWaves * kWave, 0, s>>>(a, z.plan);
+  if constexpr (attend_blocks(D, NT) >= kUnitWaves / kWaves) {
+    if (z.waves == kUnitWaves)
+      kv_attend_kernel<DT, D, NT, kUnitWaves><<<uint32_t(blocks), kUnitWaves * kWave, 0, s>>>(a, z.plan);
+  }
+  if (z.waves == kWaves) kv_attend_kernel<DT, D, NT, kWaves><<<uint32_t(blocks), kWaves * kWave, 0, s>>>(a, z.plan);
   // few units have many pieces each: more waves to a unit's join
   if (z.plan.blocks >= kManyPieces * a.rows * a.kv_heads * z.plan.groups)
     kv_attend_join_kernel<DT, D, NT, kManyWaves><<<uint32_t(joins), kManyWaves * kWave, 0, s>>>(a, z.plan);

@@ -50,6 +50,35 @@ def test_cuts_against_plain_form(case, device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("T", [1, 17])
+@pytest.mark.parametrize("D", [64, 96, 128, 192, 256])
+def test_units_no_more_than_compute_units(D, T, device):
+    """72 units of up to 18 tiles: one wide block each, two column tiles with 17
+    tokens; a request without tokens, one that ends inside its first tile, one
+    in its last; a bad value group in the third's last token."""
+    print(f"units of {D} channels, {T} tokens on {device}", flush=True)
+    KV, P, lengths = 24, 16, [0, T + 3, 1_097]
+    g = torch.Generator().manual_seed(90 + D + T)
+    cache, table = filled_cache(g, 3, P, KV, D, BF16, 69, device, 12)
+    k, v = stored(cache, table, max(lengths))
+    for b, n in enumerate(lengths):
+        table[b, (n + P - 1) // P:] = -1
+    q = (1.2 * torch.randn(3, T, KV, D, generator=g)).to(BF16)
+    call = lambda: cache.attend(q.to(device), table.to(device),  # noqa: E731
+                                torch.tensor(lengths, dtype=torch.int32, device=device))
+    good = call()
+    close(good, *R.attend(q.double().numpy(), k, v, lengths, BF16))
+    cache.check_errors()
+    at = P * D + P * (D // 32) + (lengths[2] - 1) % P * (D // 32)  # the value scales of that token
+    cache.pages[int(table[2, 68]), 5, at] = 255
+    bad = call().cpu()
+    nan = torch.zeros(bad.shape, dtype=torch.bool)
+    nan[2, T - 1, 5, :32] = True
+    assert torch.equal(torch.isnan(bad), nan)
+    assert torch.equal(bad[~nan], good.cpu()[~nan])
+
+
+@pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("D", [64, 96, 128, 192, 256])
 def test_a_bad_value_shows_only_where_its_token_is_seen(D, device):
     """A value group of infinities in a token that the last query alone sees:
