@@ -584,8 +584,12 @@ __global__ __launch_bounds__(W* kWave, W == kWaves ? attend_blocks(D, NT) : 1) v
           const int32_t c = group * plan.cols + column;
           const int32_t i = c / share, h = kvh * share + c % share;
           if (column >= plan.cols || i >= a.tokens) continue;
+          // a row past the request's queries has summed what no mask kept out
+          if (i >= n_q)
+#pragma unroll
+            for (int k = 0; k < kMine; ++k) mine[k] = f32x4{0, 0, 0, 0};
           store_columns<DT, D, kMine>(a.out + ((b * a.tokens + i) * a.heads + h) * D, v, el >> 4, mine,
-                                      whole == 0.0f ? 0.0f : 1.0f / whole);
+                                      whole == 0.0f || i >= n_q ? 0.0f : 1.0f / whole);
         } else {
           const int64_t piece = 2 * int64_t(blockIdx.x) + (pos == begin ? 0 : 1);
           float* to = plan.partials + (piece * NT + t) * ((2 + 4 * VT) * kWave);
@@ -688,8 +692,10 @@ __global__ __launch_bounds__(W* kWave) void kv_attend_join_kernel(AttendArgs a, 
   const int32_t c = unit % plan.groups * plan.cols + column;
   const int32_t i = c / share, h = unit / plan.groups * share + c % share;
   if (column >= plan.cols || i >= a.tokens) return;
+  const bool none = i >= queries_of(a, b);
+  if (none) acc[0] = acc[1] = f32x4{0, 0, 0, 0};
   store_columns<DT, D, 2>(a.out + ((b * a.tokens + i) * a.heads + h) * D, v0, lane >> 4, acc,
-                          sum == 0.0f ? 0.0f : 1.0f / sum);
+                          none || sum == 0.0f ? 0.0f : 1.0f / sum);
 }
 
 struct AttendSizes {
