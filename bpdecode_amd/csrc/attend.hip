@@ -50,6 +50,11 @@ constexpr int kWaves = 4;   // waves of a block, but for blocks that have a CU t
 constexpr int kManyWaves = 16, kManyPieces = 16;  // of a join of that many pieces a unit
 constexpr int kNever = 0x7FFFFFFF;
 
+// The power of two at which a row's largest weight stands when its maximum is
+// taken up: with the 2^8 that it may grow by, the largest that float16 holds.
+template <int DT>
+constexpr float kLift = DT == BPD_DTYPE_F16 ? 7.0f : 0.0f;
+
 // How a call's work is cut.  A unit is one request, one key head and one group
 // of query columns (tokens x heads that share the key head); all units' tiles
 // stand in one row, request by request, and every block takes an equal run of
@@ -205,11 +210,16 @@ __device__ __forceinline__ int here(int x) {
 // product takes values with channels as rows: lane (m, g) loads the channels
 // of row m, next to each other, of the tokens from 16 g, converts two codes
 // of a token at a time and swaps halves with the next token's.
-// The running maximum is followed loosely: weights may grow to 2^8 before the
+// The running maximum is followed loosely: weights may grow by 2^8 before the
 // sums are scaled down, so most tiles cost no exchange between lanes.  Scores,
 // maximum, sums and the accumulated values are floats; the weights are rounded
-// to the cache's type for the second product, half a step of which is all that
-// is lost (the values themselves are exact in it).
+// to the cache's type, because the second product takes its operands in 16
+// bits (the values themselves are exact in them): half a step of a weight,
+// which the division's unrounded sum does not follow.  In float16 a row's
+// largest weight lies between kLift and kLift + 8 powers of two, so that
+// weights down to 2^-21 of it keep all their bits, and those below are off by
+// 2^-32 of it at most (with the largest at 1, those 2^-24 below, 17 nats,
+// would lose half of themselves or all).
 //
 // (The product that takes codes and scales as they are, fp4 by fp8, was left:
 // of 8 neighbouring products it keeps bits down to 2^-13 of the largest, and
@@ -458,8 +468,9 @@ __global__ __launch_bounds__(W* kWave, W == kWaves ? attend_blocks(D, NT) : 1) v
 #pragma unroll
           for (int i = 0; i < 4; ++i) most_here = fmaxf(most_here, s[t][j][i]);
         most_here *= to_log2;
-        if (__any(most_here > top[t] + 8.0f)) {
-          float now = fmaxf(top[t], most_here);
+        // (top[t] is the exponent that counts as 0, kLift below a maximum)
+        if (__any(most_here > top[t] + (kLift<DT> + 8.0f))) {
+          float now = fmaxf(top[t], most_here - kLift<DT>);
           now = fmaxf(now, __shfl_xor(now, 16));
           now = fmaxf(now, __shfl_xor(now, 32));
           const float keep = __builtin_amdgcn_exp2f(top[t] - now);

@@ -764,10 +764,10 @@ int bpd_host_kv_read(const uint8_t* pages, int64_t num_pages, int32_t page_size,
  * lengths[b] - n + 1 + i tokens, lengths[b] counting the block.  Zeros for a
  * query that sees nothing and for those past n.  Query head h reads key head
  * h / (heads / kv_heads).  Softmax statistics and sums in float, weights
- * rounded to the cache's type once.  out lies at a multiple of 4 bytes.
- * workspace:
- * bpd_kv_attend_workspace_bytes bytes for `longest` = table_blocks *
- * page_size, 16-byte aligned (NULL where that is 0). */
+ * rounded to the cache's type once (to nearest; float16 weights below 2^-21 of
+ * their row's largest to 2^-31 of it).  out lies at a multiple of 4 bytes.
+ * workspace: bpd_kv_attend_workspace_bytes bytes for `longest` =
+ * table_blocks * page_size, 16-byte aligned (NULL where that is 0). */
 size_t bpd_kv_attend_workspace_bytes(int64_t rows, int32_t tokens, int32_t heads,
                                      int32_t kv_heads, int32_t head_dim, int64_t longest);
 int bpd_kv_attend(const uint8_t* pages, int64_t num_pages, int32_t page_size, int32_t kv_heads,
