@@ -208,6 +208,15 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def err_ptr(err: torch.Tensor | None, device: torch.device) -> int | None:
+    """Address of a call's error word, which kernels write to."""
+    if err is None:
+        return None
+    if err.dtype is not torch.int32 or err.device != device or err.numel() < 1:
+        raise RuntimeError(f"err must be int32 [1] on {device}, got {err.dtype} {list(err.shape)} on {err.device}")
+    return err.data_ptr()
+
+
 def dtype_code(dt: torch.dtype, dense: bool = False) -> int:
     """Logits dtype code; ``dense`` admits float64 (the tok_next mask only)."""
     code = (_DENSE_DTYPE_CODE if dense else _DTYPE_CODE).get(dt)

@@ -60,8 +60,7 @@ class PagedKV4:
             raise RuntimeError(f"pages must be contiguous uint8 [num_pages, kv_heads, {want}]")
         if pages.shape[1] < 1:
             raise RuntimeError("the cache needs at least one head")
-        if err is not None and (err.dtype != torch.int32 or err.device != pages.device):
-            raise RuntimeError("err must be int32 on the cache's device")
+        _lib.err_ptr(err, pages.device)
         self.pages, self.page_size, self.head_dim, self.dtype, self.err = pages, page_size, head_dim, dtype, err
         self.num_pages, self.kv_heads = pages.shape[0], pages.shape[1]
         self.device = pages.device

@@ -831,7 +831,8 @@ def dense_verify(logits, draft_tokens, uniforms, *, draft_probs=None, draft_lens
     drafts; the state of request b is ``states[slots[b]]`` with ``slots``, and
     ``write_back`` updates it there) or with ``bit_rows`` int32 [batch, drafts
     + 1], the row of ``allow_bits`` of each position.  ``vocab``: columns that
-    are tokens (all of ``logits``, or of ``tok_next``, without it)."""
+    are tokens (all of ``logits``, or of ``tok_next``, without it); ``err``:
+    int32 [1] on the logits' device, flags are OR-ed into it."""
     if logits.dim() != 3 or draft_tokens.dim() != 2 or uniforms.dim() != 2:
         raise RuntimeError("logits must be [batch, drafts + 1, vocab], draft_tokens [batch, drafts], "
                            "uniforms [batch, drafts + 1]")
@@ -856,6 +857,7 @@ def dense_verify(logits, draft_tokens, uniforms, *, draft_probs=None, draft_lens
     temp = temperature if isinstance(temperature, torch.Tensor) else None
     dev = _same_device(logits, draft_tokens, uniforms, draft_probs, draft_lens, temp, tok_next, allow_bits, bit_rows,
                        states, slots)
+    word = _lib.err_ptr(err, dev)
     code = _lib.dtype_code(logits.dtype)
     z_row, z_pos, unit = logits.stride()
     if unit != 1:
@@ -922,9 +924,9 @@ def dense_verify(logits, draft_tokens, uniforms, *, draft_probs=None, draft_lens
     if dev.type == "cuda":
         need = lib().bpd_verify_workspace_bytes(B, T, V)
         ws = logits.new_empty(need, dtype=torch.uint8)
-        check(lib().bpd_verify(*args, ptr(ws), need, ptr(err), _lib.stream_of(dev)))
+        check(lib().bpd_verify(*args, ptr(ws), need, word, _lib.stream_of(dev)))
     else:
-        check(lib().bpd_host_verify(*args, ptr(err)))
+        check(lib().bpd_host_verify(*args, word))
     return (n, token) if tok_next is None else (n, token, state)
 
 
