@@ -440,7 +440,7 @@ def pda_step(configs, g: PdaTensors, token_ids, slots=None, broken=None, err=Non
         stream = _lib.stream_of(dev)
         ws, ws_bytes = g.mask_workspace(B, dev, stream)
         check(lib().bpd_pda_advance(g.c_table(), g.c_tokens(), ptr(configs), ptr(sl), ptr(tk), code, B,
-                                    ptr(ok), ptr(broken), ptr(status), ptr(err), ptr(ws), ws_bytes,
+                                    ptr(ok), ptr(broken), ptr(status), _lib.err_ptr(err, dev), ptr(ws), ws_bytes,
                                     stream))
     else:
         check(lib().bpd_host_pda_advance(g.c_table(), g.c_tokens(), ptr(configs), ptr(sl), ptr(tk),

@@ -498,7 +498,7 @@ def dense_mask_(logits, tok_next, states, slots=None, neg_inf=float("-inf"), err
     if dev.type == "cuda":
         pp, np_ = _pending_args(pending)
         check(lib().bpd_dense_apply_mask(ptr(work), code, B, V, ld, ptr(tn), S, ptr(st), ptr(sl),
-                                         pp, np_, float(neg_inf), ptr(err), _lib.stream_of(dev)))
+                                         pp, np_, float(neg_inf), _lib.err_ptr(err, dev), _lib.stream_of(dev)))
     else:
         if pending is not None and pending.numel():
             raise RuntimeError("queued writes are applied by device launches only")
@@ -530,7 +530,7 @@ def dense_mask_bits_(logits, allow_bits, states, slots=None, neg_inf=float("-inf
     if dev.type == "cuda":
         pp, np_ = _pending_args(pending)
         check(lib().bpd_dense_apply_mask_bits(ptr(work), code, B, V, ld, ptr(allow_bits), W, S,
-                                              ptr(st), ptr(sl), pp, np_, float(neg_inf), ptr(err),
+                                              ptr(st), ptr(sl), pp, np_, float(neg_inf), _lib.err_ptr(err, dev),
                                               _lib.stream_of(dev)))
     else:
         if pending is not None and pending.numel():
@@ -579,7 +579,7 @@ def dense_advance(tok_next, states, tokens, slots=None, write_back=False, err=No
     if dev.type == "cuda":
         pp, np_ = _pending_args(pending)
         check(lib().bpd_dense_advance(ptr(tn), S, V, ptr(st), ptr(sl), pp, np_, ptr(tk), code, B,
-                                      ptr(out), int(write_back), ptr(err), _lib.stream_of(dev)))
+                                      ptr(out), int(write_back), _lib.err_ptr(err, dev), _lib.stream_of(dev)))
     else:
         if pending is not None and pending.numel():
             raise RuntimeError("queued writes are applied by device launches only")
@@ -597,7 +597,7 @@ def dense_compute_mask(tok_next, states, slots=None, err=None):
     out = torch.empty((B, (V + 31) // 32), dtype=torch.int32, device=dev)
     tn = _i32(tok_next)
     if dev.type == "cuda":
-        check(lib().bpd_dense_compute_mask(ptr(tn), S, V, ptr(st), ptr(sl), B, ptr(out), ptr(err),
+        check(lib().bpd_dense_compute_mask(ptr(tn), S, V, ptr(st), ptr(sl), B, ptr(out), _lib.err_ptr(err, dev),
                                            _lib.stream_of(dev)))
     else:
         check(lib().bpd_host_dense_compute_mask(ptr(tn), S, V, ptr(st), ptr(sl), B, ptr(out)))
@@ -644,7 +644,7 @@ def fsa_mask_(logits, fsa: FsaTensors, states, slots=None, neg_inf=float("-inf")
     sl = None if slots is None else slots.to(torch.int64).contiguous()
     ld = work.stride(0) if B > 1 else V
     check(lib().bpd_fsa_apply_mask(C.byref(fsa.c_fsa_table()), ptr(work), _lib.dtype_code(work.dtype), B, ld,
-                                   ptr(st), ptr(sl), float(neg_inf), ptr(err), _lib.stream_of(dev)))
+                                   ptr(st), ptr(sl), float(neg_inf), _lib.err_ptr(err, dev), _lib.stream_of(dev)))
     if copied:
         logits.copy_(work)
     return logits
@@ -656,7 +656,7 @@ def fsa_compute_mask(fsa: FsaTensors, states, slots=None, err=None) -> torch.Ten
     sl = None if slots is None else slots.to(torch.int64).contiguous()
     B = st.numel() if sl is None else sl.numel()
     out = torch.empty((B, (fsa.vocab_size + 31) // 32), dtype=torch.int32, device=dev)
-    check(lib().bpd_fsa_compute_mask(C.byref(fsa.c_fsa_table()), ptr(st), ptr(sl), B, ptr(out), ptr(err),
+    check(lib().bpd_fsa_compute_mask(C.byref(fsa.c_fsa_table()), ptr(st), ptr(sl), B, ptr(out), _lib.err_ptr(err, dev),
                                      _lib.stream_of(dev)))
     return out
 
@@ -684,7 +684,7 @@ def fsa_advance(fsa: FsaTensors, states, tokens, slots=None, write_back=False, e
     out = torch.empty(B, dtype=torch.int32, device=dev)
     pp, np_ = _pending_args(pending)
     check(lib().bpd_fsa_advance(C.byref(fsa.c_fsa_table()), ptr(st), ptr(sl), pp, np_, ptr(tk),
-                                _lib.index_code(tk.dtype), B, ptr(out), int(write_back), ptr(err),
+                                _lib.index_code(tk.dtype), B, ptr(out), int(write_back), _lib.err_ptr(err, dev),
                                 _lib.stream_of(dev)))
     return out.view(tokens.shape) if tokens.dim() else out.reshape(())
 
@@ -770,7 +770,7 @@ def apply_soft_prior_(logits: torch.Tensor, fsa: FsaTensors, states: torch.Tenso
         ws, ws_bytes = sc.workspace(B, dev, stream)
         check(lib().bpd_soft_prior(ptr(work), B, V, ld, S, ptr(acc), ptr(live), eos, ptr(st),
                                    ptr(sl), C.byref(sc.c_struct()), int(k), float(alpha), ptr(ws),
-                                   ws_bytes, ptr(err), stream))
+                                   ws_bytes, _lib.err_ptr(err, dev), stream))
     else:
         check(lib().bpd_host_soft_prior(ptr(work), B, V, ld, ptr(tn), S, ptr(acc), ptr(live), eos,
                                         ptr(st), ptr(sl), int(k), float(alpha)))

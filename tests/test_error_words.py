@@ -6,8 +6,13 @@ from __future__ import annotations
 import pytest
 import torch
 
-from bpdecode_amd import ops
+from bpdecode_amd import _lib, ops, synth
+from bpdecode_amd.grammar.device import build_pda_tensors, pda_step
+from bpdecode_amd.grammar.gbnf import parse_gbnf
+from bpdecode_amd.grammar.pda import CompiledGrammar
 from bpdecode_amd.kv import PagedKV4, block_bytes
+from bpdecode_amd.ops import FsaTensors
+from tests._util import PDA_VOCAB
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 
@@ -38,3 +43,25 @@ def test_the_cache_refuses_a_wrong_error_word(which, device):
     pages = torch.zeros(2, 1, block_bytes(16, 64), dtype=torch.uint8, device=device)
     with pytest.raises(RuntimeError, match="err must be int32"):
         PagedKV4(pages, 16, 64, torch.bfloat16, wrong_words(device)[which])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", range(4))
+def test_masks_and_commits_refuse_a_wrong_error_word(which, dev):
+    vocab = synth.serving_vocab(512, seed=1)
+    dense = FsaTensors.build("[a-z]+", vocab, dense=True).to(dev)
+    walked = FsaTensors.build("[a-z]+", vocab, dense=False).to(dev)
+    V = dense.vocab_size
+    s, x = torch.zeros(2, dtype=torch.int32, device=dev), torch.full((2,), 5, dtype=torch.int32, device=dev)
+    z, pool = torch.zeros(2, V, device=dev), torch.zeros(2, _lib.PDA_CONFIG_WORDS, dtype=torch.int32, device=dev)
+    g = build_pda_tensors(CompiledGrammar.build(parse_gbnf(synth.JSON_GBNF)), PDA_VOCAB).to(dev)
+    bits = dense.ensure_allow_bits()
+    calls = (lambda e: ops.dense_mask_(z, dense.tok_next, s, err=e), lambda e: ops.dense_mask_bits_(z, bits, s, err=e),
+             lambda e: ops.dense_advance(dense.tok_next, s, x, err=e),
+             lambda e: ops.dense_compute_mask(dense.tok_next, s, err=e),
+             lambda e: ops.fsa_mask_(z, walked, s, err=e), lambda e: ops.fsa_compute_mask(walked, s, err=e),
+             lambda e: ops.fsa_advance(walked, s, x, err=e), lambda e: ops.apply_soft_prior_(z, dense, s, 2, err=e),
+             lambda e: pda_step(pool, g, x, err=e))
+    for call in calls:
+        with pytest.raises(RuntimeError, match="err must be int32"):
+            call(wrong_words("cuda")[which])
