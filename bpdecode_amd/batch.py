@@ -621,13 +621,16 @@ class ConstraintBatch:
         return n, token
 
     def check_errors(self) -> None:
-        """Raise if a device kernel met an out-of-range state or token since
-        the last check (synchronises with the device)."""
+        """Raise IndexError if a device kernel met an out-of-range state or
+        token, or a verification an allowed logit of +inf or NaN, since the
+        last check (synchronises with the device)."""
         if self._err is None:
             return
         flags = int(self._err.item())
         if flags:
             self._err.zero_()
+            if flags == _lib.FLAG_LOGITS:
+                raise IndexError("an allowed logit was +inf or NaN in a verification on the device")
             raise IndexError(f"out-of-range index in a device constraint kernel (flags {flags})")
 
     # --- queries -----------------------------------------------------------

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from bpdecode_amd import _lib, ops, synth
+from bpdecode_amd.batch import ConstraintBatch
 from bpdecode_amd.grammar.device import build_pda_tensors, pda_step
 from bpdecode_amd.grammar.gbnf import parse_gbnf
 from bpdecode_amd.grammar.pda import CompiledGrammar
@@ -65,3 +66,22 @@ def test_masks_and_commits_refuse_a_wrong_error_word(which, dev):
     for call in calls:
         with pytest.raises(RuntimeError, match="err must be int32"):
             call(wrong_words("cuda")[which])
+
+
+@pytest.mark.gpu
+def test_a_batch_names_what_its_kernels_met(dev):
+    """Logits without a softmax are not reported as an index out of range."""
+    vocab = synth.serving_vocab(512, seed=1)
+    batch = ConstraintBatch(FsaTensors.build("[a-z]+", vocab, dense=True), capacity=2, device=dev)
+    batch.add(0)
+    z = torch.zeros(1, 2, vocab.size, device=dev)
+    x, u = torch.full((1, 1), -7, dtype=torch.int32, device=dev), torch.full((1, 2), 0.5, device=dev)
+    batch.verify([0], z, x, u)
+    with pytest.raises(IndexError, match="out-of-range index"):
+        batch.check_errors()
+    batch.reset(0)
+    n, token = batch.verify([0], z.fill_(float("nan")), x.fill_(0), u)
+    assert (int(n), int(token)) == (0, -1)
+    with pytest.raises(IndexError, match="logit was"):
+        batch.check_errors()
+    batch.check_errors()
