@@ -376,9 +376,10 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs a, Spa
 #pragma unroll
   for (int k = 0; k < Runs; ++k) bits[k] = run_bits(a, state, run_of(k));
   const double temp = temperature_of(a, b);
-  // half the difference does not pass the type's range; a factor past it would
-  // only make a zero of the largest logit's difference a NaN
-  const float to_log2 = temp > 0.0 ? float(fmin(2.0 * kLog2E / temp, 1e38)) : 0.0f;
+  // half the difference does not pass the type's range; a factor past it (of a
+  // subnormal temperature) would only make a zero of the largest logit's
+  // difference a NaN
+  const float to_log2 = temp > 0.0 ? float(fmin(2.0 * kLog2E / temp, 3e38)) : 0.0f;
   bool bad = false;
   float top = -INFINITY, sum = 0.0f;
   int32_t first = 0x7FFFFFFF;
