@@ -186,11 +186,18 @@ constexpr int kRun = 8;  // neighbouring tokens of a thread
 // threads with that many runs each.
 constexpr int kLongRuns = 4, kShortRuns = 1;
 constexpr double kLog2E = 1.4426950408889634;
-// Of the 32-bit sum: an exponent y is off by 3 * 2^-24 |y| (the difference, the
-// factor and their product rounded), and at least half of the mass lies at
-// y > -18, the share of one of 2^18 tokens; a lane's 128 terms and their joining
-// add 2^-18 at most, if every rounding goes the same way.
-constexpr double kSumError = 5e-6;
+// Of the 32-bit sum, if every rounding goes the same way, in units of 2^-24 of a
+// term.  Its exponent y is off by 3 |y| (a difference in float's normal range,
+// the factor and their product rounded; with every change of the maximum y is the sum of pieces of
+// one sign), which is 3 ln 2 |y| of the term; over the row |y| has a mean of
+// log2 of the vocabulary at most, below 31, because the entropy of p is no
+// more than that and no less than this mean.  Each of its exponentials is off
+// by 2 (one for itself, one for every later run's maximum, one for the wave's),
+// each of their products by 1.  It passes 3 sums of its run, one for every later
+// run and 6 of the wave's.
+constexpr double kSumUnits = 3 * 0.69314718056 * 31 + 2 * (kLongRuns + 1) + kLongRuns + 3 + (kLongRuns - 1) + 6;
+constexpr double kSumError = 5.5e-6;
+static_assert(kRun == 8 && kWave == 64 && kSumUnits * 0x1p-24 < kSumError, "the row's sum is off by more");
 // What tokens near their border may move of the whole, if all of them lie on
 // the wrong side by all of kSumError.
 constexpr double kNearly = 1e-9;
@@ -402,7 +409,8 @@ __global__ __launch_bounds__(kThreads) void verify_rows_kernel(VerifyArgs a, Spa
       }
       const float half = -0.5f * (top > -INFINITY ? top : 0.0f);
 #pragma unroll
-      for (int j = 0; j < kRun; ++j) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(z[j], 0.5f, half) * to_log2);
+      for (int j = 0; j < kRun; ++j) z[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[j], 0.5f, half) * to_log2);
+      sum += ((z[0] + z[1]) + (z[2] + z[3])) + ((z[4] + z[5]) + (z[6] + z[7]));
     } else if (here > top) {
       top = here;
 #pragma unroll
