@@ -33,8 +33,8 @@ struct AttendArgs {
 };
 
 // Tokens that query i of request b sees: none past the request's block table,
-// whatever its length says (*past is set where it says more).
-__host__ __device__ __forceinline__ int64_t seen_tokens(const AttendArgs& a, int64_t b, int32_t i, bool* past) {
+// whatever its length says (*past is set where it says more).  The host's.
+inline int64_t seen_tokens(const AttendArgs& a, int64_t b, int32_t i, bool* past) {
   *past = false;
   int32_t n = a.tokens;
   if (a.query_lens) n = a.query_lens[b] < n ? a.query_lens[b] : n;
@@ -214,8 +214,12 @@ __device__ __forceinline__ int here(int x) {
 // sums are scaled down, so most tiles cost no exchange between lanes.  Scores,
 // maximum, sums and the accumulated values are floats; the weights are rounded
 // to the cache's type, because the second product takes its operands in 16
-// bits (the values themselves are exact in them): half a step of a weight,
-// which the division's unrounded sum does not follow.  In float16 a row's
+// bits (the values themselves are exact in them).  A weight is off by half a
+// step, which the division's unrounded sum does not follow: with bfloat16 an
+// output of 1,000 tokens is off by 0.0020 of itself, the roundings of inputs
+// and output alone make that 0.0016.  (Weights as two terms of 16 bits, for
+// twice the second product: 16 columns of 128 channels 174 -> 200 us, 20 of
+// them 57 -> 66, one short request 10.6 -> 11.9.)  In float16 a row's
 // largest weight lies between kLift and kLift + 8 powers of two, so that
 // weights down to 2^-21 of it keep all their bits, and those below are off by
 // 2^-32 of it at most (with the largest at 1, those 2^-24 below, 17 nats,
@@ -355,7 +359,8 @@ __global__ __launch_bounds__(W* kWave, W == kWaves ? attend_blocks(D, NT) : 1) v
         for (int k = 0; k < Pt::width(p) / 32; ++k) {
           const uint16_t* from = row + Pt::begin(p) + (ql >> 4) * (Pt::width(p) / 4) + 8 * k;
           Frag f = {{0u, 0u, 0u, 0u}};
-          if (in && a.scale != 0.0f && (t * KW + Pt::begin(p) / 32 + k) % W == wave) __builtin_memcpy(&f, from, 16);  // at any element
+          const bool own = (t * KW + Pt::begin(p) / 32 + k) % W == wave;
+          if (own && in && a.scale != 0.0f) __builtin_memcpy(&f, from, 16);  // at any element
           if (a.scale < 0.0f)
 #pragma unroll
             for (int j = 0; j < 4; ++j) f.u[j] ^= 0x80008000u;
@@ -718,8 +723,10 @@ struct AttendSizes {
 };
 
 constexpr int kCus = 256;
-// Tiles of a unit up to which it is short, or of a middling length.  Eight
-// units of 1,000 tokens: 10.9 us, cut in runs 14.9; of 2,000: 15.9 and 14.6.
+// Tiles of a unit up to which it is short, or of a middling length, by the width
+// of the block table: the lengths are on the device.  Eight units of 1,000
+// tokens: 10.6 us, cut in runs (as in a table for 4,096 tokens or more) 12.8;
+// 128 units 11.4 and 13.7; eight of 2,000: 15.9 and 14.6.
 // 512 units of 4,000 tokens: 50 and 59, of 8,000: 92 and 99; 128 units of
 // 4,000 (a sixth of the device): 30 and 26.
 constexpr int kShort = 16, kMiddling = 128;

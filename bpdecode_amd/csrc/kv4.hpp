@@ -6,7 +6,8 @@
 // even code) and one byte e, s = 2^(e - 127).  s is the smallest power of two
 // with max|x| <= 7 s: between 4 and 6 neighbouring levels are 2 s apart, so
 // rounding is off by at most s there, and cutting 7 s to 6 s is off by no
-// more.  A power of two keeps every value exact in bfloat16 and float16 (two
+// more.  (But for float16's last values: past 7 * 2^13 = 57,344 the scale stays
+// 2^13, so 65,504 is kept as 49,152, two s below.)  A power of two keeps every value exact in bfloat16 and float16 (two
 // significant bits), so reading the cache rounds nothing, and gfx950 converts
 // two codes with their scale in one instruction.
 // 4 + 8 / 32 = 4.25 bits per element.

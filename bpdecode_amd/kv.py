@@ -9,7 +9,8 @@ A prompt is a long block, a plain decoding step a block of one token.
 
 An element takes 4.25 bits: an e2m1 code, and one power of two for 32
 neighbouring channels (the OCP microscaling layout of 4-bit floats, scales
-chosen so that the largest channel is never cut by more than a rounding).
+chosen so that the largest channel is never cut by more than a rounding; in
+float16 magnitudes past 57,344 are, and kept as 49,152).
 ``include/bpdecode_hip.h`` states the bytes of a page.  Tensors on the device
 run the HIP kernels on torch's current stream, CPU tensors the library's host
 entry points.  The cache keeps no lengths: the caller says where each request

@@ -709,13 +709,14 @@ int bpd_host_verify(const void* logits, int dtype, int64_t rows, int32_t drafts,
  * sign and 0, .5, 1, 1.5, 2, 3, 4, 6), a scale byte e stands for 2^(e - 127)
  * and 32 neighbouring channels: the smallest with max|x| <= 7 * 2^(e - 127)
  * that the cache's type holds (bfloat16: 2 <= e <= 252, float16: 104 <= e <=
- * 140); codes are rounded to nearest, ties to the even code, and 255 marks a
- * group that held an infinity or a NaN and reads as NaN.  page_size: a power
- * of two from 16 to 256; head_dim: 64, 96, 128, 192 or 256; dtype (of q, k, v
- * and every output): BPD_DTYPE_F16 or BPD_DTYPE_BF16.  Token p of request b
- * lies in page block_table[b * table_ld + p / page_size] (int32, table_blocks
- * per request).  Positions and pages outside their tables are left out and
- * set BPD_FLAG_PAGE_RANGE in `err`; no memory outside them is touched.
+ * 140, so that magnitudes past 57,344 are kept as 49,152); codes are rounded to
+ * nearest, ties to the even code, and 255 marks a group that held an infinity
+ * or a NaN and reads as NaN.  page_size: a power of two from 16 to 256;
+ * head_dim: 64, 96, 128, 192 or 256; dtype (of q, k, v and every output):
+ * BPD_DTYPE_F16 or BPD_DTYPE_BF16.  Token p of request b lies in page
+ * block_table[b * table_ld + p / page_size] (int32, table_blocks per request).
+ * Positions and pages outside their tables are left out and set
+ * BPD_FLAG_PAGE_RANGE in `err`; no memory outside them is touched.
  *
  * bpd_kv_append: tokens starts[b] + i, i < counts[b] (NULL: tokens), of k and
  * v [rows, tokens, kv_heads, head_dim] (strides in elements, channels next to
