@@ -692,7 +692,8 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a, Spa
 }
 
 // The next token, one block per request, a run of the chunk per thread: a chain
-// of loads that wait for each other (5 us for a short chunk, 8 to 10 for a long one).
+// of loads that wait for each other (5 us for a short chunk, 8 to 10 for a long
+// one; 40 to 60 us more where it forms the chunks of 151,936 tokens anew).
 template <int DT, int Runs>
 __global__ __launch_bounds__(kThreads* Runs) void verify_pick_kernel(VerifyArgs a, Space w) {
   constexpr int N = kWaves * Runs;
