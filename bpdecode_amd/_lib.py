@@ -151,6 +151,14 @@ _SIGNATURES = {
                           vp, f32, vp, i64, i32, vp, vp, vp, vp, cint, vp, vp, vp, vp, sz, vp, vp]),
     "bpd_host_verify": (cint, [vp, cint, i64, i32, i64, i64, i64, vp, cint, i64, vp, vp, cint, i64, i64, vp,
                                i64, vp, f32, vp, i64, i32, vp, vp, vp, vp, cint, vp, vp, vp, vp]),
+    "bpd_sample": (cint, [vp, cint, i64, i64, i64, vp, vp, f32, vp, i32, vp, f32, vp, f32, vp, i64, i32, vp, vp, vp, cint,
+                          vp, vp, vp, vp, vp]),
+    "bpd_host_sample": (cint, [vp, cint, i64, i64, i64, vp, vp, f32, vp, i32, vp, f32, vp, f32, vp, i64, i32, vp, vp, vp,
+                               cint, vp, vp, vp, vp]),
+    "bpd_truncate": (cint, [vp, cint, i64, i64, i64, vp, i64, i64, vp, f32, vp, i32, vp, f32, vp, f32, vp, i64, i32, vp,
+                            vp, vp, vp]),
+    "bpd_host_truncate": (cint, [vp, cint, i64, i64, i64, vp, i64, i64, vp, f32, vp, i32, vp, f32, vp, f32, vp, i64, i32,
+                                 vp, vp, vp]),
     "bpd_kv_append": (cint, [vp, i64, i32, i32, i32, cint, vp, i64, i64, i64, vp, i64, i64, i64, vp, i64, i64,
                              i64, i32, vp, i64, i32, vp, i64, i32, vp, vp, vp, vp, i64, i32, cint, vp, vp]),
     "bpd_host_kv_append": (cint, [vp, i64, i32, i32, i32, cint, vp, i64, i64, i64, vp, i64, i64, i64, vp, i64,

@@ -620,17 +620,54 @@ class ConstraintBatch:
         pool[slots] = state
         return n, token
 
+    def sample(self, seq_ids: Sequence[Hashable], logits: torch.Tensor, uniforms: torch.Tensor, *,
+               temperature: float | torch.Tensor = 1.0, top_k: int | torch.Tensor = 0, top_p: float | torch.Tensor = 1.0,
+               min_p: float | torch.Tensor = 0.0) -> tuple[torch.Tensor, torch.Tensor]:
+        """Draw a token per sequence from ``logits`` [len(seq_ids), columns]
+        under the grammar and advance each sequence by it
+        (:func:`~bpdecode_amd.ops.sample`; the logits need no mask before, and
+        the tokens no commit after).  Returns (int32 tokens, float32
+        log-probabilities); a sequence whose grammar allows nothing yields -1
+        and is ``BROKEN``."""
+        slots = self._slots(seq_ids)
+        pool = self._state
+        kw = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p, "err": self._err}
+        if self.fsa.tok_next is not None:
+            token, logprob, _ = ops.dense_sample(logits, uniforms, tok_next=self.fsa.tok_next,
+                                                 allow_bits=self.fsa.ensure_allow_bits(), states=pool, slots=slots,
+                                                 write_back=True, **kw)
+            return token, logprob
+        token, logprob, state = ops._walked_sample(logits, uniforms, self.fsa, pool[slots], **kw)
+        pool[slots] = state
+        return token, logprob
+
+    def truncate(self, seq_ids: Sequence[Hashable], logits: torch.Tensor, *, temperature: float | torch.Tensor = 1.0,
+                 top_k: int | torch.Tensor = 0, top_p: float | torch.Tensor = 1.0,
+                 min_p: float | torch.Tensor = 0.0) -> torch.Tensor:
+        """In place: ``-inf`` for every logit of ``logits`` [len(seq_ids),
+        columns] that :meth:`sample` would not draw from
+        (:func:`~bpdecode_amd.ops.truncate`): ``apply_mask`` with top-k, top-p
+        and min-p.  States stay as they are."""
+        slots = self._slots(seq_ids)
+        pool = self._state
+        kw = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p, "err": self._err, "out": logits,
+              "vocab": self.fsa.vocab_size}
+        if self.fsa.tok_next is not None:
+            return ops.dense_truncate(logits, allow_bits=self.fsa.ensure_allow_bits(), bit_rows=pool, slots=slots, **kw)
+        bits, at = ops._walked_bits(self.fsa, pool[slots])
+        return ops.dense_truncate(logits, allow_bits=bits, bit_rows=at, **kw)
+
     def check_errors(self) -> None:
         """Raise IndexError if a device kernel met an out-of-range state or
-        token, or a verification an allowed logit of +inf or NaN, since the
-        last check (synchronises with the device)."""
+        token, or a verification, draw or truncation an allowed logit of +inf
+        or NaN, since the last check (synchronises with the device)."""
         if self._err is None:
             return
         flags = int(self._err.item())
         if flags:
             self._err.zero_()
             if flags == _lib.FLAG_LOGITS:
-                raise IndexError("an allowed logit was +inf or NaN in a verification on the device")
+                raise IndexError("an allowed logit was +inf or NaN in a verification, draw or truncation on the device")
             raise IndexError(f"out-of-range index in a device constraint kernel (flags {flags})")
 
     # --- queries -----------------------------------------------------------

@@ -1,0 +1,635 @@
+// Sampling with temperature, top-k, top-p and min-p from given uniform
+// numbers, truncation of logits by the same cuts, and their host forms.
+//
+// With z the logits that the row's grammar state allows (those of -inf left
+// out), top the largest and w = exp((z - top) / temperature), tokens stand in
+// the order of falling z, equal ones in that of their index.  top-k keeps the
+// first k, top-p of these the first whose sum of w is top_p of theirs at
+// least, min-p those with z - top >= temperature * log(min_p): each is a first
+// part of the order, and so is what all of them keep.  The token drawn is the
+// first of the order whose running sum passes u times the whole sum of what
+// is kept; truncation writes -inf over everything else.  At temperature 0
+// (or where it is not positive and finite) the first token alone is kept.
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+#include "runs.hpp"
+#include "wave.hpp"
+
+namespace bpd {
+namespace {
+
+struct SampleArgs {
+  const void* logits;
+  int dtype;
+  int64_t rows, vocab, ld;
+  const float* temperature;  // per row, or temperature_all; the same below
+  float temperature_all;
+  const int32_t* top_k;
+  int32_t top_k_all;
+  const float* top_p;
+  float top_p_all;
+  const float* min_p;
+  float min_p_all;
+  const uint32_t* allow_bits;
+  int64_t words;
+  int32_t num_states;
+  int32_t* states;
+  const int64_t* slots;
+  // a draw
+  const float* uniforms;
+  const int32_t* tok_next;
+  int write_back;
+  int32_t* token;
+  float* logprob;
+  int32_t* next_state;
+  // a truncation
+  void* out;
+  int64_t cols, out_ld;
+  int32_t* err;
+};
+
+// What a row asks for.
+struct Asked {
+  double temp;   // 0: the first largest
+  int64_t top_k; // 0: all
+  float top_p;   // 1: all
+  double min_p;  // 0: all
+};
+__host__ __device__ __forceinline__ Asked asked_of(const SampleArgs& a, int64_t b) {
+  const float t = a.temperature ? a.temperature[b] : a.temperature_all;
+  const int32_t k = a.top_k ? a.top_k[b] : a.top_k_all;
+  const float p = a.top_p ? a.top_p[b] : a.top_p_all, m = a.min_p ? a.min_p[b] : a.min_p_all;
+  return Asked{t > 0.0f && t < INFINITY ? double(t) : 0.0, k > 0 ? k : 0, p < 1.0f ? (p > 0.0f ? p : 0.0f) : 1.0f,
+               m > 0.0f ? (m < 1.0f ? double(m) : 1.0) : 0.0};
+}
+
+__host__ __device__ __forceinline__ int32_t state_of(const SampleArgs& a, int64_t b) {
+  return a.allow_bits ? a.states[a.slots ? a.slots[b] : b] : 0;
+}
+
+__host__ __device__ __forceinline__ void store_drawn(const SampleArgs& a, int64_t b, int32_t state, int64_t token,
+                                                     float logprob) {
+  a.token[b] = int32_t(token);
+  a.logprob[b] = logprob;
+  if (!a.tok_next) return;
+  const int32_t s = token < 0 ? -1 : a.tok_next[int64_t(state) * a.vocab + token];
+  if (a.next_state) a.next_state[b] = s;
+  if (a.write_back) a.states[a.slots ? a.slots[b] : b] = s;
+}
+
+// ------------------------------------------------------------- the device --
+// One block per row.  Sums of weights are whole numbers of 64 bits: a weight
+// is its nearest multiple of 2^-scale of the largest, so that no sum depends
+// on its order, equal logits weigh the same, and a border that lies between
+// two sums is decided as the sums themselves are.  Off by half of that per
+// token, a row of 2^17 tokens is off by 2^-37 of its largest weight or so,
+// where a row's 10^5 borders want 10^-12 of its sum.
+typedef unsigned long long u64;
+
+constexpr int kThreads = 1024;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kStep = kThreads * kRun;  // tokens that a block reads at a time
+constexpr int kBins = 4 * kThreads;
+constexpr int kMostScale = 50;  // a weight is read off the bits of its sum with 2^52
+
+// Bits of a weight: the sum of a row's fits 63.
+__host__ __device__ __forceinline__ int scale_of(int64_t vocab) {
+  int bits = 0;
+  while ((int64_t(1) << bits) < vocab) ++bits;
+  return 62 - bits < kMostScale ? 62 - bits : kMostScale;
+}
+
+struct Row {
+  const char* logits;
+  const uint8_t* bits;  // of its state, null: every token
+  int64_t vocab;        // 0: its state allows nothing
+};
+
+// Which tokens of a run are the thread's own and allowed.
+__device__ __forceinline__ uint32_t run_bits(const Row& r, const Run& run) {
+  if (!r.bits || run.own == 0) return run.own;
+  return uint32_t(r.bits[(run.t + run.shift) / 8]) << run.shift & run.own;
+}
+
+// A logit as a number that orders as it does (-0 as 0), and back.
+__device__ __forceinline__ uint32_t key_of(float z) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, z + 0.0f);
+  return u ^ (uint32_t(int32_t(u) >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float logit_of(uint32_t key) {
+  return __builtin_bit_cast(float, key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
+
+// What the logits of a row are measured by.
+struct Measure {
+  double top, to_log2;  // y = (z - top) * to_log2, w = 2^y
+  double bins;          // bins of the first table to an octave
+  int scale;
+  __device__ __forceinline__ double y(float z) const { return (double(z) - top) * to_log2; }
+  __device__ __forceinline__ u64 weight(double y) const {
+    const double w = __builtin_fma(exp2_down(y), __builtin_ldexp(1.0, scale), 0x1p52);
+    return __builtin_bit_cast(u64, w) & ((u64(1) << 52) - 1);
+  }
+  __device__ __forceinline__ int32_t bin(double y) const { return int32_t(fmin(-y * bins, double(kBins - 1))); }
+};
+
+// A first part of the order: all tokens with larger keys, and the first `rank`
+// of those with this one.
+struct Cut {
+  uint32_t key;
+  u64 rank, sum;  // sum: of its weights
+};
+
+struct Table {
+  u64 sums[kBins];
+  uint32_t counts[kBins];
+};
+struct Scratch {
+  Table first, sub;  // by weight, and of a part of one bin of it by key
+  u64 sums[kWaves], counts[kWaves];
+  u64 hit_count, hit_sum;
+  int64_t found;
+  float tops[kWaves];
+  int32_t bad[kWaves], hit_bin;
+};
+
+__device__ __forceinline__ void clear(Table& t) {
+  for (int i = threadIdx.x; i < kBins; i += kThreads) t.sums[i] = 0, t.counts[i] = 0;
+}
+
+// The bin in which the running count or sum passes `target` (less than the
+// whole); *count and *sum become what lies before it.
+__device__ __forceinline__ int32_t find_bin(const Table& t, u64 target, bool by_count, u64* count, u64* sum, Scratch& s) {
+  constexpr int kMine = kBins / kThreads;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  u64 c = 0, x = 0;
+#pragma unroll
+  for (int k = 0; k < kMine; ++k) c += t.counts[tid * kMine + k], x += t.sums[tid * kMine + k];
+  u64 upto_c = wave_scan_sum(c), upto_x = wave_scan_sum(x);
+  if (lane == kWave - 1) s.counts[wave] = upto_c, s.sums[wave] = upto_x;
+  if (tid == 0) s.hit_bin = kBins - 1, s.hit_count = s.hit_sum = 0;
+  __syncthreads();
+  for (int k = 0; k < wave; ++k) upto_c += s.counts[k], upto_x += s.sums[k];
+  c = upto_c - c, x = upto_x - x;
+  if ((by_count ? c <= target && target < upto_c : x <= target && target < upto_x)) {
+#pragma unroll 1
+    for (int k = tid * kMine;; ++k) {
+      const u64 nc = c + t.counts[k], nx = x + t.sums[k];
+      if (k == tid * kMine + kMine - 1 || target < (by_count ? nc : nx)) {
+        s.hit_bin = k, s.hit_count = c, s.hit_sum = x;
+        break;
+      }
+      c = nc, x = nx;
+    }
+  }
+  __syncthreads();
+  *count = s.hit_count, *sum = s.hit_sum;
+  const int32_t bin = s.hit_bin;
+  __syncthreads();
+  return bin;
+}
+
+// f(z, valid, t) for the runs of tokens [begin, end) that threads take from
+// `first` on, `step` tokens apart: t is the token of z[0], `valid` says which
+// are the thread's own, allowed and not -inf.
+template <int DT, class F>
+__device__ __forceinline__ void each_run(const Row& r, int64_t first, int64_t end, int64_t step, F f) {
+#pragma unroll 1
+  for (int64_t t = first; t < end; t += step) {
+    const Run run = run_at(t, r.vocab);
+    uint32_t valid = run_bits(r, run);
+    float z[kRun];
+    load_run<DT>(r.logits, run, r.vocab, z);
+#pragma unroll
+    for (int j = 0; j < kRun; ++j)
+      if (z[j] == -INFINITY) valid &= ~(1u << j);
+    f(z, valid, run.t);
+  }
+}
+
+// The token of rank `rank` (from 1) among those with this key, by index.
+template <int DT>
+__device__ int64_t nth_token(const Row& r, uint32_t key, u64 rank, Scratch& s) {
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+  // a wave takes neighbouring tokens
+  const int64_t part = (r.vocab + kStep - 1) / kStep * (kWave * kRun);
+  const int64_t begin = part * wave, end = begin + part < r.vocab ? begin + part : r.vocab;
+  const auto same = [&](const float(&z)[kRun], uint32_t valid) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) m |= uint32_t(key_of(z[j]) == key) << j;
+    return m & valid;
+  };
+  u64 n = 0;
+  each_run<DT>(r, begin + lane * kRun, end, kWave * kRun,
+               [&](const float(&z)[kRun], uint32_t valid, int64_t) { n += __popc(same(z, valid)); });
+  n = wave_sum(n);
+  if (lane == 0) s.counts[wave] = n;
+  if (threadIdx.x == 0) s.found = -1;
+  __syncthreads();
+  u64 before = 0;
+  int hit = 0;
+  for (; hit < kWaves - 1 && before + s.counts[hit] < rank; ++hit) before += s.counts[hit];
+  if (wave == hit) {
+    for (int64_t t0 = begin; t0 < end; t0 += kWave * kRun) {
+      uint32_t m = 0;
+      int64_t at = 0;
+      each_run<DT>(r, t0 + lane * kRun, t0 + lane * kRun + 1 < end ? t0 + lane * kRun + 1 : end, kWave * kRun,
+                   [&](const float(&z)[kRun], uint32_t valid, int64_t t) { m = same(z, valid), at = t; });
+      const u64 upto = before + wave_scan_sum(u64(__popc(m)));
+      if (upto >= rank && upto - __popc(m) < rank) {
+        for (u64 k = upto - __popc(m) + 1; k < rank; ++k) m &= m - 1;
+        s.found = at + __builtin_ctz(m);
+      }
+      before = of_lane(upto, kWave - 1);
+      if (before >= rank) break;
+    }
+  }
+  __syncthreads();
+  const int64_t found = s.found;
+  __syncthreads();
+  return found;
+}
+
+// floor(x * f) for f in [0, 1), exactly; `ceil_less_one`: ceil(x * f) - 1, no
+// less than 0.
+__device__ __forceinline__ u64 share_of(u64 x, float f, bool ceil_less_one) {
+  if (!(f > 0.0f)) return 0;
+  int e;
+  const u64 m = u64(frexpf(f, &e) * 0x1p24f);  // f = m 2^(e - 24)
+  const int down = 24 - e;                      // at least 24
+  u64 lo = x * m, hi = __umul64hi(x, m);
+  if (lo == 0 && hi == 0) return 0;
+  if (ceil_less_one) hi -= lo == 0, lo -= 1;
+  if (down >= 128) return 0;
+  if (down >= 64) return hi >> (down - 64);
+  return hi << (64 - down) | lo >> down;
+}
+
+template <int DT>
+__device__ void sample_row(const SampleArgs& a, const Row& r, const Asked& want, int64_t b, bool draw, Scratch& s,
+                           Cut* cut_out, int64_t* last_out, float* logprob, bool* bad_out) {
+  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  float top = -INFINITY;
+  bool bad = false;
+  each_run<DT>(r, tid * kRun, r.vocab, kStep, [&](const float(&z)[kRun], uint32_t valid, int64_t) {
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      if (!(valid >> j & 1)) continue;
+      bad |= !(z[j] < INFINITY);
+      top = fmaxf(top, z[j]);
+    }
+  });
+  top = wave_max(top);
+  bad = __any(bad);
+  if (lane == 0) s.tops[wave] = top, s.bad[wave] = bad;
+  __syncthreads();
+  bad = false;
+  for (int k = 0; k < kWaves; ++k) top = fmaxf(top, s.tops[k]), bad |= s.bad[k] != 0;
+  *bad_out = bad;
+  *last_out = -1;
+  *logprob = -INFINITY;
+  if (bad || top == -INFINITY) return;
+  const uint32_t top_key = key_of(top);
+  Cut cut{top_key, 1, 1};
+  Measure m{double(top), want.temp > 0.0 ? kLog2E / want.temp : 0.0, 0.0, scale_of(r.vocab)};
+  m.bins = double(kBins) / (m.scale + 2);
+  const bool whole = want.temp > 0.0 && want.top_k == 0 && want.top_p >= 1.0f && want.min_p <= 0.0;
+  if (!draw && whole) {
+    cut.key = cut.rank = 0;
+  } else if (want.temp > 0.0) {
+    clear(s.first);
+    __syncthreads();
+    each_run<DT>(r, tid * kRun, r.vocab, kStep, [&](const float(&z)[kRun], uint32_t valid, int64_t) {
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
+        if (!(valid >> j & 1)) continue;
+        const double y = m.y(z[j]);
+        const int32_t i = m.bin(y);
+        atomicAdd(&s.first.counts[i], 1u);
+        atomicAdd(&s.first.sums[i], m.weight(y));
+      }
+    });
+    __syncthreads();
+    // all of the row
+    u64 count = 0, sum = 0;
+    {
+      u64 c = 0, x = 0;
+      for (int i = tid; i < kBins; i += kThreads) c += s.first.counts[i], x += s.first.sums[i];
+      c = wave_sum(c), x = wave_sum(x);
+      if (lane == 0) s.counts[wave] = c, s.sums[wave] = x;
+      __syncthreads();
+      for (int k = 0; k < kWaves; ++k) count += s.counts[k], sum += s.sums[k];
+      __syncthreads();
+    }
+    cut = Cut{0, 0, sum};
+    // the first part of the order that ends where the running count or sum passes `target`
+    const auto select = [&](u64 target, bool by_count) {
+      u64 c, x;
+      const int32_t bin = find_bin(s.first, target, by_count, &c, &x, s);
+      // keys that the bin can hold, generously
+      const double per = m.bins * m.to_log2, slack = fabs(m.top) * 0x1p-50;
+      const double from = m.top - bin / per, to = m.top - (bin + 1) / per;
+      const double off = slack + (m.top - to) * 0x1p-50;
+      uint32_t hi = top_key, lo = key_of(-3.402823466e38f);
+      if (from + off < m.top) hi = min(hi, key_of(float(from + off)) + 2);
+      if (bin < kBins - 1 && to - off > -3.4e38) lo = max(lo, key_of(float(to - off)) - 2);
+      for (;;) {
+        const uint32_t range = hi - lo;
+        const int shift = range < uint32_t(kBins) ? 0 : 32 - __builtin_clz(range) - __builtin_ctz(uint32_t(kBins));
+        clear(s.sub);
+        __syncthreads();
+        each_run<DT>(r, tid * kRun, r.vocab, kStep, [&](const float(&z)[kRun], uint32_t valid, int64_t) {
+#pragma unroll
+          for (int j = 0; j < kRun; ++j) {
+            const uint32_t key = key_of(z[j]);
+            if (!(valid >> j & 1) || key < lo || key > hi) continue;
+            const double y = m.y(z[j]);
+            if (m.bin(y) != bin) continue;
+            atomicAdd(&s.sub.counts[(hi - key) >> shift], 1u);
+            atomicAdd(&s.sub.sums[(hi - key) >> shift], m.weight(y));
+          }
+        });
+        __syncthreads();
+        u64 dc, dx;
+        const uint32_t i = uint32_t(find_bin(s.sub, target - (by_count ? c : x), by_count, &dc, &dx, s));
+        c += dc, x += dx;
+        hi -= i << shift;
+        if (shift == 0 || hi <= lo) break;
+        lo = max(lo, hi - ((1u << shift) - 1));
+      }
+      const u64 w = m.weight(m.y(logit_of(hi)));
+      const u64 rank = by_count ? target - c + 1 : (target - x) / w + 1;
+      return Cut{hi, rank, x + rank * w};
+    };
+    if (want.top_k > 0 && u64(want.top_k) < count) cut = select(u64(want.top_k) - 1, true);
+    if (want.top_p < 1.0f) cut = select(share_of(cut.sum, want.top_p, true), false);
+    if (want.min_p > 0.0) {
+      // the least key that min-p keeps
+      const double least = want.temp * log(want.min_p);
+      uint32_t lo = 0, hi = top_key;  // lo is not kept, hi is
+      while (hi - lo > 1) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (mid > 0x007FFFFFu && double(logit_of(mid)) - m.top >= least) hi = mid;
+        else lo = mid;
+      }
+      if (hi > cut.key) {
+        u64 x = 0;
+        each_run<DT>(r, tid * kRun, r.vocab, kStep, [&](const float(&z)[kRun], uint32_t valid, int64_t) {
+#pragma unroll
+          for (int j = 0; j < kRun; ++j)
+            if ((valid >> j & 1) && key_of(z[j]) >= hi) x += m.weight(m.y(z[j]));
+        });
+        x = wave_sum(x);
+        if (lane == 0) s.sums[wave] = x;
+        __syncthreads();
+        cut = Cut{hi - 1, 0, 0};
+        for (int k = 0; k < kWaves; ++k) cut.sum += s.sums[k];
+        __syncthreads();
+      }
+    }
+    if (draw) {
+      const float u = a.uniforms[b];
+      u64 target = u < 1.0f ? share_of(cut.sum, u, false) : cut.sum;
+      if (target >= cut.sum) target = cut.sum - 1;
+      const u64 kept = cut.sum;
+      cut = select(target, false);
+      *logprob = float((double(logit_of(cut.key)) - m.top) / want.temp - log(double(kept) * __builtin_ldexp(1.0, -m.scale)));
+    }
+  } else {
+    *logprob = 0.0f;
+  }
+  *cut_out = cut;
+  if (cut.rank > 0) *last_out = nth_token<DT>(r, cut.key, cut.rank, s);
+}
+
+__device__ __forceinline__ Row row_of(const SampleArgs& a, int64_t b, int32_t* state, int32_t* flags) {
+  *state = state_of(a, b);
+  *flags = a.allow_bits && *state >= a.num_states ? BPD_FLAG_STATE_RANGE : 0;
+  const bool some = !a.allow_bits || (*state >= 0 && *state < a.num_states);
+  return Row{static_cast<const char*>(a.logits) + b * a.ld * (a.dtype == BPD_DTYPE_F32 ? 4 : 2),
+             a.allow_bits && some ? reinterpret_cast<const uint8_t*>(a.allow_bits + int64_t(*state) * a.words) : nullptr,
+             some ? a.vocab : 0};
+}
+
+template <int DT, bool Draw>
+__global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
+  __shared__ Scratch s;
+  const int64_t b = blockIdx.x;
+  int32_t state, flags;
+  const Row r = row_of(a, b, &state, &flags);
+  Cut cut{0xFFFFFFFFu, 0, 0};
+  int64_t last = -1;
+  float logprob = -INFINITY;
+  bool bad = false;
+  sample_row<DT>(a, r, asked_of(a, b), b, Draw, s, &cut, &last, &logprob, &bad);
+  if (bad) flags |= BPD_FLAG_LOGITS;
+  if (flags && a.err && threadIdx.x == 0) atomicOr(a.err, flags);
+  if constexpr (Draw) {
+    if (threadIdx.x == 0) store_drawn(a, b, state, last, logprob);
+    return;
+  }
+  constexpr int kBytes = DT == BPD_DTYPE_F32 ? 4 : 2;
+  const uint32_t none = DT == BPD_DTYPE_F32 ? 0xFF800000u : DT == BPD_DTYPE_BF16 ? 0xFF80u : 0xFC00u;
+  char* out = static_cast<char*>(a.out) + b * a.out_ld * kBytes;
+  const auto put = [&](int64_t t, uint32_t x) {
+    if (kBytes == 4) reinterpret_cast<uint32_t*>(out)[t] = x;
+    else reinterpret_cast<uint16_t*>(out)[t] = uint16_t(x);
+  };
+  for (int64_t t = threadIdx.x * kRun; t < a.vocab; t += kStep) {
+    const Run run = run_at(t, a.vocab);
+    uint32_t keep = r.vocab ? run_bits(r, run) : 0;
+    const Raw<DT> raw = load_raw<DT>(static_cast<const char*>(a.logits) + b * a.ld * kBytes, run, a.vocab);
+    float z[kRun];
+    unpack<DT>(raw, z);
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      const uint32_t key = key_of(z[j]);
+      const bool in = key > cut.key || (key == cut.key && run.t + j <= last);
+      const uint32_t x = kBytes == 4 ? raw.w[kBytes == 4 ? j / 4 : 0][j % 4] : raw.w[0][j / 2] >> (16 * (j & 1)) & 0xFFFFu;
+      if (run.own >> j & 1) put(run.t + j, in && (keep >> j & 1) ? x : none);
+    }
+  }
+  for (int64_t t = a.vocab + threadIdx.x; t < a.cols; t += kThreads) put(t, none);
+}
+
+template <int DT, bool Draw>
+int launch_sample_rows(const SampleArgs& a, hipStream_t s) {
+  sample_kernel<DT, Draw><<<uint32_t(a.rows), kThreads, 0, s>>>(a);
+  BPD_LAUNCHED();
+  return BPD_OK;
+}
+template <bool Draw>
+int launch_sample(const SampleArgs& a, hipStream_t s) {
+  if (a.dtype == BPD_DTYPE_BF16) return launch_sample_rows<BPD_DTYPE_BF16, Draw>(a, s);
+  if (a.dtype == BPD_DTYPE_F16) return launch_sample_rows<BPD_DTYPE_F16, Draw>(a, s);
+  return launch_sample_rows<BPD_DTYPE_F32, Draw>(a, s);
+}
+
+// --------------------------------------------------------------- the host --
+void host_sample(const SampleArgs& a, bool draw) {
+  int32_t flags = 0;
+  std::vector<int32_t> order;
+  std::vector<double> w;
+  for (int64_t b = 0; b < a.rows; ++b) {
+    const Asked want = asked_of(a, b);
+    const int32_t state = state_of(a, b);
+    if (a.allow_bits && state >= a.num_states) flags |= BPD_FLAG_STATE_RANGE;
+    const bool some = !a.allow_bits || (state >= 0 && state < a.num_states);
+    const uint32_t* bits = a.allow_bits && some ? a.allow_bits + int64_t(state) * a.words : nullptr;
+    const auto z = [&](int64_t t) { return load_elem(a.logits, a.dtype, b * a.ld + t); };
+    bool bad = false;
+    order.clear();
+    for (int64_t t = 0; t < (some ? a.vocab : 0); ++t) {
+      if (!allowed(bits, t) || z(t) == -INFINITY) continue;
+      bad |= !(z(t) < INFINITY);
+      order.push_back(int32_t(t));
+    }
+    if (bad) flags |= BPD_FLAG_LOGITS, order.clear();
+    int64_t n = int64_t(order.size());
+    double whole = 1.0;
+    if (n > 0) {
+      std::sort(order.begin(), order.end(), [&](int32_t x, int32_t y) { return z(x) > z(y) || (z(x) == z(y) && x < y); });
+      const double top = z(order[0]);
+      if (!(want.temp > 0.0)) n = 1;
+      else if (want.top_k > 0) n = std::min(n, want.top_k);
+      w.resize(size_t(n));
+      whole = 0.0;
+      for (int64_t i = 0; i < n; ++i) whole += w[i] = want.temp > 0.0 ? std::exp((z(order[i]) - top) / want.temp) : 1.0;
+      if (want.top_p < 1.0f) {
+        const double most = double(want.top_p) * whole;
+        double upto = 0.0;
+        int64_t i = 0;
+        while (i < n && (i == 0 || upto < most)) upto += w[i++];
+        n = i, whole = upto;
+      }
+      if (want.min_p > 0.0 && want.temp > 0.0) {
+        const double least = want.temp * std::log(want.min_p);
+        int64_t i = n;
+        while (z(order[i - 1]) - top < least) --i;
+        if (i < n) {
+          n = i, whole = 0.0;
+          for (int64_t k = 0; k < n; ++k) whole += w[k];
+        }
+      }
+    }
+    if (draw) {
+      int64_t at = -1;
+      if (n > 0) {
+        const float u = a.uniforms[b];
+        const double target = u > 0.0f ? double(u) * whole : 0.0;
+        double upto = 0.0;
+        for (int64_t i = 0; i < n; ++i) {
+          if (!(w[i] > 0.0)) break;
+          upto += w[i], at = i;
+          if (upto > target) break;
+        }
+      }
+      store_drawn(a, b, state, at < 0 ? -1 : order[at],
+                  at < 0 ? -INFINITY
+                         : float((want.temp > 0.0 ? (z(order[at]) - double(z(order[0]))) / want.temp : 0.0) - std::log(whole)));
+      continue;
+    }
+    std::vector<char> keep(size_t(a.vocab), 0);
+    for (int64_t i = 0; i < n; ++i) keep[order[i]] = 1;
+    for (int64_t t = 0; t < a.cols; ++t) {
+      const bool in = t < a.vocab && keep[t];
+      if (a.dtype == BPD_DTYPE_F32) {
+        float* out = static_cast<float*>(a.out) + b * a.out_ld + t;
+        *out = in ? static_cast<const float*>(a.logits)[b * a.ld + t] : -INFINITY;
+      } else {
+        uint16_t* out = static_cast<uint16_t*>(a.out) + b * a.out_ld + t;
+        *out = in ? static_cast<const uint16_t*>(a.logits)[b * a.ld + t] : a.dtype == BPD_DTYPE_BF16 ? 0xFF80 : 0xFC00;
+      }
+    }
+  }
+  if (flags && a.err) *a.err |= flags;
+}
+
+int check_sample(const SampleArgs& a, bool draw) {
+  BPD_REQUIRE(elem_bytes(a.dtype) != 0, "unknown logits dtype code %d", a.dtype);
+  BPD_REQUIRE(a.rows >= 0 && a.rows < (int64_t(1) << 21), "at most 2^21 - 1 rows in one call");
+  BPD_REQUIRE(a.vocab >= 1 && a.vocab < (int64_t(1) << 31), "a vocabulary of 1 to 2^31 - 1 tokens (got %lld)",
+              (long long)a.vocab);
+  if (a.rows == 0) return BPD_OK;
+  BPD_REQUIRE(a.logits, "null pointer argument");
+  BPD_REQUIRE(a.temperature || (std::isfinite(a.temperature_all) && a.temperature_all >= 0.0f),
+              "the temperature must be finite and not negative");
+  BPD_REQUIRE(a.top_k || a.top_k_all >= 0, "top_k must not be negative");
+  BPD_REQUIRE(a.top_p || (a.top_p_all >= 0.0f && a.top_p_all <= 1.0f), "top_p must lie between 0 and 1");
+  BPD_REQUIRE(a.min_p || (a.min_p_all >= 0.0f && a.min_p_all <= 1.0f), "min_p must lie between 0 and 1");
+  BPD_REQUIRE(!a.allow_bits || (a.states && a.num_states >= 0 && a.words >= (a.vocab + 31) / 32),
+              "allow bits need states, and a row of ceil(vocab / 32) words");
+  if (draw) {
+    BPD_REQUIRE(a.uniforms && a.token && a.logprob, "null pointer argument");
+    BPD_REQUIRE(!a.tok_next || a.allow_bits, "a grammar needs its allow bits");
+    BPD_REQUIRE(!(a.write_back || a.next_state) || a.tok_next, "states are advanced through tok_next only");
+  } else {
+    BPD_REQUIRE(a.out && a.cols >= a.vocab && (a.rows == 1 || a.out_ld >= a.cols), "the output's rows overlap or are too short");
+  }
+  return BPD_OK;
+}
+
+}  // namespace
+}  // namespace bpd
+
+using namespace bpd;
+
+#define BPD_SAMPLE_ARGS                                                                                               \
+  SampleArgs a {}; /* by name: two calls share it */                                                                  \
+  a.logits = logits, a.dtype = dtype, a.rows = rows, a.vocab = vocab, a.ld = ld, a.temperature = temperature,         \
+  a.temperature_all = temperature_all, a.top_k = top_k, a.top_k_all = top_k_all, a.top_p = top_p,                     \
+  a.top_p_all = top_p_all, a.min_p = min_p, a.min_p_all = min_p_all, a.allow_bits = allow_bits, a.words = words,      \
+  a.num_states = num_states, a.slots = slots, a.err = err
+#define BPD_DRAW_ARGS                                                                                                 \
+  BPD_SAMPLE_ARGS, a.states = states, a.uniforms = uniforms, a.tok_next = tok_next, a.write_back = write_back,        \
+                   a.token = token, a.logprob = logprob, a.next_state = next_state
+#define BPD_TRUNCATE_ARGS \
+  BPD_SAMPLE_ARGS, a.states = const_cast<int32_t*>(states), a.out = out, a.cols = cols, a.out_ld = out_ld
+
+extern "C" int bpd_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, const float* uniforms,
+                          const float* temperature, float temperature_all, const int32_t* top_k, int32_t top_k_all,
+                          const float* top_p, float top_p_all, const float* min_p, float min_p_all,
+                          const uint32_t* allow_bits, int64_t words, int32_t num_states, const int32_t* tok_next,
+                          int32_t* states, const int64_t* slots, int write_back, int32_t* token, float* logprob,
+                          int32_t* next_state, int32_t* err, void* stream) {
+  BPD_DRAW_ARGS;
+  if (int rc = check_sample(a, true)) return rc;
+  return rows == 0 ? BPD_OK : launch_sample<true>(a, as_stream(stream));
+}
+
+extern "C" int bpd_host_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld,
+                               const float* uniforms, const float* temperature, float temperature_all,
+                               const int32_t* top_k, int32_t top_k_all, const float* top_p, float top_p_all,
+                               const float* min_p, float min_p_all, const uint32_t* allow_bits, int64_t words,
+                               int32_t num_states, const int32_t* tok_next, int32_t* states, const int64_t* slots,
+                               int write_back, int32_t* token, float* logprob, int32_t* next_state, int32_t* err) {
+  BPD_DRAW_ARGS;
+  if (int rc = check_sample(a, true)) return rc;
+  if (rows > 0) host_sample(a, true);
+  return BPD_OK;
+}
+
+extern "C" int bpd_truncate(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, void* out,
+                            int64_t cols, int64_t out_ld, const float* temperature, float temperature_all,
+                            const int32_t* top_k, int32_t top_k_all, const float* top_p, float top_p_all,
+                            const float* min_p, float min_p_all, const uint32_t* allow_bits, int64_t words,
+                            int32_t num_states, const int32_t* states, const int64_t* slots, int32_t* err,
+                            void* stream) {
+  BPD_TRUNCATE_ARGS;
+  if (int rc = check_sample(a, false)) return rc;
+  return rows == 0 ? BPD_OK : launch_sample<false>(a, as_stream(stream));
+}
+
+extern "C" int bpd_host_truncate(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, void* out,
+                                 int64_t cols, int64_t out_ld, const float* temperature, float temperature_all,
+                                 const int32_t* top_k, int32_t top_k_all, const float* top_p, float top_p_all,
+                                 const float* min_p, float min_p_all, const uint32_t* allow_bits, int64_t words,
+                                 int32_t num_states, const int32_t* states, const int64_t* slots, int32_t* err) {
+  BPD_TRUNCATE_ARGS;
+  if (int rc = check_sample(a, false)) return rc;
+  if (rows > 0) host_sample(a, false);
+  return BPD_OK;
+}

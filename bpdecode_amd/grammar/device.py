@@ -30,6 +30,7 @@ import torch
 
 from .. import _lib
 from .._lib import PDA_CONFIG_WORDS, PDA_MAX_CONFIGS, PDA_MAX_DEPTH, check, lib, ptr
+from ..ops import dense_sample
 from ..tokenizer import Vocabulary
 from .nfa import RuleNFA
 from .frames import frame_lists
@@ -611,6 +612,23 @@ class CFGConstraintBatch:
         self._flush()
         _, status = pda_step(self._pool, self.g, tk, slots, self._flags, self._err, low32=True)
         return status
+
+    def sample(self, seq_ids, logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """Draw a token per sequence from ``logits`` [len(seq_ids), columns]
+        under the grammar and advance each sequence by it
+        (:func:`~bpdecode_amd.ops.sample`).  Returns (int32 tokens, float32
+        log-probabilities); a sequence that is broken or allows nothing yields
+        -1 and is broken."""
+        slots = self._slots(seq_ids)
+        self._flush()
+        rows = torch.arange(len(seq_ids), dtype=torch.int32, device=self.device)
+        token, logprob = dense_sample(
+            logits, uniforms, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, vocab=self.g.vocab_size,
+            allow_bits=pda_compute_mask(self.g, self._pool, slots), bit_rows=torch.where(self._flags[slots], -1, rows),
+            err=self._err)
+        pda_step(self._pool, self.g, token.clamp(min=0), slots, self._flags, self._err)
+        self._flags[slots] |= token < 0
+        return token, logprob
 
     def is_complete(self, seq_id: Hashable) -> bool:
         slot = self._slot_of[seq_id]

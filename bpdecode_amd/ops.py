@@ -24,6 +24,7 @@ walked by the table builder, entry for entry the same ``step``.
 from __future__ import annotations
 
 import ctypes as C
+import operator
 from dataclasses import dataclass, replace
 
 import numpy as np
@@ -988,6 +989,201 @@ def verify_draft(logits: torch.Tensor, draft_tokens: torch.Tensor, uniforms: tor
         return _walked_verify(logits, draft_tokens, uniforms, fsa, states, **kw)
     return dense_verify(logits, draft_tokens, uniforms, tok_next=fsa.tok_next, allow_bits=fsa.ensure_allow_bits(),
                         states=states, **kw)
+
+
+def _asked(value, name: str, rows: int, dtype: torch.dtype, what) -> tuple[torch.Tensor | None, object]:
+    """(tensor of one value per row, None) or (None, the value for all)."""
+    if isinstance(value, torch.Tensor):
+        if value.shape != (rows,):
+            raise RuntimeError(f"one {name} per row, or one number")
+        return value.to(dtype).contiguous(), what(0)
+    return None, what(value)
+
+
+def _cut_args(logits, temperature, top_k, top_p, min_p, vocab, allow_bits, states, slots, err, *others):
+    """What sampling and truncation hand on alike: (logits with unit column
+    stride, rows, vocabulary, arguments up to the row stride, the cuts and the
+    allow bits, the tensors that the arguments point to)."""
+    if logits.dim() != 2:
+        raise RuntimeError("logits must be [batch, vocab]")
+    B, columns = logits.shape
+    V = columns if vocab is None else vocab
+    if not 1 <= V <= columns:
+        raise RuntimeError(f"logits have {columns} columns for a vocabulary of {V} tokens")
+    code = _lib.dtype_code(logits.dtype)
+    t, t_all = _asked(temperature, "temperature", B, torch.float32, float)
+    k, k_all = _asked(top_k, "top_k", B, torch.int32, lambda x: min(operator.index(x), 2 ** 31 - 1))
+    p, p_all = _asked(top_p, "top_p", B, torch.float32, float)
+    m, m_all = _asked(min_p, "min_p", B, torch.float32, float)
+    dev = _same_device(logits, t, k, p, m, allow_bits, states, slots, *others)
+    word = _lib.err_ptr(err, dev)
+    S = words = 0
+    sl = None
+    if allow_bits is not None:
+        if allow_bits.dim() != 2 or allow_bits.dtype != torch.int32 or allow_bits.shape[1] != (V + 31) // 32:
+            raise RuntimeError(f"allow_bits must be int32 [states, {(V + 31) // 32}]")
+        if states is None:
+            raise RuntimeError("allow_bits needs one state per row")
+        allow_bits = allow_bits.contiguous()
+        S, words = allow_bits.shape
+        if slots is not None:
+            if slots.numel() != B:
+                raise RuntimeError("one slot per row")
+            sl = slots.to(torch.int64).contiguous()
+        elif states.numel() != B:
+            raise RuntimeError(f"one state per row (got {states.numel()} states for {B} rows)")
+    elif states is not None or slots is not None:
+        raise RuntimeError("states without a grammar")
+    work, _ = _unit_stride_rows(logits)
+    head = (work.data_ptr(), code, B, V, work.stride(0) if B > 1 else columns)
+    cuts = (ptr(t), t_all, ptr(k), k_all, ptr(p), p_all, ptr(m), m_all, ptr(allow_bits), words, S)
+    return work, dev, B, V, head, cuts, ptr(sl), word, (t, k, p, m, allow_bits, sl)
+
+
+def dense_sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, vocab=None, tok_next=None,
+                 allow_bits=None, bit_rows=None, states=None, slots=None, write_back=False, err=None):
+    """:func:`sample` over the tables themselves: ``allow_bits`` (packed, one
+    row per state) with ``tok_next`` and ``states`` (the state of row b is
+    ``states[slots[b]]`` with ``slots``, and ``write_back`` updates it there) or
+    with ``bit_rows`` int32 [batch], the row of ``allow_bits`` of each (-1:
+    allows nothing).  ``vocab``: columns that are tokens (all of ``logits``, or
+    of ``tok_next``, without it); ``err``: int32 [1] on the logits' device, flags
+    are OR-ed into it.  (token, logprob), and with ``tok_next`` the state."""
+    if tok_next is not None:
+        if vocab is None:
+            vocab = tok_next.shape[-1]
+        if tok_next.dim() != 2 or tok_next.shape[1] != vocab:
+            raise RuntimeError(f"tok_next has {list(tok_next.shape)} entries for a vocabulary of {vocab} tokens")
+        if states is None:
+            raise RuntimeError("tok_next needs the rows' states")
+        tok_next = _i32(tok_next)
+    if (tok_next is None) == (bit_rows is None) and allow_bits is not None:
+        raise RuntimeError("allow_bits needs tok_next or bit_rows")
+    if allow_bits is None and (tok_next is not None or bit_rows is not None):
+        raise RuntimeError("tok_next and bit_rows need allow_bits")
+    if tok_next is None and (write_back or states is not None or slots is not None):
+        raise RuntimeError("states are advanced through tok_next only")
+    if write_back and (states.dtype != torch.int32 or not states.is_contiguous()):
+        raise RuntimeError("write_back needs a contiguous int32 state pool")
+    at = states if tok_next is not None else bit_rows
+    at = None if at is None else _i32(at)
+    if uniforms.shape != logits.shape[:1] or uniforms.dtype != torch.float32:
+        raise RuntimeError("uniforms must be float32 [batch]")
+    uniforms = uniforms.contiguous()
+    work, dev, B, V, head, cuts, sl, word, kept = _cut_args(logits, temperature, top_k, top_p, min_p, vocab, allow_bits, at,
+                                                           slots, err, uniforms, tok_next)
+    if tok_next is not None and tok_next.shape[0] != allow_bits.shape[0]:
+        raise RuntimeError(f"tok_next has {tok_next.shape[0]} states but allow_bits has {allow_bits.shape[0]}")
+    token, state = logits.new_empty((2, B), dtype=torch.int32).unbind(0)
+    logprob = logits.new_empty(B, dtype=torch.float32)
+    args = (*head, uniforms.data_ptr(), *cuts, ptr(tok_next), ptr(at), sl, int(write_back), token.data_ptr(),
+            logprob.data_ptr(), state.data_ptr() if tok_next is not None else None, word)
+    if dev.type == "cuda":
+        check(lib().bpd_sample(*args, _lib.stream_of(dev)))
+    else:
+        check(lib().bpd_host_sample(*args))
+    return (token, logprob) if tok_next is None else (token, logprob, state)
+
+
+def dense_truncate(logits, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, vocab=None, allow_bits=None, bit_rows=None,
+                   slots=None, out=None, err=None):
+    """:func:`truncate` over the tables themselves: ``bit_rows`` int32, the row
+    of ``allow_bits`` of each row of logits (of ``bit_rows[slots[b]]`` with
+    ``slots``); ``out``: a tensor like ``logits`` to write to, which may be
+    ``logits``."""
+    work, dev, B, V, head, cuts, sl, word, kept = _cut_args(logits, temperature, top_k, top_p, min_p, vocab, allow_bits,
+                                                           None if bit_rows is None else _i32(bit_rows), slots, err, out)
+    at = None if bit_rows is None else _i32(bit_rows)
+    if out is None:
+        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
+    elif out.shape != logits.shape or out.dtype != logits.dtype:
+        raise RuntimeError(f"out must be {logits.dtype} {list(logits.shape)}")
+    elif out is not logits and out.untyped_storage().data_ptr() == logits.untyped_storage().data_ptr() \
+            and (out.data_ptr() != logits.data_ptr() or out.stride() != logits.stride()):
+        raise RuntimeError("out must be logits itself or share no memory with it")
+    to, copied = _unit_stride_rows(out)
+    args = (*head, to.data_ptr(), out.shape[1], to.stride(0) if B > 1 else out.shape[1], *cuts, ptr(at), sl, word)
+    if dev.type == "cuda":
+        check(lib().bpd_truncate(*args, _lib.stream_of(dev)))
+    else:
+        check(lib().bpd_host_truncate(*args))
+    if copied:
+        out.copy_(to)
+    return out
+
+
+def _walked_bits(fsa: FsaTensors, states: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """(allow bits, row of each state) for a bundle without ``tok_next``: its
+    allow-bit table, or masks walked for these states."""
+    bits = fsa.allow_bits_or_none()
+    if bits is not None:
+        return bits, states
+    return compute_mask(fsa, states), torch.arange(states.numel(), dtype=torch.int32, device=states.device)
+
+
+def _walked_sample(logits, uniforms, fsa: FsaTensors, states, **kw):
+    states = _i32(states)
+    bits, at = _walked_bits(fsa, states)
+    token, logprob = dense_sample(logits, uniforms, vocab=fsa.vocab_size, allow_bits=bits, bit_rows=at, **kw)
+    nxt = advance_state(fsa, states, token.clamp(min=0))
+    return token, logprob, torch.where(token < 0, -1, nxt)
+
+
+def sample(logits: torch.Tensor, uniforms: torch.Tensor, fsa: FsaTensors | None = None, states: torch.Tensor | None = None,
+           *, temperature: float | torch.Tensor = 1.0, top_k: int | torch.Tensor = 0, top_p: float | torch.Tensor = 1.0,
+           min_p: float | torch.Tensor = 0.0):
+    """One token for each row of ``logits`` [batch, columns], drawn by
+    ``uniforms`` float32 [batch] in [0, 1).
+
+    Tokens that the grammar ``fsa`` allows in the row's state stand in the
+    order of falling logits, equal ones in that of their index.  Of their
+    softmax at ``temperature``, ``top_k`` keeps the first k (0: all), ``top_p`` of
+    these the first that hold that share of their probability (1: all), and
+    ``min_p`` those at least that share as likely as the first (0: all); the
+    token is the first of the order whose running sum passes the row's uniform
+    number times the sum of what is kept.  Temperature 0 keeps the first alone.
+    Each is one number or a tensor of one per row.  Columns past the grammar's
+    vocabulary never count.
+
+    Returns int32 tokens and float32 log-probabilities (of the token among
+    what is kept), and with ``fsa`` and ``states`` (one per row) the states after
+    the tokens; a row that allows nothing yields -1, -inf and -1."""
+    kw = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p}
+    if fsa is None:
+        if states is not None:
+            raise RuntimeError("states without a grammar")
+        return dense_sample(logits, uniforms, **kw)
+    if states is None:
+        raise RuntimeError("a grammar needs one state per row")
+    if fsa.tok_next is None:
+        return _walked_sample(logits, uniforms, fsa, states, **kw)
+    return dense_sample(logits, uniforms, tok_next=fsa.tok_next, allow_bits=fsa.ensure_allow_bits(), states=states, **kw)
+
+
+def truncate(logits: torch.Tensor, fsa: FsaTensors | None = None, states: torch.Tensor | None = None, *,
+             temperature: float | torch.Tensor = 1.0, top_k: int | torch.Tensor = 0, top_p: float | torch.Tensor = 1.0,
+             min_p: float | torch.Tensor = 0.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The logits that :func:`sample` would draw from, ``-inf`` elsewhere (the
+    kept ones as they are, not divided by the temperature).  Their softmax at
+    the same temperature is the distribution of the draw: what a draft is
+    sampled from, and what :func:`verify_draft` on them verifies against."""
+    kw = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p, "out": out}
+    if fsa is None:
+        if states is not None:
+            raise RuntimeError("states without a grammar")
+        return dense_truncate(logits, **kw)
+    if states is None:
+        raise RuntimeError("a grammar needs one state per row")
+    if fsa.tok_next is not None:
+        bits, at = fsa.ensure_allow_bits(), states
+    else:
+        bits, at = _walked_bits(fsa, _i32(states))
+    return dense_truncate(logits, vocab=fsa.vocab_size, allow_bits=bits, bit_rows=at, **kw)
+
+
+def truncate_(logits: torch.Tensor, fsa: FsaTensors | None = None, states: torch.Tensor | None = None, **kw) -> torch.Tensor:
+    """:func:`truncate` in place."""
+    return truncate(logits, fsa, states, out=logits, **kw)
 
 
 # registers torch.ops.bpdecode.* (the reference loads its extension at this point)

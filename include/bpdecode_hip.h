@@ -701,6 +701,57 @@ int bpd_host_verify(const void* logits, int dtype, int64_t rows, int32_t drafts,
                     const int32_t* bit_rows, int write_back, int32_t* accepted,
                     int32_t* next_token, int32_t* next_state, int32_t* err);
 
+/* bpd_sample: one token per row from logits [rows, >= vocab] (row stride ld
+ * elements) by uniforms[b] in [0, 1).  z: the logits that the row's grammar
+ * state states[slots ? slots[b] : b] allows (allow_bits uint32 [num_states,
+ * words], NULL: all), those of -inf left out; w = exp((z - max z) /
+ * temperature).  Tokens stand in the order of falling z, equal ones in that of
+ * their index.  top_k (0 or less: all) keeps the first k; top_p (1 or more:
+ * all) of these the first whose sum of w is top_p of theirs at least, one at
+ * least; min_p (0 or less: all; over 1 as 1) those with z - max z >=
+ * temperature * log(min_p).  token[b] is the first of the order whose running
+ * sum passes uniforms[b] times the sum of what is kept, logprob[b] the
+ * logarithm of its share of that sum.  Temperature 0 (or not positive and
+ * finite): the first token.  Each of the four is float (top_k int32) [rows] on
+ * the device, or NULL and one value for all.  A row without tokens (its state
+ * allows none, is negative or, BPD_FLAG_STATE_RANGE, not below num_states;
+ * every allowed logit -inf; one +inf or NaN, BPD_FLAG_LOGITS): token -1,
+ * logprob -inf.  With tok_next, next_state[b] (may be NULL) and, with
+ * write_back, the pool entry become the state after the token, -1 where there
+ * is none.  Sums that decide are held in 64 bits.
+ * bpd_truncate: out [rows, cols >= vocab] (row stride out_ld) = the logits
+ * that bpd_sample would draw from, -inf elsewhere; out may be logits itself
+ * (the same rows), and overlaps them in no other way.  bpd_verify on
+ * truncated logits verifies drafts against the truncated distribution.
+ * Rows may lie at any element.  No counterpart in the reference, which leaves
+ * sampling to its caller. */
+int bpd_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld,
+               const float* uniforms, const float* temperature, float temperature_all,
+               const int32_t* top_k, int32_t top_k_all, const float* top_p, float top_p_all,
+               const float* min_p, float min_p_all, const uint32_t* allow_bits, int64_t words,
+               int32_t num_states, const int32_t* tok_next, int32_t* states,
+               const int64_t* slots, int write_back, int32_t* token, float* logprob,
+               int32_t* next_state, int32_t* err, void* stream);
+int bpd_host_sample(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld,
+                    const float* uniforms, const float* temperature, float temperature_all,
+                    const int32_t* top_k, int32_t top_k_all, const float* top_p, float top_p_all,
+                    const float* min_p, float min_p_all, const uint32_t* allow_bits, int64_t words,
+                    int32_t num_states, const int32_t* tok_next, int32_t* states,
+                    const int64_t* slots, int write_back, int32_t* token, float* logprob,
+                    int32_t* next_state, int32_t* err);
+int bpd_truncate(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, void* out,
+                 int64_t cols, int64_t out_ld, const float* temperature, float temperature_all,
+                 const int32_t* top_k, int32_t top_k_all, const float* top_p, float top_p_all,
+                 const float* min_p, float min_p_all, const uint32_t* allow_bits, int64_t words,
+                 int32_t num_states, const int32_t* states, const int64_t* slots, int32_t* err,
+                 void* stream);
+int bpd_host_truncate(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t ld,
+                      void* out, int64_t cols, int64_t out_ld, const float* temperature,
+                      float temperature_all, const int32_t* top_k, int32_t top_k_all,
+                      const float* top_p, float top_p_all, const float* min_p, float min_p_all,
+                      const uint32_t* allow_bits, int64_t words, int32_t num_states,
+                      const int32_t* states, const int64_t* slots, int32_t* err);
+
 /* The paged key/value cache in 4 bits.  pages uint8 [num_pages, kv_heads,
  * bytes], 16-byte aligned; the block of one page and head holds, for its
  * page_size tokens in order: key codes [page_size, head_dim / 2], value codes

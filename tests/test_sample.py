@@ -1,0 +1,430 @@
+"""Sampling with temperature, top-k, top-p and min-p (ops.sample,
+ops.dense_sample, ConstraintBatch.sample, CFGConstraintBatch.sample) and
+truncation by the same cuts, against a plain 64-bit form.
+
+Tokens and kept sets are whole and have to be equal: the kernels sum weights
+in whole numbers of 2^-45 of the largest or finer, the plain form in 64-bit
+floats, so a border would have to lie within about 1e-9 of a token's weight
+for the two to differ.  Log-probabilities are rounded to float32 once (2^-24 of
+themselves) from sums that are right to 1e-9.  Numbers asked for are float32."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from bpdecode_amd import _lib, ops, synth
+from bpdecode_amd.batch import BROKEN, ConstraintBatch
+from bpdecode_amd.grammar.device import CFGConstraintBatch, build_pda_tensors
+from bpdecode_amd.grammar.gbnf import parse_gbnf
+from bpdecode_amd.grammar.pda import CompiledGrammar
+from bpdecode_amd.ops import FsaTensors
+from tests import _step_ref as R
+from tests._util import PDA_VOCAB, TOY_VOCAB
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+INF = float("inf")
+MIXED = [(1.0, 0, 1.0, 0.0), (0.7, 0, 0.9, 0.0), (1.3, 5, 1.0, 0.0), (0.0, 3, 0.5, 0.5), (1.0, 0, 1.0, 0.1), (0.5, 40, 0.8, 0.02),
+         (2.5, 0, 0.999, 0.0), (1.0, 1, 1.0, 0.0), (1.0, 0, 0.0, 0.0), (1.0, 0, 1.0, 1.0), (30.0, 0, 0.5, 0.0), (0.05, 0, 0.95, 0.001),
+         (1.0, 10 ** 6, 0.3, 0.0), (float("nan"), 0, 1.0, 0.0), (INF, 0, 1.0, 0.0), (1e-38, 0, 0.9, 0.0), (3e38, 0, 0.5, 0.0),
+         (1.0, -4, 2.0, -1.0)]
+
+
+def asked_tensors(B, device, dealt=MIXED):
+    rows = [dealt[i % len(dealt)] for i in range(B)]
+    t, k, p, m = zip(*rows)
+    return (torch.tensor(t, device=device), torch.tensor(k, dtype=torch.int32, device=device), torch.tensor(p, device=device),
+            torch.tensor(m, device=device))
+
+
+def pack(allow: torch.Tensor) -> torch.Tensor:
+    a = torch.nn.functional.pad(allow, (0, -allow.shape[1] % 32)).view(allow.shape[0], -1, 32)
+    w = (a.to(torch.int64) << torch.arange(32)).sum(-1)
+    return torch.where(w >= 2 ** 31, w - 2 ** 32, w).to(torch.int32)
+
+
+def check(logits, V, asked, u, device, allow=None, **kw):
+    """Draws and truncates on ``device`` and compares both with the plain form."""
+    B = logits.shape[0]
+    x = logits.double().numpy()
+    a = tuple(v.double().cpu().numpy() if isinstance(v, torch.Tensor) else float(np.float32(v)) for v in asked)
+    want = R.rows(x, B, V, a, None if allow is None else allow.numpy())
+    names = dict(zip(("temperature", "top_k", "top_p", "min_p"), asked))
+    to = lambda t: t.to(device)  # noqa: E731
+    if allow is not None:
+        kw["allow_bits"] = to(pack(allow))
+        kw["bit_rows"] = torch.arange(B, dtype=torch.int32, device=device)
+    err = torch.zeros(1, dtype=torch.int32, device=device)
+    token, logprob = ops.dense_sample(to(logits), to(u), vocab=V, err=err, **names, **kw)
+    drawn = [R.draw(t, w, float(v)) for (t, w), v in zip(want, u)]
+    assert token.tolist() == [t for t, _ in drawn]
+    for got, (_, p) in zip(logprob.tolist(), drawn):
+        assert got == p or abs(got - p) <= 2.0 ** -24 * abs(p) + 1e-9
+    cut = ops.dense_truncate(to(logits), vocab=V, err=err, **names, **kw).cpu()
+    assert cut.dtype == logits.dtype and cut.shape == logits.shape
+    for b, (tokens, _) in enumerate(want):
+        assert np.array_equal(np.nonzero(~np.isneginf(cut[b].double().numpy()))[0], np.sort(tokens)), b
+        assert torch.equal(cut[b, tokens], logits[b, tokens])
+    bad = any(len(t) == 0 and (np.isnan(r).any() or np.isposinf(r).any()) for (t, _), r in zip(want, x[:, :V]))
+    assert (int(err) & _lib.FLAG_LOGITS != 0) == bad
+    return token, cut
+
+
+VOCABS = [1, 2, 7, 8, 9, 31, 33, 511, 1_000, 8_191, 8_193, 20_011]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+@pytest.mark.parametrize("V", VOCABS)
+def test_draws_and_kept_sets_equal_the_plain_form(V, dtype, device):
+    print(f"sample {V} {dtype} on {device}", flush=True)
+    B = 2 * len(MIXED)
+    g = torch.Generator().manual_seed(V)
+    logits = (2.5 * torch.randn(B, V + 3, generator=g)).to(dtype)
+    check(logits, V, asked_tensors(B, device), torch.rand(B, generator=g), device)
+    check(logits, V, (0.8, 12, 0.9, 0.01), torch.rand(B, generator=g), device)
+    check(logits, V, (1.0, 0, 1.0, 0.0), torch.rand(B, generator=g), device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+def test_a_large_vocabulary(dtype, device):
+    print(f"sample 151,936 {dtype} on {device}", flush=True)
+    B, V = (6 if device == "cpu" else 18), 151_936
+    g = torch.Generator().manual_seed(3)
+    logits = (3.0 * torch.randn(B, V, generator=g)).to(dtype)
+    allow = torch.rand(B, V, generator=g) < torch.linspace(0.0, 1.0, B)[:, None] ** 4
+    check(logits, V, asked_tensors(B, device), torch.rand(B, generator=g), device)
+    check(logits, V, asked_tensors(B, device, MIXED[1:]), torch.rand(B, generator=g), device, allow)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+@pytest.mark.parametrize("V", [5, 700, 9_001])
+def test_ties_zeros_and_far_logits(V, dtype, device):
+    """Rows of one value, of two, of zeros of both signs, of the type's lowest
+    and largest numbers, of subnormal ones; each asked for everything in turn."""
+    g = torch.Generator().manual_seed(V + 1)
+    fi = torch.finfo(dtype)
+    r = torch.rand(V, generator=g)
+    rows = [torch.full((V,), 3.0), torch.zeros(V), torch.where(r < 0.5, -0.0, 0.0), torch.where(r < 0.1, 1.0, -1.0),
+            torch.where(r < 0.02, 1.0, fi.min), torch.full((V,), fi.min), torch.full((V,), fi.max), torch.where(r < 0.3, fi.max, fi.min),
+            r * fi.tiny, -r * fi.tiny * 4, torch.round(8 * r), torch.where(r < 0.01, -INF, r), torch.linspace(-40, 40, V),
+            torch.where(r < 0.97, -INF, 5 * r)]
+    for i, row in enumerate(rows):
+        logits = row.expand(len(MIXED), V).contiguous().to(dtype)
+        print(f"ties row {i} of {V} {dtype} on {device}", flush=True)
+        check(logits, V, asked_tensors(len(MIXED), device), torch.rand(len(MIXED), generator=g), device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_many_equal_logits_of_a_large_vocabulary(dtype, device):
+    """More equal logits than 16 bits count: all, half, and behind some that differ."""
+    V = 151_936
+    g = torch.Generator().manual_seed(4)
+    few = torch.randperm(V, generator=g)[:900]
+    rows = torch.zeros(4, V)
+    rows[1, V // 2 - 7:] = -2.0
+    rows[2] = torch.finfo(dtype).min
+    rows[2, few] = 2 * torch.randn(900, generator=g)
+    rows[3] = -1.0
+    rows[3, few] = 3 + torch.randn(900, generator=g)
+    logits = rows.to(dtype)
+    for dealt in ([(1.0, 0, 1.0, 0.0)], [(1.0, 0, 0.75, 0.0)], [(0.9, 100_000, 0.99, 0.0)], [(1.5, 0, 1.0, 0.01)]):
+        check(logits, V, asked_tensors(4, device, dealt), torch.rand(4, generator=g), device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+def test_borders_of_the_uniform_numbers(dtype, device):
+    """0 draws the first of the order, the largest below 1 the last of equal
+    ones; a number on a border draws the token after it."""
+    V = 1_001
+    logits = torch.zeros(6, V)
+    logits[2:4, 8:] = -INF
+    logits[4] = torch.arange(V).flip(0) * 0.01
+    u = torch.tensor([0.0, 1 - 2.0 ** -24, 0.5, 0.875, 0.0, 2.0 ** -149])
+    token, _ = check(logits.to(dtype), V, (1.0, 0, 1.0, 0.0), u, device)
+    assert token.tolist() == [0, V - 1, 4, 7, 0, 0]
+    # two thirds of three, a quarter of four, exactly
+    logits = torch.full((2, V), -INF)
+    logits[0, [3, 500, 900, 1_000]] = 1.0
+    logits[1, 7:15] = -4.0
+    _, cut = check(logits.to(dtype), V, (1.0, 0, 0.75, 0.0), torch.tensor([0.4, 0.99]), device)
+    assert (~cut.isneginf()).sum(1).tolist() == [3, 6]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+def test_rows_without_a_softmax(dtype, device):
+    """NaN and +inf among the allowed logits, on masked ones, and rows of -inf."""
+    B, V = 8, 530
+    g = torch.Generator().manual_seed(5)
+    logits = torch.randn(B, V, generator=g)
+    logits[0, 7] = float("nan")
+    logits[1, 529] = INF
+    logits[2] = -INF
+    logits[3, 100] = -float("nan")
+    logits[4, 3] = INF
+    allow = torch.ones(B, V, dtype=torch.bool)
+    allow[4, 3] = allow[6] = False
+    allow[5] = False
+    allow[5, 528] = True
+    u = torch.rand(B, generator=g)
+    for one in ((1.0, 0, 1.0, 0.0), (0.0, 0, 1.0, 0.0), (0.7, 9, 0.9, 0.1)):
+        token, _ = check(logits.to(dtype), V, one, u, device, allow)
+        assert [t < 0 for t in token.tolist()] == [True, True, True, True, False, False, True, False]
+        assert int(token[5]) == 528
+        check(logits[4:].to(dtype), V, one, u[4:], device)
+
+
+def tables(g, S, V):
+    tok_next = torch.randint(0, S, (S, V), generator=g, dtype=torch.int32)
+    share = torch.tensor([0.9, 0.02, 0.3, 0.0, 1.0, 0.6])[:S]
+    tok_next[torch.rand(S, V, generator=g) >= share[:, None]] = -1
+    return tok_next
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_states_slots_and_their_advance(dtype, device):
+    B, V, S = 12, 3_001, 6
+    g = torch.Generator().manual_seed(6)
+    tn = tables(g, S, V)
+    logits = (2 * torch.randn(B, V + 7, generator=g)).to(dtype)
+    pool = torch.randint(0, S, (20,), generator=g, dtype=torch.int32)
+    slots = torch.randperm(20, generator=g)[:B]
+    pool[slots[:4]] = torch.tensor([-1, -2, S, 3], dtype=torch.int32)
+    u = torch.rand(B, generator=g)
+    states = pool[slots]
+    allow = torch.zeros(B, V, dtype=torch.bool)
+    inside = (states >= 0) & (states < S)
+    allow[inside] = tn[states[inside].long()] >= 0
+    want = [R.draw(*R.kept(logits[b, :V].double().numpy(), allow[b].numpy(), 0.9, 50, 0.95, 0.0), float(u[b])) for b in range(B)]
+    to = lambda t: t.to(device)  # noqa: E731
+    bits = to(pack(tn >= 0))
+    kw = {"temperature": 0.9, "top_k": 50, "top_p": 0.95, "tok_next": to(tn), "allow_bits": bits}
+    before = to(pool.clone())
+    err = torch.zeros(1, dtype=torch.int32, device=device)
+    token, logprob, state = ops.dense_sample(to(logits), to(u), states=before, slots=to(slots), err=err, **kw)
+    assert int(err) == _lib.FLAG_STATE_RANGE and torch.equal(before.cpu(), pool)
+    after = [-1 if t < 0 else int(tn[int(s), t]) for s, (t, _) in zip(states, want)]
+    assert token.tolist() == [t for t, _ in want] and state.tolist() == after
+    ops.dense_sample(to(logits), to(u), states=before, slots=to(slots), write_back=True, **kw)
+    changed = pool.clone()
+    changed[slots] = torch.tensor(after, dtype=torch.int32)
+    assert torch.equal(before.cpu(), changed)
+    by_row = ops.dense_sample(to(logits), to(u), states=to(states), **kw)
+    assert by_row[0].tolist() == token.tolist() and by_row[2].tolist() == after
+    cut = ops.dense_truncate(to(logits), temperature=0.9, top_k=50, top_p=0.95, vocab=V, allow_bits=bits, bit_rows=to(pool),
+                             slots=to(slots), err=err)
+    assert all((cut[b, t] > -INF) == (t >= 0) for b, (t, _) in enumerate(want))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+def test_rows_at_any_stride_and_alignment(dtype, device):
+    B, V = 5, 1_237
+    g = torch.Generator().manual_seed(7)
+    wide = (2 * torch.randn(B, 2 * V + 9, generator=g)).to(dtype).to(device)
+    u = torch.rand(2 * B, generator=g).to(device)[::2]
+    for view in (wide[:, 1:V + 1], wide[:, 3:3 + 2 * V:2], wide.t()[:V].t(), wide[0, 5:5 + V].expand(B, V), wide[1:2, 7:7 + V]):
+        n = view.shape[0]
+        kw = {"temperature": 0.9, "top_p": 0.9, "top_k": 300}
+        a = ops.dense_sample(view, u[:n], **kw)
+        b = ops.dense_sample(view.contiguous(), u[:n].contiguous(), **kw)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+        x, y = ops.truncate(view, **kw), ops.truncate(view.contiguous(), **kw)
+        assert torch.equal(x, y)
+    for view in (wide[:, 1:V + 1], wide[:, 3:3 + 2 * V:2]):  # in place, nothing beside the view touched
+        before = wide.clone()
+        want = ops.truncate(view, **kw)
+        got = ops.truncate_(view, **kw)
+        assert got is view and torch.equal(view, want)
+        view.copy_(ops.truncate(view * 0))
+        mask = torch.zeros_like(wide, dtype=torch.bool)
+        cols = torch.arange(wide.shape[1], device=device)
+        mask[:, cols[1:V + 1] if view.stride(1) == 1 else cols[3:3 + 2 * V:2]] = True
+        assert torch.equal(wide[~mask], before[~mask])
+        wide.copy_(before)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dense", [True, False])
+def test_a_batch_draws_as_masked_logits_do(dense, device):
+    """ConstraintBatch.sample is apply_mask, a draw and commit; truncate is
+    apply_mask and the cuts."""
+    fsa = FsaTensors.build("-?[0-9]+(\\.[0-9]+)?", TOY_VOCAB, dense=dense)
+    one, two = (ConstraintBatch(fsa, capacity=6, device=device) for _ in range(2))
+    for i in range(5):
+        one.add(i), two.add(i)
+    g = torch.Generator().manual_seed(8)
+    ids = [3, 0, 4, 1]
+    for step in range(12):
+        logits = torch.randn(4, TOY_VOCAB.size + 2, generator=g).to(device)
+        u = torch.rand(4, generator=g).to(device)
+        masked = two.apply_mask(ids, logits[:, :TOY_VOCAB.size].clone())
+        cuts = {"temperature": 0.8, "top_k": torch.tensor([0, 2, 5, 1], device=device), "top_p": 0.95}
+        cut = one.truncate(ids, logits.clone(), **cuts)
+        assert torch.equal(cut[:, :TOY_VOCAB.size], ops.truncate(masked, **cuts)) and cut[:, TOY_VOCAB.size:].isneginf().all()
+        token, logprob = one.sample(ids, logits, u, **cuts)
+        want, p = ops.sample(masked, u, **cuts)
+        assert torch.equal(token, want) and torch.equal(logprob, p)
+        two.commit(ids, token.clamp(min=0))
+        for i, t in zip(ids, token.tolist()):
+            assert one.state_of(i) == (two.state_of(i) if t >= 0 else BROKEN)
+        if step % 5 == 4:
+            one.reset(3), two.reset(3)
+    one.check_errors()
+    assert not one.is_broken(2)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_recursive_grammar_draws_as_masked_logits_do(device):
+    g = build_pda_tensors(CompiledGrammar.build(parse_gbnf(synth.JSON_GBNF)), PDA_VOCAB)
+    one, two = (CFGConstraintBatch(g, capacity=5, device=device) for _ in range(2))
+    for i in range(4):
+        one.add(i), two.add(i)
+    gen = torch.Generator().manual_seed(9)
+    ids = [2, 0, 3, 1]
+    for step in range(10):
+        logits = torch.randn(4, PDA_VOCAB.size, generator=gen).to(device)
+        if step == 6:
+            logits[1] = float("nan")
+        u = torch.rand(4, generator=gen).to(device)
+        masked = two.apply_mask(ids, logits.clone())
+        broken = [two.is_broken(i) for i in ids]
+        token, logprob = one.sample(ids, logits, u, top_p=0.9)
+        want, p = ops.sample(masked, u, top_p=0.9)
+        assert torch.equal(token, want) and torch.equal(logprob, p)
+        assert [t < 0 for t in token.tolist()] == [b or (step == 6 and r == 1) for r, b in enumerate(broken)]
+        two.commit(ids, token.clamp(min=0))
+        if step == 6:
+            two._broken[two._slots(ids)[1:2]] = True
+        assert [one.is_broken(i) for i in ids] == [two.is_broken(i) for i in ids]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_verification_of_truncated_logits(device):
+    """verify_draft on truncated logits emits kept tokens alone, with the
+    distribution of the draw: over a grid of uniform numbers every kept token
+    comes up as often as its probability asks, to one point of the grid."""
+    V, N = 300, 4_000
+    g = torch.Generator().manual_seed(10)
+    logits = (2 * torch.randn(1, V, generator=g)).to(device)
+    cuts = {"temperature": 0.9, "top_k": 30, "top_p": 0.9, "min_p": 0.01}
+    cut = ops.truncate(logits, **cuts)
+    tokens, w = R.kept(logits[0].double().cpu().numpy(), np.ones(V, bool), 0.9, 30, float(np.float32(0.9)), float(np.float32(0.01)))
+    u = ((torch.arange(N) + 0.5) / N).to(device)
+    none = torch.zeros(N, 0, dtype=torch.int32, device=device)
+    _, verified = ops.verify_draft(cut.expand(N, V)[:, None].contiguous(), none, u[:, None], temperature=0.9)
+    drawn, _ = ops.sample(logits.expand(N, V).contiguous(), u, **cuts)
+    p = torch.zeros(V, dtype=torch.float64)
+    p[torch.from_numpy(tokens)] = torch.from_numpy(w / w.sum())
+    for got in (verified, drawn):
+        assert ((torch.bincount(got.cpu().long(), minlength=V) - p * N).abs() <= 1.001).all()
+
+
+@pytest.mark.gpu
+def test_streams_and_captured_graphs(dev):
+    """Replays over new logits, uniform numbers and cuts, with eager work
+    between them; a side stream."""
+    B, V, S = 9, 40_003, 6
+    g = torch.Generator().manual_seed(11)
+    tn = tables(g, S, V).to(dev)
+    bits = pack((tn >= 0).cpu()).to(dev)
+    logits = torch.zeros(B, V, dtype=BF16, device=dev)
+    u, pool = torch.zeros(B, device=dev), torch.zeros(B, dtype=torch.int32, device=dev)
+    t, k, p, m = asked_tensors(B, dev)
+    kw = {"temperature": t, "top_k": k, "top_p": p, "min_p": m, "tok_next": tn, "allow_bits": bits}
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        ops.dense_sample(logits, u, states=pool.clone(), write_back=True, **kw)
+        ops.truncate(logits, temperature=t, top_k=k, top_p=p, min_p=m)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.dense_sample(logits, u, states=pool, write_back=True, **kw)
+        cut = ops.truncate(logits, temperature=t, top_k=k, top_p=p, min_p=m)
+    for seed in range(4):
+        g.manual_seed(100 + seed)
+        logits.copy_(2 * torch.randn(B, V, generator=g))
+        u.copy_(torch.rand(B, generator=g))
+        pool.copy_(torch.randint(-1, S, (B,), generator=g))
+        t.copy_(asked_tensors(B, dev, MIXED[seed:])[0])
+        p.copy_(asked_tensors(B, dev, MIXED[seed:])[2])
+        start = pool.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = ops.dense_sample(logits, u, states=start, **kw)
+        for x, y in zip(out, want):
+            assert torch.equal(x, y)
+        assert torch.equal(pool, want[2])
+        assert torch.equal(cut, ops.truncate(logits, temperature=t, top_k=k, top_p=p, min_p=m))
+        with torch.cuda.stream(side):
+            side.wait_stream(torch.cuda.default_stream())
+            again = ops.dense_sample(logits, u, states=start, **kw)
+        side.synchronize()
+        assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals(device):
+    z, u = torch.zeros(2, 40, device=device), torch.zeros(2, device=device)
+    bits, at = torch.zeros(3, 2, dtype=torch.int32, device=device), torch.zeros(2, dtype=torch.int32, device=device)
+    tn = torch.zeros(3, 40, dtype=torch.int32, device=device)
+    other = torch.zeros(2, device="meta")
+    bad = [
+        (dict(temperature=-1.0), "temperature"), (dict(temperature=float("nan")), "temperature"), (dict(temperature=INF), "temperature"),
+        (dict(temperature=torch.ones(3, device=device)), "one temperature per row"), (dict(top_k=-1), "top_k"),
+        (dict(top_p=1.5), "top_p"), (dict(top_p=float("nan")), "top_p"), (dict(min_p=-0.1), "min_p"), (dict(min_p=2.0), "min_p"),
+        (dict(top_k=torch.ones(2, 1, dtype=torch.int32, device=device)), "one top_k per row"), (dict(vocab=41), "columns"),
+        (dict(vocab=0), "columns"), (dict(allow_bits=bits), "bit_rows"), (dict(bit_rows=at), "allow_bits"),
+        (dict(allow_bits=bits[:, :1], bit_rows=at), "allow_bits must be"), (dict(allow_bits=bits.long(), bit_rows=at), "allow_bits must be"),
+        (dict(allow_bits=bits, bit_rows=at[:1]), "one state per row"), (dict(err=torch.zeros(1, device=device)), "err must be int32"),
+        (dict(min_p=other), "same device"),
+    ]
+    for kw, match in bad:
+        with pytest.raises(RuntimeError, match=match):
+            ops.dense_sample(z, u, **kw)
+        if "bit_rows" in kw and "allow_bits" not in kw:
+            match = "states without a grammar"
+        elif match == "bit_rows":
+            match = "one state per row"
+        with pytest.raises(RuntimeError, match=match):
+            ops.dense_truncate(z, **kw)
+    for kw, match in [
+        (dict(tok_next=tn, states=at), "need allow_bits"), (dict(tok_next=tn, allow_bits=bits), "states"),
+        (dict(tok_next=tn[:2], allow_bits=bits, states=at), "tok_next has 2 states"),
+        (dict(tok_next=tn, allow_bits=bits, states=at.long(), write_back=True), "contiguous int32"),
+        (dict(tok_next=tn[:, :39], vocab=40, allow_bits=bits, states=at), "entries"), (dict(write_back=True), "tok_next only"),
+        (dict(tok_next=tn, allow_bits=bits, states=at, slots=at[:1].long()), "one slot per row"),
+    ]:
+        with pytest.raises(RuntimeError, match=match):
+            ops.dense_sample(z, u, **kw)
+    for x in (u[:1], u.double(), u[:, None]):
+        with pytest.raises(RuntimeError, match="uniforms must be float32"):
+            ops.dense_sample(z, x)
+    with pytest.raises(RuntimeError, match="must be \\[batch, vocab\\]"):
+        ops.dense_sample(z[None], u[:1])
+    with pytest.raises(RuntimeError, match="not supported"):
+        ops.sample(z.double(), u)
+    with pytest.raises(RuntimeError, match="states without a grammar"):
+        ops.sample(z, u, None, at)
+    fsa = FsaTensors.build("a+b*", TOY_VOCAB, dense=True).to(device)
+    with pytest.raises(RuntimeError, match="one state per row"):
+        ops.sample(z, u, fsa)
+    with pytest.raises(RuntimeError, match="one state per row"):
+        ops.truncate(z, fsa)
+    wide = torch.zeros(2, 50, device=device)
+    for out, match in [(z[:1], "out must be"), (z.half(), "out must be")]:
+        with pytest.raises(RuntimeError, match=match):
+            ops.dense_truncate(z, out=out)
+    with pytest.raises(RuntimeError, match="share no memory"):
+        ops.dense_truncate(wide[:, :40], out=wide[:, 10:])
+    assert ops.dense_sample(z[:0], u[:0])[0].shape == (0,) and ops.truncate(z[:0]).shape == (0, 40)
