@@ -26,6 +26,7 @@ MAX_INLINE_VALUES = 960  # BPD_MAX_INLINE_VALUES
 MAX_PRIOR_INLINE_VALUES = 320  # BPD_MAX_PRIOR_INLINE_VALUES
 FLAG_STATE_RANGE, FLAG_TOKEN_RANGE, FLAG_PAGE_RANGE, FLAG_LOGITS = 1, 2, 4, 8
 MAX_DRAFTS = 63  # BPD_MAX_DRAFTS
+MAX_AXES = 4  # BPD_MAX_AXES
 PDA_MAX_CONFIGS = 8
 PDA_MAX_DEPTH = 32
 PDA_CONFIG_WORDS = 2 + PDA_MAX_CONFIGS + PDA_MAX_CONFIGS * PDA_MAX_DEPTH
@@ -164,6 +165,12 @@ _SIGNATURES = {
     "bpd_host_kv_append": (cint, [vp, i64, i32, i32, i32, cint, vp, i64, i64, i64, vp, i64, i64, i64, vp, i64,
                                   i64, i64, i32, vp, i64, i32, vp, i64, i32, vp, vp, vp, vp, i64, i32, cint,
                                   vp]),
+    "bpd_kv_append_axes": (cint, [vp, i64, i32, i32, i32, cint, vp, i64, i64, i64, vp, i64, i64, i64, vp, i64, i64,
+                                  i64, i32, vp, i64, i32, vp, i64, i32, vp, vp, vp, vp, i64, i32, cint, vp, i64, i64,
+                                  i64, i32, vp, vp, vp]),
+    "bpd_host_kv_append_axes": (cint, [vp, i64, i32, i32, i32, cint, vp, i64, i64, i64, vp, i64, i64, i64, vp, i64,
+                                       i64, i64, i32, vp, i64, i32, vp, i64, i32, vp, vp, vp, vp, i64, i32, cint,
+                                       vp, i64, i64, i64, i32, vp, vp]),
     "bpd_kv_read": (cint, [vp, i64, i32, i32, i32, cint, vp, vp, i64, i32, vp, i64, i32, vp, vp, vp, vp]),
     "bpd_host_kv_read": (cint, [vp, i64, i32, i32, i32, cint, vp, vp, i64, i32, vp, i64, i32, vp, vp, vp]),
     "bpd_kv_attend_workspace_bytes": (sz, [i64, i32, i32, i32, i32, i64]),

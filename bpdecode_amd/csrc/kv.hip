@@ -31,17 +31,58 @@ struct AppendArgs {
   int32_t rotary;
   int32_t interleaved;
   int32_t* err;
+  // positions apart from the place in the cache: of each token on `num_axes`
+  // axes (0: none), and the axis of each channel pair (null: the first)
+  const int32_t* places;
+  int64_t place_axis, place_row, place_token;
+  int32_t num_axes;
+  const int32_t* axes;
 };
 
+// A token's rows of the rotation's tables, by axis.
+struct Turns {
+  int32_t at[BPD_MAX_AXES];
+};
+__host__ __device__ __forceinline__ int32_t turn_on(const Turns& t, int32_t axis) {
+  int32_t x = t.at[0];
+  for (int k = 1; k < BPD_MAX_AXES; ++k) x = axis >= k ? t.at[k] : x;  // an axis past the last is read as it
+  return x;
+}
+// False where one lies outside the tables.
+__host__ __device__ __forceinline__ bool turns_of(const AppendArgs& a, int64_t b, int32_t i, Turns* t) {
+  bool ok = true;
+  for (int k = 0; k < BPD_MAX_AXES; ++k) {
+    const int32_t last = a.num_axes - 1, axis = k < last ? k : last;
+    t->at[k] = a.places[axis * a.place_axis + b * a.place_row + i * a.place_token];
+    ok = ok && t->at[k] >= 0 && t->at[k] < a.positions;
+  }
+  return ok;
+}
+
+// The axis of a pair; one that is not there is flagged.
+__host__ __device__ __forceinline__ int32_t axis_of(const AppendArgs& a, int32_t pair) {
+  const int32_t x = a.axes ? a.axes[pair] : 0;
+  if ((x < 0 || x >= a.num_axes) && a.err) {
+#ifdef __HIP_DEVICE_COMPILE__
+    atomicOr(a.err, BPD_FLAG_PAGE_RANGE);
+#else
+    *a.err |= BPD_FLAG_PAGE_RANGE;
+#endif
+  }
+  return x;
+}
+
 // Whether token i of request b is appended, and where; sets *bad where it
-// should be and cannot.  *turn: its row of the rotation's tables, or -1.
+// should be and cannot.  *turn: its row of the rotation's tables (without axes
+// of its own), or -1.
 __host__ __device__ __forceinline__ int64_t append_place(const AppendArgs& a, int64_t b, int32_t i, int64_t* pos,
                                                          int64_t* turn, bool* bad) {
   *bad = false;
   *turn = -1;
   if (a.counts && i >= a.counts[b]) return -1;
   *pos = int64_t(a.starts[b]) + i;
-  if (*pos < 0 || (a.rotary > 0 && *pos >= a.positions)) {
+  Turns t;
+  if (*pos < 0 || (a.num_axes > 0 ? !turns_of(a, b, i, &t) : a.rotary > 0 && *pos >= a.positions)) {
     *bad = true;
     return -1;
   }
@@ -84,7 +125,10 @@ enum Partners { kHalves, kNeighbours, kAnywhere };
 // rounded one by one (kv4.hpp); the codes come from the hardware's conversion.
 // Bound by memory: 49,000 tokens of 48 heads of 128, 1.2 GB with the rotated
 // queries, in 276 us, 4.4 TB/s, where a large copy reaches 4.9.
-template <int DT, int D, int Passes, int Mode>
+// With Axes a pair's row of the tables goes by its axis; 8 pairs of one axis
+// (blocks of them, as models with axes for time, height and width lay them out)
+// are read as without, others one by one.
+template <int DT, int D, int Passes, int Mode, bool Axes>
 __global__ __launch_bounds__(kKvThreads) void kv_append_kernel(AppendArgs a, uint32_t parts) {
   using B = KvBlock<D>;
   const int tid = threadIdx.x, slot = tid / B::per_head, d0 = tid % B::per_head * kKvWidth;
@@ -122,7 +166,28 @@ __global__ __launch_bounds__(kKvThreads) void kv_append_kernel(AppendArgs a, uin
   if (bad && a.err && tid == 0 && part == 0) atomicOr(a.err, BPD_FLAG_PAGE_RANGE);
   const bool turns = rotated && turn >= 0;
   float c[kKvWidth], sn[kKvWidth];
-  if (Mode != kAnywhere && turns) {
+  Turns own{};
+  if (Axes && turns) turns_of(a, b, i, &own);
+  bool apart = false;  // the pairs lie on several axes
+  if (Axes && Mode != kAnywhere && turns) {
+    constexpr int kPairs = Mode == kHalves ? kKvWidth : kKvWidth / 2;
+    const int32_t pair = Mode == kNeighbours ? d0 / 2 : upper ? d0 - half : d0;
+    int32_t axis[kPairs];
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) {
+      axis[j] = axis_of(a, pair + j);
+      apart |= axis[j] != axis[0];
+    }
+    turn = turn_on(own, axis[0]);
+    if (apart) {
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) {
+        const int64_t at = int64_t(turn_on(own, axis[j])) * half + pair + j;
+        c[j] = a.cos[at], sn[j] = Mode == kHalves && !upper ? -a.sin[at] : a.sin[at];
+      }
+    }
+  }
+  if (Mode != kAnywhere && turns && !apart) {
     const int64_t at = turn * half + (Mode == kNeighbours ? d0 / 2 : upper ? d0 - half : d0);
 #pragma unroll
     for (int k = 0; k < (Mode == kHalves ? 2 : 1); ++k) {
@@ -155,7 +220,10 @@ __global__ __launch_bounds__(kKvThreads) void kv_append_kernel(AppendArgs a, uin
         const uint16_t* from = kind[p] == 0 ? qs + head[p] * a.qs.head : ks + head[p] * a.ks.head;
 #pragma unroll
         for (int j = 0; j < kKvWidth; ++j)
-          val[j] = rotated_channel<DT>(from, d0 + j, a.rotary, a.interleaved, a.cos + turn * half, a.sin + turn * half);
+          val[j] = rotated_channel<DT>(from, d0 + j, a.rotary, a.interleaved, [&](int32_t pair, float* x, float* y) {
+            const int64_t at = (Axes ? turn_on(own, axis_of(a, pair)) : turn) * half + pair;
+            *x = a.cos[at], *y = a.sin[at];
+          });
       }
     }
     if (kind[p] == 0) {
@@ -197,13 +265,17 @@ void host_append(const AppendArgs& a) {
       bool bad;
       const int64_t page = append_place(a, b, i, &pos, &turn, &bad);
       if (bad && a.err) *a.err |= BPD_FLAG_PAGE_RANGE;
-      const float *cos = a.cos + std::max<int64_t>(turn, 0) * (a.rotary / 2),
-                  *sin = a.sin + std::max<int64_t>(turn, 0) * (a.rotary / 2);
+      Turns own{};
+      if (turn >= 0 && a.num_axes > 0) turns_of(a, b, i, &own);
+      const auto angle = [&](int32_t pair, float* c, float* s) {
+        const int64_t at = (a.num_axes > 0 ? turn_on(own, axis_of(a, pair)) : turn) * (a.rotary / 2) + pair;
+        *c = a.cos[at], *s = a.sin[at];
+      };
       for (int32_t h = 0; h < a.heads; ++h) {
         const uint16_t* x = a.q + b * a.qs.row + i * a.qs.token + h * a.qs.head;
         uint16_t* out = a.q_out + ((b * a.tokens + i) * a.heads + h) * D;
         for (int32_t d = 0; d < D; ++d)
-          out[d] = turn >= 0 ? float_elem16<DT>(rotated_channel<DT>(x, d, a.rotary, a.interleaved, cos, sin)) : 0;
+          out[d] = turn >= 0 ? float_elem16<DT>(rotated_channel<DT>(x, d, a.rotary, a.interleaved, angle)) : 0;
       }
       if (page < 0) continue;
       const int32_t t = int32_t(pos % a.page.page_size);
@@ -219,7 +291,7 @@ void host_append(const AppendArgs& a) {
           float val[kKvGroup];
           uint32_t most = 0;
           for (int32_t j = 0; j < kKvGroup; ++j) {
-            val[j] = rotated_channel<DT>(x, g * kKvGroup + j, is_v ? 0 : a.rotary, a.interleaved, cos, sin);
+            val[j] = rotated_channel<DT>(x, g * kKvGroup + j, is_v ? 0 : a.rotary, a.interleaved, angle);
             most = std::max(most, float_bits(val[j]) & 0x7FFFFFFFu);
           }
           const int32_t e = kv_scale_byte<DT>(most);
@@ -326,6 +398,9 @@ int check_append(const AppendArgs& a, int dtype) {
   BPD_REQUIRE(a.rotary >= 0 && a.rotary % 2 == 0 && a.rotary <= a.page.dim,
               "the rotated channels must be even and at most head_dim (got %d of %d)", a.rotary, a.page.dim);
   BPD_REQUIRE(a.rotary == 0 || (a.cos && a.sin && a.positions >= 0), "the rotation needs its tables");
+  BPD_REQUIRE(a.num_axes >= 0 && a.num_axes <= BPD_MAX_AXES, "positions of 1 to %d axes (got %d)", BPD_MAX_AXES, a.num_axes);
+  BPD_REQUIRE(a.num_axes == 0 || a.rotary > 0, "positions need the rotation's tables");
+  BPD_REQUIRE(a.num_axes == 0 || a.places || a.rows * a.tokens == 0, "null positions");
   BPD_REQUIRE((reinterpret_cast<uintptr_t>(a.q_out) & 15u) == 0, "the output must lie at a multiple of 16 bytes");
   BPD_REQUIRE(a.heads >= 0 && (a.heads == 0 || (a.q && a.q_out) || a.rows * a.tokens == 0), "null query pointer");
   BPD_REQUIRE(a.rows * int64_t(a.tokens) == 0 || (a.k && a.v && a.table.block_table && a.starts),
@@ -356,7 +431,10 @@ int launch_append(const AppendArgs& a, hipStream_t s) {
   const int64_t parts = B::blocks(total, many ? kKvPasses : 1);
   BPD_REQUIRE(n * parts < (int64_t(1) << 31), "too many tokens in one call");
   const auto launch = [&](auto passes, auto mode) {
-    kv_append_kernel<DT, D, passes(), mode()><<<uint32_t(n * parts), kKvThreads, 0, s>>>(a, uint32_t(parts));
+    if (a.num_axes > 0)
+      kv_append_kernel<DT, D, passes(), mode(), true><<<uint32_t(n * parts), kKvThreads, 0, s>>>(a, uint32_t(parts));
+    else
+      kv_append_kernel<DT, D, passes(), mode(), false><<<uint32_t(n * parts), kKvThreads, 0, s>>>(a, uint32_t(parts));
   };
   const std::integral_constant<int, 1> one;
   const std::integral_constant<int, kKvPasses> more;
@@ -411,8 +489,13 @@ using namespace bpd;
     pages, KvPage{page_size, head_dim}, KvTable{block_table, table_ld, table_blocks, num_pages}, kv_heads, heads,  \
         static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), static_cast<const uint16_t*>(q),         \
         {k_row, k_token, k_head}, {v_row, v_token, v_head}, {q_row, q_token, q_head},                              \
-        static_cast<uint16_t*>(q_out), rows, tokens, starts, counts, cos, sin, positions, rotary, interleaved, err \
+        static_cast<uint16_t*>(q_out), rows, tokens, starts, counts, cos, sin, positions, rotary, interleaved, err, \
+        nullptr, 0, 0, 0, 0, nullptr                                                                               \
   }
+#define BPD_APPEND_AXES                                                                                           \
+  a.places = places, a.place_axis = place_axis, a.place_row = place_row, a.place_token = place_token,             \
+  a.num_axes = num_axes, a.axes = axes;                                                                           \
+  BPD_REQUIRE(num_axes >= 1, "positions of 1 to %d axes (got %d)", BPD_MAX_AXES, num_axes)
 
 extern "C" int bpd_kv_append(uint8_t* pages, int64_t num_pages, int32_t page_size, int32_t kv_heads, int32_t head_dim,
                              int dtype, const void* k, int64_t k_row, int64_t k_token, int64_t k_head, const void* v,
@@ -436,6 +519,43 @@ extern "C" int bpd_host_kv_append(uint8_t* pages, int64_t num_pages, int32_t pag
                                   const int32_t* counts, const float* cos, const float* sin, int64_t positions,
                                   int32_t rotary, int interleaved, int32_t* err) {
   BPD_APPEND_ARGS;
+  if (int rc = check_append(a, dtype)) return rc;
+  if (rows == 0 || tokens == 0) return BPD_OK;
+  if (dtype == BPD_DTYPE_BF16)
+    host_append<BPD_DTYPE_BF16>(a);
+  else
+    host_append<BPD_DTYPE_F16>(a);
+  return BPD_OK;
+}
+
+extern "C" int bpd_kv_append_axes(uint8_t* pages, int64_t num_pages, int32_t page_size, int32_t kv_heads, int32_t head_dim,
+                             int dtype, const void* k, int64_t k_row, int64_t k_token, int64_t k_head, const void* v,
+                             int64_t v_row, int64_t v_token, int64_t v_head, const void* q, int64_t q_row,
+                             int64_t q_token, int64_t q_head, int32_t heads, void* q_out, int64_t rows,
+                             int32_t tokens, const int32_t* block_table, int64_t table_ld, int32_t table_blocks,
+                             const int32_t* starts, const int32_t* counts, const float* cos, const float* sin,
+                             int64_t positions, int32_t rotary, int interleaved, const int32_t* places,
+                                  int64_t place_axis, int64_t place_row, int64_t place_token, int32_t num_axes,
+                                  const int32_t* axes, int32_t* err, void* stream) {
+  BPD_APPEND_ARGS;
+  BPD_APPEND_AXES;
+  if (int rc = check_append(a, dtype)) return rc;
+  if (rows == 0 || tokens == 0) return BPD_OK;
+  return with_kv(dtype, head_dim, [&](auto dt, auto dim) { return launch_append<dt(), dim()>(a, as_stream(stream)); });
+}
+
+extern "C" int bpd_host_kv_append_axes(uint8_t* pages, int64_t num_pages, int32_t page_size, int32_t kv_heads,
+                                  int32_t head_dim, int dtype, const void* k, int64_t k_row, int64_t k_token,
+                                  int64_t k_head, const void* v, int64_t v_row, int64_t v_token, int64_t v_head,
+                                  const void* q, int64_t q_row, int64_t q_token, int64_t q_head, int32_t heads,
+                                  void* q_out, int64_t rows, int32_t tokens, const int32_t* block_table,
+                                  int64_t table_ld, int32_t table_blocks, const int32_t* starts,
+                                  const int32_t* counts, const float* cos, const float* sin, int64_t positions,
+                                  int32_t rotary, int interleaved, const int32_t* places, int64_t place_axis,
+                                       int64_t place_row, int64_t place_token, int32_t num_axes, const int32_t* axes,
+                                       int32_t* err) {
+  BPD_APPEND_ARGS;
+  BPD_APPEND_AXES;
   if (int rc = check_append(a, dtype)) return rc;
   if (rows == 0 || tokens == 0) return BPD_OK;
   if (dtype == BPD_DTYPE_BF16)

@@ -140,19 +140,22 @@ __host__ __device__ __forceinline__ float rot_second(float a, float b, float c, 
   return x + y;
 }
 
-// Channel d of a head of `x`, rotated: pairs (d, d + rot / 2), or neighbours.
-template <int DT>
-__host__ __device__ __forceinline__ float rotated_channel(const uint16_t* x, int32_t d, int32_t rot,
-                                                          bool interleaved, const float* cos, const float* sin) {
+// Channel d of a head of `x`, rotated: pairs (d, d + rot / 2), or neighbours;
+// angle(pair, &c, &s) gives a pair's cosine and sine.
+template <int DT, class F>
+__host__ __device__ __forceinline__ float rotated_channel(const uint16_t* x, int32_t d, int32_t rot, bool interleaved,
+                                                          F angle) {
   const float v = elem16_float<DT>(x[d]);
   if (d >= rot) return v;
-  const int32_t h = rot / 2;
+  const int32_t h = rot / 2, pair = interleaved ? d >> 1 : d < h ? d : d - h;
+  float c, s;
+  angle(pair, &c, &s);
   if (interleaved) {
     const float w = elem16_float<DT>(x[d ^ 1]);
-    return (d & 1) ? rot_second(w, v, cos[d >> 1], sin[d >> 1]) : rot_first(v, w, cos[d >> 1], sin[d >> 1]);
+    return (d & 1) ? rot_second(w, v, c, s) : rot_first(v, w, c, s);
   }
-  if (d < h) return rot_first(v, elem16_float<DT>(x[d + h]), cos[d], sin[d]);
-  return rot_second(elem16_float<DT>(x[d - h]), v, cos[d - h], sin[d - h]);
+  if (d < h) return rot_first(v, elem16_float<DT>(x[d + h]), c, s);
+  return rot_second(elem16_float<DT>(x[d - h]), v, c, s);
 }
 
 // Where token `pos` of a request lies: the index of its page's block of head

@@ -113,7 +113,8 @@ class PagedKV4:
     # --- operators -----------------------------------------------------------
     def append(self, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, starts: torch.Tensor, *,
                counts: torch.Tensor | None = None, cos: torch.Tensor | None = None, sin: torch.Tensor | None = None,
-               interleaved: bool = False, q: torch.Tensor | None = None) -> torch.Tensor | None:
+               interleaved: bool = False, q: torch.Tensor | None = None, positions: torch.Tensor | None = None,
+               axes: torch.Tensor | None = None) -> torch.Tensor | None:
         """Append ``k`` and ``v`` [requests, tokens, kv_heads, head_dim]: token
         i < ``counts[b]`` (all without ``counts``) of request b at position
         ``starts[b] + i``, over whatever was there.  With ``cos`` and ``sin``
@@ -122,7 +123,14 @@ class PagedKV4:
         that position first, in float32: channel pairs (j, j + R / 2), or
         (2j, 2j + 1) with ``interleaved``.  Returns the rotated ``q`` (zeros
         past ``counts[b]``), None without ``q``.  Two requests must not append
-        to one page in one call."""
+        to one page in one call.
+
+        With ``positions`` (int32 [axes, requests, tokens], up to 4 axes, or
+        [requests, tokens]) the rotation goes by them, not by the place in the
+        cache: pair j by the position on axis ``axes[j]`` (int32 [R / 2]; all
+        on the first without it), as models place the patches of images and
+        video by time, height and width.  A token with a position outside the
+        rotation's tables is left out."""
         k, ks = self._block(k, "k", self.kv_heads)
         v, vs = self._block(v, "v", self.kv_heads)
         B, T, _, _ = k.shape
@@ -130,7 +138,7 @@ class PagedKV4:
             raise RuntimeError(f"k and v differ in shape: {list(k.shape)} and {list(v.shape)}")
         block_table, table = self._table(block_table, B)
         starts, counts = self._per_request(starts, "starts", B), self._per_request(counts, "counts", B)
-        rotary = positions = 0
+        rotary = rows = 0
         if (cos is None) != (sin is None):
             raise RuntimeError("the rotation needs both cos and sin")
         if cos is not None:
@@ -138,23 +146,43 @@ class PagedKV4:
                     or sin.dtype is not torch.float32 or cos.device != self.device or sin.device != self.device:
                 raise RuntimeError(f"cos and sin must be float32 [positions, R / 2] on {self.device}")
             cos, sin = cos.contiguous(), sin.contiguous()
-            positions, rotary = cos.shape
+            rows, rotary = cos.shape
             rotary *= 2
             if rotary > self.head_dim:
                 raise RuntimeError(f"{rotary} rotated channels in heads of {self.head_dim}")
+        on_axes = ()
+        if positions is not None:
+            if cos is None:
+                raise RuntimeError("positions need the rotation's cos and sin")
+            if positions.dim() == 2:
+                positions = positions[None]
+            if positions.dim() != 3 or positions.shape[1:] != (B, T) or not 1 <= positions.shape[0] <= _lib.MAX_AXES \
+                    or positions.dtype is not torch.int32 or positions.device != self.device:
+                raise RuntimeError(f"positions must be int32 [1 to {_lib.MAX_AXES} axes, {B}, {T}] on {self.device}")
+            if axes is not None:
+                if axes.dtype is not torch.int32 or axes.shape != cos.shape[1:] or axes.device != self.device:
+                    raise RuntimeError(f"axes must be int32 [{cos.shape[1]}] on {self.device}")
+                axes = axes.contiguous()
+            elif positions.shape[0] > 1:
+                raise RuntimeError("positions on several axes need the axis of each channel pair")
+            on_axes = (positions.data_ptr(), *positions.stride(), positions.shape[0], ptr(axes)) if cos.shape[1] else ()
+        elif axes is not None:
+            raise RuntimeError("axes need positions")
         out, heads, qs = None, 0, (None, 0, 0, 0)
         if q is not None:
             q, qs = self._block(q, "q")
-            rows, tokens, heads, _ = q.shape
-            if rows != B or tokens != T:
+            if q.shape[:2] != k.shape[:2]:
                 raise RuntimeError(f"q and k differ in requests or tokens: {list(q.shape)} and {list(k.shape)}")
+            heads = q.shape[2]
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         args = (*self._head, *ks, *vs, *qs, heads, ptr(out), B, T, *table, ptr(starts), ptr(counts), ptr(cos), ptr(sin),
-                positions, rotary, int(interleaved), ptr(self.err))
+                rows, rotary, int(interleaved), *on_axes, ptr(self.err))
         if self._on_dev:
-            check(lib().bpd_kv_append(*args, _lib.stream_of(self.device)))
+            append = lib().bpd_kv_append_axes if on_axes else lib().bpd_kv_append
+            check(append(*args, _lib.stream_of(self.device)))
         else:
-            check(lib().bpd_host_kv_append(*args))
+            append = lib().bpd_host_kv_append_axes if on_axes else lib().bpd_host_kv_append
+            check(append(*args))
         return out
 
     def read(self, block_table: torch.Tensor, starts: torch.Tensor, tokens: int, *,

@@ -777,10 +777,20 @@ int bpd_host_truncate(const void* logits, int dtype, int64_t rows, int64_t vocab
  * by cos/sin float [positions, rotary / 2] at the token's position.  q_out
  * [rows, tokens, heads, head_dim] contiguous, zeros for tokens past counts[b].
  * Two requests must not append to one page.
+ * bpd_kv_append_axes: the same, with positions for the rotation apart from the
+ * place in the cache: token i of request b stands at places[x * place_axis +
+ * b * place_row + i * place_token] (int32, strides in elements) on axis x <
+ * num_axes (1 to BPD_MAX_AXES: time, height and width of an image's or
+ * video's patches, say), and channel pair j turns by the position on axis
+ * axes[j] (int32 [rotary / 2]; NULL: all on the first).  A token with a
+ * position outside [0, positions) on any axis is left out as one with a place
+ * outside its tables is; an axis outside its range is read as the nearest; both
+ * set BPD_FLAG_PAGE_RANGE.
  * bpd_kv_read: tokens starts[b] + i, i < counts[b], back as k_out and v_out
  * [rows, tokens, kv_heads, head_dim] contiguous; zeros past counts[b] and for
  * tokens outside the tables.  q_out, k_out and v_out lie at multiples of 16
  * bytes; k, v and q at any element. */
+#define BPD_MAX_AXES 4
 int bpd_kv_append(uint8_t* pages, int64_t num_pages, int32_t page_size, int32_t kv_heads,
                   int32_t head_dim, int dtype, const void* k, int64_t k_row, int64_t k_token,
                   int64_t k_head, const void* v, int64_t v_row, int64_t v_token, int64_t v_head,
@@ -798,6 +808,27 @@ int bpd_host_kv_append(uint8_t* pages, int64_t num_pages, int32_t page_size, int
                        const int32_t* starts, const int32_t* counts, const float* cos,
                        const float* sin, int64_t positions, int32_t rotary, int interleaved,
                        int32_t* err);
+int bpd_kv_append_axes(uint8_t* pages, int64_t num_pages, int32_t page_size, int32_t kv_heads,
+                  int32_t head_dim, int dtype, const void* k, int64_t k_row, int64_t k_token,
+                  int64_t k_head, const void* v, int64_t v_row, int64_t v_token, int64_t v_head,
+                  const void* q, int64_t q_row, int64_t q_token, int64_t q_head, int32_t heads,
+                  void* q_out, int64_t rows, int32_t tokens, const int32_t* block_table,
+                  int64_t table_ld, int32_t table_blocks, const int32_t* starts,
+                  const int32_t* counts, const float* cos, const float* sin, int64_t positions,
+                  int32_t rotary, int interleaved, const int32_t* places, int64_t place_axis,
+                       int64_t place_row, int64_t place_token, int32_t num_axes,
+                       const int32_t* axes, int32_t* err, void* stream);
+int bpd_host_kv_append_axes(uint8_t* pages, int64_t num_pages, int32_t page_size, int32_t kv_heads,
+                       int32_t head_dim, int dtype, const void* k, int64_t k_row, int64_t k_token,
+                       int64_t k_head, const void* v, int64_t v_row, int64_t v_token,
+                       int64_t v_head, const void* q, int64_t q_row, int64_t q_token,
+                       int64_t q_head, int32_t heads, void* q_out, int64_t rows, int32_t tokens,
+                       const int32_t* block_table, int64_t table_ld, int32_t table_blocks,
+                       const int32_t* starts, const int32_t* counts, const float* cos,
+                       const float* sin, int64_t positions, int32_t rotary, int interleaved,
+                            const int32_t* places, int64_t place_axis, int64_t place_row,
+                            int64_t place_token, int32_t num_axes, const int32_t* axes,
+                            int32_t* err);
 int bpd_kv_read(const uint8_t* pages, int64_t num_pages, int32_t page_size, int32_t kv_heads,
                 int32_t head_dim, int dtype, void* k_out, void* v_out, int64_t rows,
                 int32_t tokens, const int32_t* block_table, int64_t table_ld,
