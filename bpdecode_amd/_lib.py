@@ -178,6 +178,11 @@ _SIGNATURES = {
                              vp, vp, f32, vp, sz, vp, vp]),
     "bpd_host_kv_attend": (cint, [vp, i64, i32, i32, i32, cint, vp, i64, i64, i64, i32, vp, i64, i32, vp, i64,
                                   i32, vp, vp, f32, vp]),
+    "bpd_kv_attend_shared_workspace_bytes": (sz, [i64, i32, i32, i32, i32, i64, i64]),
+    "bpd_kv_attend_shared": (cint, [vp, i64, i32, i32, i32, cint, vp, i64, i64, i64, i32, vp, i64, i32, vp, i32, vp, i32, vp,
+                                    i64, i32, vp, vp, f32, vp, sz, vp, vp]),
+    "bpd_host_kv_attend_shared": (cint, [vp, i64, i32, i32, i32, cint, vp, i64, i64, i64, i32, vp, i64, i32, vp, i32, vp,
+                                         i32, vp, i64, i32, vp, vp, f32, vp]),
 }
 
 _lib = None

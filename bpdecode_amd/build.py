@@ -20,7 +20,7 @@ CSRC = PKG / "csrc"
 OBJ = CSRC / "_build"
 LIB = PKG / "libbpdecode_hip.so"
 SOURCES = ["dense.hip", "fsa.hip", "pda.hip", "soft.hip", "stage.hip", "frames.hip", "verify.hip", "sample.hip", "kv.hip",
-           "attend.hip", "host.cpp"]
+           "attend.hip", "shared.hip", "host.cpp"]
 ARCH = os.environ.get("BPDECODE_OFFLOAD_ARCH", "gfx950")
 
 FLAGS = [
@@ -57,7 +57,7 @@ def _compile(src: str) -> Path:
 def build_library(verbose: bool = False) -> Path:
     OBJ.mkdir(exist_ok=True)
     present = [s for s in SOURCES if (CSRC / s).exists()]
-    with ThreadPoolExecutor(max_workers=min(4, len(present))) as ex:
+    with ThreadPoolExecutor(max_workers=min(6, len(present))) as ex:
         objs = list(ex.map(_compile, present))
     tmp = LIB.with_suffix(".so.tmp")
     cmd = [_hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)]

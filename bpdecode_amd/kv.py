@@ -228,6 +228,46 @@ class PagedKV4:
             check(lib().bpd_host_kv_attend(*args, ptr(self.err)))
         return out
 
+    def attend_shared(self, q: torch.Tensor, prefix_table: torch.Tensor, shared: int | torch.Tensor,
+                      block_table: torch.Tensor, lengths: torch.Tensor, *, query_lens: torch.Tensor | None = None,
+                      scale: float | None = None) -> torch.Tensor:
+        """:meth:`attend` for a batch whose requests begin with the same
+        ``shared`` tokens (a number, or int32 [1] on the device), which are
+        attended to once for all of them.  Those, cut to whole pages, lie in the
+        pages of ``prefix_table`` int32 [blocks]; ``block_table`` and ``lengths``
+        are those of the whole requests, as :meth:`append` and :meth:`attend`
+        take them (a table's entries before the shared pages' end are not
+        read).  The result is :meth:`attend`'s with the shared pages first in
+        every request's table."""
+        q, qs = self._block(q, "q")
+        B, T, H, D = q.shape
+        if H < 1 or H % self.kv_heads:
+            raise RuntimeError(f"query heads ({H}) must be a multiple of the cache's heads ({self.kv_heads})")
+        block_table, table = self._table(block_table, B)
+        lengths, query_lens = self._per_request(lengths, "lengths", B), self._per_request(query_lens, "query_lens", B)
+        if prefix_table.dim() != 1 or prefix_table.dtype is not torch.int32 or prefix_table.device != self.device:
+            raise RuntimeError(f"prefix_table must be int32 [blocks] on {self.device}")
+        prefix_table = prefix_table.contiguous()
+        blocks, count = prefix_table.shape[0], 0
+        if isinstance(shared, torch.Tensor):
+            if shared.dtype is not torch.int32 or shared.numel() != 1 or shared.device != self.device:
+                raise RuntimeError(f"shared must be a number or int32 [1] on {self.device}")
+        else:
+            shared, count = None, shared
+            if not 0 <= count <= blocks * self.page_size:
+                raise RuntimeError(f"{count} shared tokens in a prefix of {blocks} pages of {self.page_size}")
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        args = (*self._head, *qs, H, out.data_ptr(), B, T, ptr(prefix_table), blocks, ptr(shared), count, *table,
+                ptr(lengths), ptr(query_lens), D ** -0.5 if scale is None else float(scale))
+        if self._on_dev:
+            need = lib().bpd_kv_attend_shared_workspace_bytes(B, T, H, self.kv_heads, D, table[2] * self.page_size,
+                                                              blocks * self.page_size)
+            ws = self.pages.new_empty(need)
+            check(lib().bpd_kv_attend_shared(*args, ptr(ws), need, ptr(self.err), _lib.stream_of(self.device)))
+        else:
+            check(lib().bpd_host_kv_attend_shared(*args, ptr(self.err)))
+        return out
+
     def check_errors(self) -> None:
         """Raise if a call met a position or page outside its tables since the
         last check (synchronises with the device)."""

@@ -866,6 +866,40 @@ int bpd_host_kv_attend(const uint8_t* pages, int64_t num_pages, int32_t page_siz
                        int32_t table_blocks, const int32_t* lengths, const int32_t* query_lens,
                        float scale, int32_t* err);
 
+/* bpd_kv_attend_shared: bpd_kv_attend for a batch whose requests begin with the
+ * same tokens, which are attended to once for all of them.  The first `shared`
+ * tokens (*shared, int32 on the device, or with NULL shared_all), cut to whole
+ * pages, lie in the pages of prefix_table (int32 [prefix_blocks]) for every
+ * request; its block table names the pages behind them, at their places in
+ * the whole request (entries before those are not read).  Lengths count the
+ * shared tokens, and a query sees what it would in bpd_kv_attend over the whole
+ * request, also where a request is shorter than the prefix.  More shared
+ * tokens than prefix_table has room for count as many as it has
+ * (BPD_FLAG_PAGE_RANGE; shared_all is refused).  Sums of the prefix and of the
+ * rest are kept apart in float and joined in float.  workspace:
+ * bpd_kv_attend_shared_workspace_bytes bytes for `longest` = table_blocks *
+ * page_size and `prefix` = prefix_blocks * page_size, 16-byte aligned. */
+size_t bpd_kv_attend_shared_workspace_bytes(int64_t rows, int32_t tokens, int32_t heads,
+                                            int32_t kv_heads, int32_t head_dim, int64_t longest,
+                                            int64_t prefix);
+int bpd_kv_attend_shared(const uint8_t* pages, int64_t num_pages, int32_t page_size,
+                         int32_t kv_heads, int32_t head_dim, int dtype, const void* q,
+                         int64_t q_row, int64_t q_token, int64_t q_head, int32_t heads, void* out,
+                         int64_t rows, int32_t tokens, const int32_t* prefix_table,
+                         int32_t prefix_blocks, const int32_t* shared, int32_t shared_all,
+                         const int32_t* block_table, int64_t table_ld, int32_t table_blocks,
+                         const int32_t* lengths, const int32_t* query_lens, float scale,
+                         void* workspace, size_t workspace_bytes, int32_t* err, void* stream);
+int bpd_host_kv_attend_shared(const uint8_t* pages, int64_t num_pages, int32_t page_size,
+                              int32_t kv_heads, int32_t head_dim, int dtype, const void* q,
+                              int64_t q_row, int64_t q_token, int64_t q_head, int32_t heads,
+                              void* out, int64_t rows, int32_t tokens,
+                              const int32_t* prefix_table, int32_t prefix_blocks,
+                              const int32_t* shared, int32_t shared_all,
+                              const int32_t* block_table, int64_t table_ld, int32_t table_blocks,
+                              const int32_t* lengths, const int32_t* query_lens, float scale,
+                              int32_t* err);
+
 #ifdef __cplusplus
 }
 #endif
