@@ -88,10 +88,7 @@ __host__ __device__ __forceinline__ void store_drawn(const SampleArgs& a, int64_
 // where a row's 10^5 borders want 10^-12 of its sum.
 typedef unsigned long long u64;
 
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / kWave;
-constexpr int kStep = kThreads * kRun;  // tokens that a block reads at a time
-constexpr int kBins = 4 * kThreads;
+constexpr int kBins = 4096;
 constexpr int kMostScale = 50;  // a weight is read off the bits of its sum with 2^52
 
 // Bits of a weight: the sum of a row's fits 63.
@@ -146,23 +143,27 @@ struct Table {
   u64 sums[kBins];
   uint32_t counts[kBins];
 };
+template <int N>  // threads
 struct Scratch {
+  static constexpr int waves = N / kWave, step = N * kRun;  // tokens that a block reads at a time
   Table first, sub;  // by weight, and of a part of one bin of it by key
-  u64 sums[kWaves], counts[kWaves];
+  u64 sums[waves], counts[waves];
   u64 hit_count, hit_sum;
   int64_t found;
-  float tops[kWaves];
-  int32_t bad[kWaves], hit_bin;
+  float tops[waves];
+  int32_t bad[waves], hit_bin;
 };
 
+template <int N>
 __device__ __forceinline__ void clear(Table& t) {
-  for (int i = threadIdx.x; i < kBins; i += kThreads) t.sums[i] = 0, t.counts[i] = 0;
+  for (int i = threadIdx.x; i < kBins; i += N) t.sums[i] = 0, t.counts[i] = 0;
 }
 
 // The bin in which the running count or sum passes `target` (less than the
 // whole); *count and *sum become what lies before it.
-__device__ __forceinline__ int32_t find_bin(const Table& t, u64 target, bool by_count, u64* count, u64* sum, Scratch& s) {
-  constexpr int kMine = kBins / kThreads;
+template <int N>
+__device__ __forceinline__ int32_t find_bin(const Table& t, u64 target, bool by_count, u64* count, u64* sum, Scratch<N>& s) {
+  constexpr int kMine = kBins / N;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   u64 c = 0, x = 0;
 #pragma unroll
@@ -210,8 +211,9 @@ __device__ __forceinline__ void each_run(const Row& r, int64_t first, int64_t en
 }
 
 // The token of rank `rank` (from 1) among those with this key, by index.
-template <int DT>
-__device__ int64_t nth_token(const Row& r, uint32_t key, u64 rank, Scratch& s) {
+template <int DT, int N>
+__device__ int64_t nth_token(const Row& r, uint32_t key, u64 rank, Scratch<N>& s) {
+  constexpr int kWaves = N / kWave, kStep = N * kRun;
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   // a wave takes neighbouring tokens
   const int64_t part = (r.vocab + kStep - 1) / kStep * (kWave * kRun);
@@ -268,9 +270,10 @@ __device__ __forceinline__ u64 share_of(u64 x, float f, bool ceil_less_one) {
   return hi << (64 - down) | lo >> down;
 }
 
-template <int DT>
-__device__ void sample_row(const SampleArgs& a, const Row& r, const Asked& want, int64_t b, bool draw, Scratch& s,
+template <int DT, int N>
+__device__ void sample_row(const SampleArgs& a, const Row& r, const Asked& want, int64_t b, bool draw, Scratch<N>& s,
                            Cut* cut_out, int64_t* last_out, float* logprob, bool* bad_out) {
+  constexpr int kWaves = N / kWave, kStep = N * kRun;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   float top = -INFINITY;
   bool bad = false;
@@ -300,7 +303,7 @@ __device__ void sample_row(const SampleArgs& a, const Row& r, const Asked& want,
   if (!draw && whole) {
     cut.key = cut.rank = 0;
   } else if (want.temp > 0.0) {
-    clear(s.first);
+    clear<N>(s.first);
     __syncthreads();
     each_run<DT>(r, tid * kRun, r.vocab, kStep, [&](const float(&z)[kRun], uint32_t valid, int64_t) {
 #pragma unroll
@@ -317,7 +320,7 @@ __device__ void sample_row(const SampleArgs& a, const Row& r, const Asked& want,
     u64 count = 0, sum = 0;
     {
       u64 c = 0, x = 0;
-      for (int i = tid; i < kBins; i += kThreads) c += s.first.counts[i], x += s.first.sums[i];
+      for (int i = tid; i < kBins; i += N) c += s.first.counts[i], x += s.first.sums[i];
       c = wave_sum(c), x = wave_sum(x);
       if (lane == 0) s.counts[wave] = c, s.sums[wave] = x;
       __syncthreads();
@@ -339,7 +342,7 @@ __device__ void sample_row(const SampleArgs& a, const Row& r, const Asked& want,
       for (;;) {
         const uint32_t range = hi - lo;
         const int shift = range < uint32_t(kBins) ? 0 : 32 - __builtin_clz(range) - __builtin_ctz(uint32_t(kBins));
-        clear(s.sub);
+        clear<N>(s.sub);
         __syncthreads();
         each_run<DT>(r, tid * kRun, r.vocab, kStep, [&](const float(&z)[kRun], uint32_t valid, int64_t) {
 #pragma unroll
@@ -402,7 +405,7 @@ __device__ void sample_row(const SampleArgs& a, const Row& r, const Asked& want,
     *logprob = 0.0f;
   }
   *cut_out = cut;
-  if (cut.rank > 0) *last_out = nth_token<DT>(r, cut.key, cut.rank, s);
+  if (cut.rank > 0) *last_out = nth_token<DT, N>(r, cut.key, cut.rank, s);
 }
 
 __device__ __forceinline__ Row row_of(const SampleArgs& a, int64_t b, int32_t* state, int32_t* flags) {
@@ -414,9 +417,11 @@ __device__ __forceinline__ Row row_of(const SampleArgs& a, int64_t b, int32_t* s
              some ? a.vocab : 0};
 }
 
+constexpr int kThreads = 1024;
 template <int DT, bool Draw>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
-  __shared__ Scratch s;
+  constexpr int kStep = kThreads * kRun;
+  __shared__ Scratch<kThreads> s;
   const int64_t b = blockIdx.x;
   int32_t state, flags;
   const Row r = row_of(a, b, &state, &flags);
@@ -424,7 +429,7 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   int64_t last = -1;
   float logprob = -INFINITY;
   bool bad = false;
-  sample_row<DT>(a, r, asked_of(a, b), b, Draw, s, &cut, &last, &logprob, &bad);
+  sample_row<DT, kThreads>(a, r, asked_of(a, b), b, Draw, s, &cut, &last, &logprob, &bad);
   if (bad) flags |= BPD_FLAG_LOGITS;
   if (flags && a.err && threadIdx.x == 0) atomicOr(a.err, flags);
   if constexpr (Draw) {
@@ -455,9 +460,421 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   for (int64_t t = a.vocab + threadIdx.x; t < a.cols; t += kThreads) put(t, none);
 }
 
+// ---------------------------------------------- rows of 16-bit logits --
+// A 16-bit type has few values, and a weight follows from the value: a row is
+// counted by value, once, and all sums are those of counts times weights.  The
+// counts lie in LDS, a word to a magnitude, positive ones in its lower half;
+// the row stays in registers, where its equal tokens are told apart by index
+// and the kept ones written.  Values stand at positions in falling order.
+constexpr int kMagnitudes = 32768;
+// Half the threads that a CU holds, with twice the registers: 40 runs are the
+// row of a vocabulary of 163,840.
+constexpr int kThreads16 = 512, kWaves16 = kThreads16 / kWave, kStep16 = kThreads16 * kRun, kHeld = 40;
+constexpr int kChunk = 4 * kWave;               // words of counts that a wave takes at a time
+constexpr int kChunks = 2 * kMagnitudes / kChunk;
+
+template <int DT>
+struct Half {
+  static constexpr uint32_t inf = DT == BPD_DTYPE_BF16 ? 0x7F80u : 0x7C00u;
+};
+template <int DT>
+__device__ __forceinline__ float value_of(uint32_t magnitude) {
+  if (DT == BPD_DTYPE_BF16) return __builtin_bit_cast(float, magnitude << 16);
+  return float(__builtin_bit_cast(_Float16, uint16_t(magnitude)));
+}
+template <int DT>
+__device__ __forceinline__ float value_at(int32_t position) {
+  return position < kMagnitudes ? value_of<DT>(uint32_t(kMagnitudes - 1 - position))
+                                : -value_of<DT>(uint32_t(position - kMagnitudes));
+}
+
+struct Counted {
+  uint32_t words[kMagnitudes];
+  u64 sums[kChunks];  // by chunks of positions
+  uint32_t counts[kChunks];
+  uint32_t added[kWaves16], found[kWaves16];
+  int32_t most[kWaves16], least_below[kWaves16], most_below[kWaves16];  // magnitudes: positive, negative
+  // what the first wave comes to
+  int32_t position;
+  uint32_t rank;  // 0: all of the position
+  float logprob;
+  int64_t last;
+};
+
+// A first part of the order, as Cut, by position.
+struct Place16 {
+  int32_t position;
+  uint32_t rank;
+  u64 sum;
+};
+
+// Counts of a position's magnitude; zeros of both signs stand at the first.
+__device__ __forceinline__ uint32_t count_at(const uint32_t* words, int32_t position) {
+  const bool below = position >= kMagnitudes;
+  const int32_t m = below ? position - kMagnitudes : kMagnitudes - 1 - position;
+  const uint32_t w = words[m];
+  if (m == 0) return below ? 0 : (w & 0xFFFFu) + (w >> 16);
+  return below ? w >> 16 : w & 0xFFFFu;
+}
+
+// The first wave's view of the chunks: each lane has four of them.
+template <int DT>
+struct Chunks {
+  const Counted& s;
+  const Measure& m;
+  int lane;
+  u64 sum_before, sum_mine;
+  uint32_t count_before, count_mine;
+  __device__ __forceinline__ Chunks(const Counted& s_, const Measure& m_, int lane_) : s(s_), m(m_), lane(lane_) {
+    sum_mine = 0, count_mine = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sum_mine += s.sums[4 * lane + k], count_mine += s.counts[4 * lane + k];
+    sum_before = wave_scan_sum(sum_mine) - sum_mine;
+    count_before = wave_scan_sum(count_mine) - count_mine;
+  }
+  __device__ __forceinline__ u64 sum() const { return of_lane(sum_before + sum_mine, kWave - 1); }
+  __device__ __forceinline__ uint32_t count() const { return of_lane(count_before + count_mine, kWave - 1); }
+  // what stands before chunk `c`
+  __device__ __forceinline__ void before(int c, uint32_t* count, u64* sum) const {
+    *count = of_lane(count_before, c / 4), *sum = of_lane(sum_before, c / 4);
+    for (int k = c / 4 * 4; k < c; ++k) *count += s.counts[k], *sum += s.sums[k];
+  }
+  // the lane's four positions of chunk `c`: counts, and weights of one each
+  __device__ __forceinline__ void positions(int c, uint32_t (&n)[4], u64 (&w)[4]) const {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int32_t at = c * kChunk + 4 * lane + k;
+      n[k] = count_at(s.words, at);
+      w[k] = n[k] ? m.weight(m.y(value_at<DT>(at))) : 0;
+    }
+  }
+  // where the running count (of tokens) or sum (of weights) passes `target`
+  template <bool ByCount>
+  __device__ __forceinline__ Place16 find(u64 target) const {
+    const u64 from = ByCount ? count_before : sum_before, own = ByCount ? count_mine : sum_mine;
+    const int l = __builtin_ctzll(__ballot(from <= target && target < from + own) | u64(1) << 63);
+    int c = 4 * l;
+    uint32_t cb;
+    u64 sb;
+    before(c, &cb, &sb);
+    for (int k = 0; k < 3; ++k) {
+      const uint32_t nc = cb + s.counts[c];
+      const u64 ns = sb + s.sums[c];
+      if (target < (ByCount ? nc : ns)) break;
+      cb = nc, sb = ns, ++c;
+    }
+    uint32_t n[4];
+    u64 w[4];
+    positions(c, n, w);
+    uint32_t nc = 0;
+    u64 ns = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) nc += n[k], ns += n[k] * w[k];
+    const uint32_t upto_c = cb + wave_scan_sum(nc);
+    const u64 upto_s = sb + wave_scan_sum(ns);
+    const u64 hits = __ballot(target < (ByCount ? upto_c : upto_s));
+    const int hit = hits ? __builtin_ctzll(hits) : kWave - 1;
+    cb = of_lane(upto_c - nc, hit), sb = of_lane(upto_s - ns, hit);
+    Place16 p{c * kChunk + 4 * hit, 1, 0};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t kn = of_lane(n[k], hit);
+      const u64 kw = of_lane(w[k], hit), end_s = sb + kn * kw;
+      if (kn && target < (ByCount ? u64(cb + kn) : end_s)) {
+        p.position += k;
+        p.rank = uint32_t(ByCount ? target - cb : (target - sb) / kw) + 1;
+        p.sum = sb + p.rank * kw;
+        return p;
+      }
+      cb += kn, sb = end_s;
+    }
+    return p;
+  }
+  // the sum of all positions up to this one
+  __device__ __forceinline__ u64 sum_upto(int32_t position) const {
+    const int c = position / kChunk;
+    uint32_t cb, n[4];
+    u64 sb, w[4], x = 0;
+    before(c, &cb, &sb);
+    positions(c, n, w);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x += c * kChunk + 4 * lane + k <= position ? n[k] * w[k] : 0;
+    return sb + wave_sum(x);
+  }
+};
+
+// One block per row.
+template <int DT, bool Draw>
+__global__ __launch_bounds__(kThreads16) void sample16_kernel(SampleArgs a) {
+  __shared__ union {
+    Counted s;
+    Scratch<kThreads16> general;
+  } shared;
+  Counted& s = shared.s;
+  const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int64_t b = blockIdx.x, V = a.vocab;
+  const char* row = static_cast<const char*>(a.logits) + b * a.ld * 2;
+  const int32_t runs = int32_t((V + kStep16 - 1) / kStep16), held = runs < kHeld ? runs : kHeld;
+  // a wave takes neighbouring tokens
+  const int64_t begin = int64_t(wave) * runs * (kWave * kRun);
+  const auto run_of = [&](int32_t k) { return run_at(begin + int64_t(k) * (kWave * kRun) + lane * kRun, V); };
+  const auto inside = [&](int32_t k) { return begin + int64_t(k + 1) * (kWave * kRun) <= V; };
+  Raw<DT> raw[kHeld];
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k)
+    if (k < held) raw[k] = load_raw<DT>(row, run_of(k), V);
+  int32_t state, flags;
+  const Row r = row_of(a, b, &state, &flags);
+  const Asked want = asked_of(a, b);
+  for (int i = tid; i < kMagnitudes / 4; i += kThreads16) reinterpret_cast<uint4*>(s.words)[i] = uint4{0, 0, 0, 0};
+  constexpr uint32_t kNone = Half<DT>::inf | 0x8000u;
+  // -inf for what is not the thread's own or not allowed
+  const auto mask = [&](Raw<DT>& x, int32_t k) {
+    if (inside(k) && !r.bits && r.vocab) return;
+    const uint32_t valid = r.vocab ? run_bits(r, run_of(k)) : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (!(valid >> (2 * i) & 1)) x.w[0][i] = (x.w[0][i] & 0xFFFF0000u) | kNone;
+      if (!(valid >> (2 * i + 1) & 1)) x.w[0][i] = (x.w[0][i] & 0xFFFFu) | kNone << 16;
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k)
+    if (k < held) mask(raw[k], k);
+  __syncthreads();
+  uint32_t added = 0;
+  const auto add = [&](const Raw<DT>& x) {
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      const uint32_t h = x.w[0][j / 2] >> (16 * (j & 1)) & 0xFFFFu;
+      const bool on = h != kNone;
+      if (on) atomicAdd(&s.words[h & 0x7FFFu], h & 0x8000u ? 0x10000u : 1u);
+      added += __popcll(__ballot(on));
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k)
+    if (k < held) add(raw[k]);
+#pragma unroll 1
+  for (int32_t k = held; k < runs; ++k) {
+    Raw<DT> x = load_raw<DT>(row, run_of(k), V);
+    mask(x, k);
+    add(x);
+  }
+  if (lane == 0) s.added[wave] = added;
+  __syncthreads();
+
+  // the largest value, whether all are numbers, and whether all were counted:
+  // a count past 16 bits leaves fewer
+  int32_t most = -1, least_below = kMagnitudes, most_below = -1;
+  uint32_t counted = 0;
+#pragma unroll
+  for (int i = 0; i < kMagnitudes / 4 / kThreads16; ++i) {
+    const int32_t at = (i * kThreads16 + tid) * 4;
+    const uint4 q = *reinterpret_cast<const uint4*>(s.words + at);
+    if ((q.x | q.y | q.z | q.w) == 0) continue;
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (w[k] & 0xFFFFu) most = max(most, at + k);
+      if (w[k] >> 16) least_below = min(least_below, at + k), most_below = max(most_below, at + k);
+      counted += (w[k] & 0xFFFFu) + (w[k] >> 16);
+    }
+  }
+  most = -wave_min(-most), least_below = wave_min(least_below), most_below = -wave_min(-most_below);
+  counted = wave_sum(counted);
+  if (lane == 0) s.most[wave] = most, s.least_below[wave] = least_below, s.most_below[wave] = most_below, s.found[wave] = counted;
+  __syncthreads();
+  uint32_t all = 0;
+  counted = 0;
+  for (int k = 0; k < kWaves16; ++k) {
+    most = max(most, s.most[k]), least_below = min(least_below, s.least_below[k]), most_below = max(most_below, s.most_below[k]);
+    all += s.added[k], counted += s.found[k];
+  }
+  const bool bad = most >= int32_t(Half<DT>::inf) || most_below > int32_t(Half<DT>::inf);
+  const bool none = bad || (most < 0 && least_below == kMagnitudes);
+  if (bad) flags |= BPD_FLAG_LOGITS;
+  int64_t last = -1;
+  float border = INFINITY, logprob = -INFINITY;  // what lies above it is kept, and of what equals it all up to `last`
+  if (!none && counted != all) {
+    __syncthreads();
+    Cut cut{0xFFFFFFFFu, 0, 0};
+    bool is_bad;
+    sample_row<DT, kThreads16>(a, r, want, b, Draw, shared.general, &cut, &last, &logprob, &is_bad);
+    if (is_bad) flags |= BPD_FLAG_LOGITS;
+    if (cut.rank) border = logit_of(cut.key);
+    else if (cut.key == 0) border = -INFINITY;
+    else if (cut.key != 0xFFFFFFFFu) border = logit_of(cut.key + 1), last = INT64_MAX;
+  } else if (!none) {
+    const float top = most >= 0 ? value_of<DT>(uint32_t(most)) : -value_of<DT>(uint32_t(least_below));
+    const int32_t first = most >= 0 ? kMagnitudes - 1 - most : kMagnitudes + (least_below == 0 ? -1 : least_below);
+    Measure m{double(top), want.temp > 0.0 ? kLog2E / want.temp : 0.0, 0.0, scale_of(V)};
+    const bool whole = want.temp > 0.0 && want.top_k == 0 && want.top_p >= 1.0f && want.min_p <= 0.0;
+    if (want.temp > 0.0 && (Draw || !whole)) {
+      // counts and sums of the chunks
+#pragma unroll 1
+      for (int i = 0; i < kChunks / 2 / kWaves16; ++i) {
+        const int32_t c = i * kWaves16 + wave;
+        const uint4 q = reinterpret_cast<const uint4*>(s.words)[c * kWave + lane];
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+        const bool any = __any((q.x | q.y | q.z | q.w) != 0);
+        uint32_t n[2] = {0, 0};
+        u64 x[2] = {0, 0};
+        if (any) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int32_t at = c * kChunk + 4 * lane + k;
+            uint32_t here[2] = {w[k] & 0xFFFFu, w[k] >> 16};
+            if (at == 0) here[0] += here[1], here[1] = 0;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              n[e] += here[e];
+              if (__any(here[e] != 0)) x[e] += here[e] * m.weight(m.y(e ? -value_of<DT>(at) : value_of<DT>(at)));
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) n[e] = wave_sum(n[e]), x[e] = wave_sum(x[e]);
+        }
+        if (lane == 0) {
+          s.counts[kChunks / 2 - 1 - c] = n[0], s.sums[kChunks / 2 - 1 - c] = x[0];
+          s.counts[kChunks / 2 + c] = n[1], s.sums[kChunks / 2 + c] = x[1];
+        }
+      }
+      __syncthreads();
+      if (wave == 0) {
+        const Chunks<DT> chunks(s, m, lane);
+        Place16 cut{kChunks * kChunk - 1, 0, chunks.sum()};
+        if (want.top_k > 0 && want.top_k < int64_t(chunks.count())) cut = chunks.template find<true>(u64(want.top_k) - 1);
+        if (want.top_p < 1.0f) cut = chunks.template find<false>(share_of(cut.sum, want.top_p, true));
+        if (want.min_p > 0.0) {
+          const double least = want.temp * log(want.min_p);
+          int32_t in = first, out = kMagnitudes + int32_t(Half<DT>::inf);
+          while (out - in > 1) {
+            const int32_t mid = (in + out) / 2;
+            if (double(value_at<DT>(mid)) - m.top >= least) in = mid;
+            else out = mid;
+          }
+          if (in < cut.position) cut = Place16{in, 0, chunks.sum_upto(in)};
+        }
+        if (Draw) {
+          const float u = a.uniforms[b];
+          u64 target = u < 1.0f ? share_of(cut.sum, u, false) : cut.sum;
+          if (target >= cut.sum) target = cut.sum - 1;
+          const u64 kept = cut.sum;
+          cut = chunks.template find<false>(target);
+          if (lane == 0)
+            s.logprob = float((double(value_at<DT>(cut.position)) - m.top) / want.temp - log(double(kept) * __builtin_ldexp(1.0, -m.scale)));
+        }
+        if (lane == 0) s.position = cut.position, s.rank = cut.rank;
+      }
+    } else if (tid == 0) {
+      s.position = whole ? kChunks * kChunk - 1 : first, s.rank = whole ? 0 : 1, s.logprob = 0.0f;
+    }
+    __syncthreads();
+    const uint32_t rank = s.rank;
+    border = s.position == kChunks * kChunk - 1 ? -INFINITY : value_at<DT>(s.position);
+    logprob = s.logprob;
+    last = INT64_MAX;
+    if (rank > 0) {
+      // the token of that rank among those that equal the border
+      uint32_t n[kHeld], mine = 0;
+      const auto same = [&](const Raw<DT>& x) {
+        float z[kRun];
+        unpack<DT>(x, z);
+        uint32_t e = 0;
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) e |= uint32_t(z[j] == border) << j;
+        return e;
+      };
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k) {
+        n[k] = 0;
+        if (k < held) {
+          float z[kRun];
+          unpack<DT>(raw[k], z);
+#pragma unroll
+          for (int j = 0; j < kRun; ++j) n[k] += __popcll(__ballot(z[j] == border));
+        }
+        mine += n[k];
+      }
+#pragma unroll 1
+      for (int32_t k = held; k < runs; ++k) {
+        Raw<DT> x = load_raw<DT>(row, run_of(k), V);
+        mask(x, k);
+        mine += wave_sum(uint32_t(__popc(same(x))));
+      }
+      if (lane == 0) s.found[wave] = mine;
+      if (tid == 0) s.last = -1;
+      __syncthreads();
+      uint32_t before = 0;
+      for (int k = 0; k < wave; ++k) before += s.found[k];
+      if (before < rank && rank <= before + mine) {
+        const auto look = [&](const Raw<DT>& x, int32_t k) {
+          uint32_t e = same(x);
+          const uint32_t own = __popc(e), upto = before + wave_scan_sum(own);
+          if (upto - own < rank && rank <= upto) {
+            for (uint32_t i = upto - own + 1; i < rank; ++i) e &= e - 1;
+            s.last = run_of(k).t + __builtin_ctz(e);
+          }
+        };
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) {
+          if (before < rank && rank <= before + n[k]) look(raw[k], k);
+          before += n[k];
+        }
+#pragma unroll 1
+        for (int32_t k = held; k < runs && before < rank; ++k) {
+          Raw<DT> x = load_raw<DT>(row, run_of(k), V);
+          mask(x, k);
+          look(x, k);
+          before += wave_sum(uint32_t(__popc(same(x))));
+        }
+      }
+      __syncthreads();
+      last = s.last;
+    }
+  }
+  if (flags && a.err && tid == 0) atomicOr(a.err, flags);
+  if constexpr (Draw) {
+    if (tid == 0) store_drawn(a, b, state, last, logprob);
+    return;
+  }
+  uint16_t* out = static_cast<uint16_t*>(a.out) + b * a.out_ld;
+  const auto put = [&](Raw<DT> x, int32_t k) {
+    const Run run = run_of(k);
+    float z[kRun];
+    unpack<DT>(x, z);
+#pragma unroll
+    for (int j = 0; j < kRun; ++j) {
+      const bool in = z[j] > border || (z[j] == border && run.t + j <= last);
+      if (!in) x.w[0][j / 2] = j & 1 ? (x.w[0][j / 2] & 0xFFFFu) | kNone << 16 : (x.w[0][j / 2] & 0xFFFF0000u) | kNone;
+    }
+    if (run.own == 0xFFu) {
+      __builtin_memcpy(__builtin_assume_aligned(out + run.t, 2), &x, sizeof(x));
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < kRun; ++j)
+      if (run.own >> j & 1) out[run.t + j] = uint16_t(x.w[0][j / 2] >> (16 * (j & 1)));
+  };
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k)
+    if (k < held) put(raw[k], k);
+#pragma unroll 1
+  for (int32_t k = held; k < runs; ++k) {
+    Raw<DT> x = load_raw<DT>(row, run_of(k), V);
+    mask(x, k);
+    put(x, k);
+  }
+  for (int64_t t = V + tid; t < a.cols; t += kThreads16) out[t] = uint16_t(kNone);
+}
+
 template <int DT, bool Draw>
 int launch_sample_rows(const SampleArgs& a, hipStream_t s) {
-  sample_kernel<DT, Draw><<<uint32_t(a.rows), kThreads, 0, s>>>(a);
+  if constexpr (DT == BPD_DTYPE_F32)
+    sample_kernel<DT, Draw><<<uint32_t(a.rows), kThreads, 0, s>>>(a);
+  else
+    sample16_kernel<DT, Draw><<<uint32_t(a.rows), kThreads16, 0, s>>>(a);
   BPD_LAUNCHED();
   return BPD_OK;
 }

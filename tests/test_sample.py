@@ -374,6 +374,41 @@ def test_streams_and_captured_graphs(dev):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_a_vocabulary_past_what_a_block_holds(dtype, device):
+    """Ties that reach over the end of what registers hold, an odd length."""
+    B, V = 6, 200_003
+    g = torch.Generator().manual_seed(12)
+    logits = torch.round(4 * torch.randn(B, V + 5, generator=g)) / 2
+    logits[1, :170_000] = -INF
+    logits[2, 163_840:] += 20.0
+    allow = torch.rand(B, V, generator=g) < 0.5
+    allow[4, :180_000] = False
+    print(f"sample 200,003 {dtype} on {device}", flush=True)
+    check(logits.to(dtype), V, asked_tensors(B, device), torch.rand(B, generator=g), device)
+    check(logits.to(dtype), V, asked_tensors(B, device, MIXED[4:]), torch.rand(B, generator=g), device, allow)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_exactly_as_many_as_16_bits_count(dtype, device):
+    """65,535 to 131,073 tokens of one value, of zeros of both signs, of +inf and NaN."""
+    V = 131_080
+    rows, u = [], []
+    for n in (65_535, 65_536, 65_537, 131_072, 131_073):
+        for value in (2.0, -2.0, 0.0, -0.0, INF, float("nan"), -INF):
+            row = torch.full((V,), -INF)
+            row[:7] = torch.tensor([-3.0, 1.0, -1.0, 0.5, 0.0, -0.0, -3.0])
+            row[7:7 + n] = value
+            rows.append(row[:V])
+            u.append((n % 7) / 7)
+    logits = torch.stack(rows).to(dtype)
+    print(f"16 bits {dtype} on {device}", flush=True)
+    for one in ((1.0, 0, 0.8, 0.0), (0.7, 66_000, 1.0, 0.0), (0.0, 0, 1.0, 0.0)):
+        check(logits, V, one, torch.tensor(u), device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_refusals(device):
     z, u = torch.zeros(2, 40, device=device), torch.zeros(2, device=device)
     bits, at = torch.zeros(3, 2, dtype=torch.int32, device=device), torch.zeros(2, dtype=torch.int32, device=device)
