@@ -12,6 +12,8 @@
 // (or where it is not positive and finite) the first token alone is kept.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
+#include <utility>
 #include <vector>
 
 #include "runs.hpp"
@@ -212,7 +214,7 @@ __device__ __forceinline__ void each_run(const Row& r, int64_t first, int64_t en
 
 // The token of rank `rank` (from 1) among those with this key, by index.
 template <int DT, int N>
-__device__ int64_t nth_token(const Row& r, uint32_t key, u64 rank, Scratch<N>& s) {
+__device__ __forceinline__ int64_t nth_token(const Row& r, uint32_t key, u64 rank, Scratch<N>& s) {
   constexpr int kWaves = N / kWave, kStep = N * kRun;
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   // a wave takes neighbouring tokens
@@ -271,7 +273,7 @@ __device__ __forceinline__ u64 share_of(u64 x, float f, bool ceil_less_one) {
 }
 
 template <int DT, int N>
-__device__ void sample_row(const SampleArgs& a, const Row& r, const Asked& want, int64_t b, bool draw, Scratch<N>& s,
+__device__ __forceinline__ void sample_row(const SampleArgs& a, const Row& r, const Asked& want, int64_t b, bool draw, Scratch<N>& s,
                            Cut* cut_out, int64_t* last_out, float* logprob, bool* bad_out) {
   constexpr int kWaves = N / kWave, kStep = N * kRun;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
@@ -417,19 +419,15 @@ __device__ __forceinline__ Row row_of(const SampleArgs& a, int64_t b, int32_t* s
              some ? a.vocab : 0};
 }
 
-constexpr int kThreads = 1024;
-template <int DT, bool Draw>
-__global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
-  constexpr int kStep = kThreads * kRun;
-  __shared__ Scratch<kThreads> s;
-  const int64_t b = blockIdx.x;
-  int32_t state, flags;
-  const Row r = row_of(a, b, &state, &flags);
+// All of a row's work, by a block of N threads.
+template <int DT, bool Draw, int N>
+__device__ __forceinline__ void general_row(const SampleArgs& a, const Row& r, const Asked& want, int64_t b, int32_t state, int32_t flags,
+                            Scratch<N>& s) {
   Cut cut{0xFFFFFFFFu, 0, 0};
   int64_t last = -1;
   float logprob = -INFINITY;
   bool bad = false;
-  sample_row<DT, kThreads>(a, r, asked_of(a, b), b, Draw, s, &cut, &last, &logprob, &bad);
+  sample_row<DT, N>(a, r, want, b, Draw, s, &cut, &last, &logprob, &bad);
   if (bad) flags |= BPD_FLAG_LOGITS;
   if (flags && a.err && threadIdx.x == 0) atomicOr(a.err, flags);
   if constexpr (Draw) {
@@ -443,10 +441,10 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
     if (kBytes == 4) reinterpret_cast<uint32_t*>(out)[t] = x;
     else reinterpret_cast<uint16_t*>(out)[t] = uint16_t(x);
   };
-  for (int64_t t = threadIdx.x * kRun; t < a.vocab; t += kStep) {
+  for (int64_t t = threadIdx.x * kRun; t < a.vocab; t += N * kRun) {
     const Run run = run_at(t, a.vocab);
     uint32_t keep = r.vocab ? run_bits(r, run) : 0;
-    const Raw<DT> raw = load_raw<DT>(static_cast<const char*>(a.logits) + b * a.ld * kBytes, run, a.vocab);
+    const Raw<DT> raw = load_raw<DT>(r.logits, run, a.vocab);
     float z[kRun];
     unpack<DT>(raw, z);
 #pragma unroll
@@ -457,25 +455,38 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
       if (run.own >> j & 1) put(run.t + j, in && (keep >> j & 1) ? x : none);
     }
   }
-  for (int64_t t = a.vocab + threadIdx.x; t < a.cols; t += kThreads) put(t, none);
+  for (int64_t t = a.vocab + threadIdx.x; t < a.cols; t += N) put(t, none);
+}
+
+constexpr int kThreads = 1024;
+template <int DT, bool Draw>
+__global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
+  __shared__ Scratch<kThreads> s;
+  const int64_t b = blockIdx.x;
+  int32_t state, flags;
+  const Row r = row_of(a, b, &state, &flags);
+  general_row<DT, Draw, kThreads>(a, r, asked_of(a, b), b, state, flags, s);
 }
 
 // ---------------------------------------------- rows of 16-bit logits --
 // A 16-bit type has few values, and a weight follows from the value: a row is
 // counted by value, once, and all sums are those of counts times weights.  The
-// counts lie in LDS, a word to a magnitude, positive ones in its lower half;
-// the row stays in registers, where its equal tokens are told apart by index
-// and the kept ones written.  Values stand at positions in falling order.
+// counts lie in LDS, a word to a magnitude: tokens of both signs in its lower
+// half, the negative ones in its upper.  The row stays in registers, where its
+// equal tokens are told apart by index and the kept ones written.  Values stand
+// at positions in falling order.
 constexpr int kMagnitudes = 32768;
 // Half the threads that a CU holds, with twice the registers: 40 runs are the
 // row of a vocabulary of 163,840.
 constexpr int kThreads16 = 512, kWaves16 = kThreads16 / kWave, kStep16 = kThreads16 * kRun, kHeld = 40;
-constexpr int kChunk = 4 * kWave;               // words of counts that a wave takes at a time
+constexpr int kWaveRun = kWave * kRun;  // tokens of a wave's run
+constexpr int kAhead = 8;               // runs on their way while one is counted
+constexpr int kChunk = 4 * kWave;       // words of counts that a wave takes at a time
 constexpr int kChunks = 2 * kMagnitudes / kChunk;
 
 template <int DT>
 struct Half {
-  static constexpr uint32_t inf = DT == BPD_DTYPE_BF16 ? 0x7F80u : 0x7C00u;
+  static constexpr uint32_t inf = DT == BPD_DTYPE_BF16 ? 0x7F80u : 0x7C00u, none = inf | 0x8000u;
 };
 template <int DT>
 __device__ __forceinline__ float value_of(uint32_t magnitude) {
@@ -488,12 +499,35 @@ __device__ __forceinline__ float value_at(int32_t position) {
                                 : -value_of<DT>(uint32_t(position - kMagnitudes));
 }
 
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pair_max(uint32_t x, uint32_t y) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, x), __builtin_bit_cast(u16x2, y)));
+}
+__device__ __forceinline__ uint32_t pair_signed_max(uint32_t x, uint32_t y) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(i16x2, x), __builtin_bit_cast(i16x2, y)));
+}
+__device__ __forceinline__ uint32_t pair_min(uint32_t x, uint32_t y) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, x), __builtin_bit_cast(u16x2, y)));
+}
+
+// f(k) for k = 0 .. N - 1 as constants: arrays that it indexes stay in registers.
+template <class F, int... K>
+__device__ __forceinline__ void each_of(std::integer_sequence<int, K...>, F f) {
+  (f(std::integral_constant<int, K>()), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void each(F f) {
+  each_of(std::make_integer_sequence<int, N>(), f);
+}
+
 struct Counted {
   uint32_t words[kMagnitudes];
+  uint32_t left_out[kWave];  // what a lane does not count goes to its own word
   u64 sums[kChunks];  // by chunks of positions
   uint32_t counts[kChunks];
   uint32_t added[kWaves16], found[kWaves16];
-  int32_t most[kWaves16], least_below[kWaves16], most_below[kWaves16];  // magnitudes: positive, negative
+  int32_t tops[kWaves16], bad[kWaves16];
   // what the first wave comes to
   int32_t position;
   uint32_t rank;  // 0: all of the position
@@ -507,15 +541,6 @@ struct Place16 {
   uint32_t rank;
   u64 sum;
 };
-
-// Counts of a position's magnitude; zeros of both signs stand at the first.
-__device__ __forceinline__ uint32_t count_at(const uint32_t* words, int32_t position) {
-  const bool below = position >= kMagnitudes;
-  const int32_t m = below ? position - kMagnitudes : kMagnitudes - 1 - position;
-  const uint32_t w = words[m];
-  if (m == 0) return below ? 0 : (w & 0xFFFFu) + (w >> 16);
-  return below ? w >> 16 : w & 0xFFFFu;
-}
 
 // The first wave's view of the chunks: each lane has four of them.
 template <int DT>
@@ -541,11 +566,14 @@ struct Chunks {
   }
   // the lane's four positions of chunk `c`: counts, and weights of one each
   __device__ __forceinline__ void positions(int c, uint32_t (&n)[4], u64 (&w)[4]) const {
+    const int32_t at = c * kChunk + 4 * lane;
+    const bool below = c >= kChunks / 2;
+    const uint4 q = *reinterpret_cast<const uint4*>(s.words + (below ? at - kMagnitudes : kMagnitudes - 4 - at));
+    const uint32_t x[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int32_t at = c * kChunk + 4 * lane + k;
-      n[k] = count_at(s.words, at);
-      w[k] = n[k] ? m.weight(m.y(value_at<DT>(at))) : 0;
+      n[k] = below ? x[k] >> 16 : (x[3 - k] & 0xFFFFu) - (x[3 - k] >> 16);
+      w[k] = m.weight(m.y(value_at<DT>(at + k)));
     }
   }
   // where the running count (of tokens) or sum (of weights) passes `target`
@@ -584,6 +612,8 @@ struct Chunks {
         p.position += k;
         p.rank = uint32_t(ByCount ? target - cb : (target - sb) / kw) + 1;
         p.sum = sb + p.rank * kw;
+        // zeros of both signs are equal: those of the first position count too
+        if (p.position == kMagnitudes) p.rank += (s.words[0] & 0xFFFFu) - (s.words[0] >> 16);
         return p;
       }
       cb += kn, sb = end_s;
@@ -604,143 +634,219 @@ struct Chunks {
 };
 
 // One block per row.
-template <int DT, bool Draw>
+template <int DT, bool Draw, bool Grammar>
 __global__ __launch_bounds__(kThreads16) void sample16_kernel(SampleArgs a) {
   __shared__ union {
     Counted s;
     Scratch<kThreads16> general;
   } shared;
   Counted& s = shared.s;
+  constexpr uint32_t kNone = Half<DT>::none;
   const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int64_t b = blockIdx.x, V = a.vocab;
   const char* row = static_cast<const char*>(a.logits) + b * a.ld * 2;
-  const int32_t runs = int32_t((V + kStep16 - 1) / kStep16), held = runs < kHeld ? runs : kHeld;
-  // a wave takes neighbouring tokens
-  const int64_t begin = int64_t(wave) * runs * (kWave * kRun);
-  const auto run_of = [&](int32_t k) { return run_at(begin + int64_t(k) * (kWave * kRun) + lane * kRun, V); };
-  const auto inside = [&](int32_t k) { return begin + int64_t(k + 1) * (kWave * kRun) <= V; };
+  // A wave takes neighbouring tokens: runs that lie whole in the row, the first
+  // of them held, and maybe one that does not.
+  const int32_t runs = int32_t((V + kStep16 - 1) / kStep16);
+  const int64_t begin = int64_t(wave) * runs * kWaveRun, left = V - begin;
+  const int32_t full = left <= 0 ? 0 : left < int64_t(runs) * kWaveRun ? int32_t(left / kWaveRun) : runs;
+  const bool tail = left > int64_t(full) * kWaveRun && full < runs;
+  const int32_t held = full < kHeld ? full : kHeld;
+  // (formed anew at each use: the registers hold the row instead)
+  const auto token_of = [&](int32_t k) {
+    int32_t l = lane;
+    asm volatile("" : "+v"(l));
+    return begin + int64_t(k) * kWaveRun + l * kRun;
+  };
+  const char* mine = row + (begin + lane * kRun) * 2;
+  const auto load = [&](int32_t k) {
+    Raw<DT> x;
+    __builtin_memcpy(&x, __builtin_assume_aligned(mine + int64_t(k) * (kWaveRun * 2), 2), sizeof(x));
+    return x;
+  };
   Raw<DT> raw[kHeld];
-#pragma unroll
-  for (int k = 0; k < kHeld; ++k)
-    if (k < held) raw[k] = load_raw<DT>(row, run_of(k), V);
+  each<kAhead>([&](auto k) {
+    if (k < held) raw[k] = load(k);
+  });
   int32_t state, flags;
   const Row r = row_of(a, b, &state, &flags);
+  const uint8_t* allow = Grammar && r.bits ? r.bits + (begin + lane * kRun) / 8 : nullptr;
+  const auto load_bits = [&](int32_t k) -> uint32_t { return allow ? allow[k * (kWaveRun / 8)] : 0u; };
+  uint32_t bits[kAhead];
+  if constexpr (Grammar)
+    each<kAhead>([&](auto k) {
+      if (k < held) bits[k] = load_bits(k);
+    });
   const Asked want = asked_of(a, b);
   for (int i = tid; i < kMagnitudes / 4; i += kThreads16) reinterpret_cast<uint4*>(s.words)[i] = uint4{0, 0, 0, 0};
-  constexpr uint32_t kNone = Half<DT>::inf | 0x8000u;
-  // -inf for what is not the thread's own or not allowed
-  const auto mask = [&](Raw<DT>& x, int32_t k) {
-    if (inside(k) && !r.bits && r.vocab) return;
-    const uint32_t valid = r.vocab ? run_bits(r, run_of(k)) : 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (!(valid >> (2 * i) & 1)) x.w[0][i] = (x.w[0][i] & 0xFFFF0000u) | kNone;
-      if (!(valid >> (2 * i + 1) & 1)) x.w[0][i] = (x.w[0][i] & 0xFFFFu) | kNone << 16;
-    }
-  };
-#pragma unroll
-  for (int k = 0; k < kHeld; ++k)
-    if (k < held) mask(raw[k], k);
-  __syncthreads();
-  uint32_t added = 0;
-  const auto add = [&](const Raw<DT>& x) {
-#pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      const uint32_t h = x.w[0][j / 2] >> (16 * (j & 1)) & 0xFFFFu;
-      const bool on = h != kNone;
-      if (on) atomicAdd(&s.words[h & 0x7FFFu], h & 0x8000u ? 0x10000u : 1u);
-      added += __popcll(__ballot(on));
-    }
-  };
-#pragma unroll
-  for (int k = 0; k < kHeld; ++k)
-    if (k < held) add(raw[k]);
-#pragma unroll 1
-  for (int32_t k = held; k < runs; ++k) {
-    Raw<DT> x = load_raw<DT>(row, run_of(k), V);
-    mask(x, k);
-    add(x);
-  }
-  if (lane == 0) s.added[wave] = added;
+  if (tid < kChunks) s.counts[tid] = 0, s.sums[tid] = 0;
   __syncthreads();
 
-  // the largest value, whether all are numbers, and whether all were counted:
-  // a count past 16 bits leaves fewer
-  int32_t most = -1, least_below = kMagnitudes, most_below = -1;
-  uint32_t counted = 0;
+  // -inf for tokens whose bit is not set
+  const auto mask = [&](Raw<DT>& x, uint32_t valid) {
 #pragma unroll
-  for (int i = 0; i < kMagnitudes / 4 / kThreads16; ++i) {
-    const int32_t at = (i * kThreads16 + tid) * 4;
-    const uint4 q = *reinterpret_cast<const uint4*>(s.words + at);
-    if ((q.x | q.y | q.z | q.w) == 0) continue;
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = uint32_t(int32_t(valid << (31 - 2 * i)) >> 31), hi = uint32_t(int32_t(valid << (30 - 2 * i)) >> 31);
+      const uint32_t keep = (lo & 0xFFFFu) | (hi & 0xFFFF0000u);
+      x.w[0][i] = (x.w[0][i] & keep) | ((kNone << 16 | kNone) & ~keep);
+    }
+  };
+  // Counts a run, and follows the largest of the values that are not negative.
+  // Five instructions a token, and two for its run's part: what bounds this,
+  // beside the LDS, which takes 7.3 cycles for 64 additions at random words.
+  uint32_t most = 0xFFFFFFFFu, not_counted = 0;
+  char* words = reinterpret_cast<char*>(s.words);
+  const auto count = [&](const Raw<DT>& x) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (w[k] & 0xFFFFu) most = max(most, at + k);
-      if (w[k] >> 16) least_below = min(least_below, at + k), most_below = max(most_below, at + k);
-      counted += (w[k] & 0xFFFFu) + (w[k] >> 16);
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = x.w[0][i];
+      most = pair_signed_max(most, w);
+      atomicAdd(reinterpret_cast<uint32_t*>(words + (w << 2 & 0x1FFFCu)), (w << 1 & 0x10000u) | 1u);
+      atomicAdd(reinterpret_cast<uint32_t*>(words + (w >> 14 & 0x1FFFCu)), (w >> 15 & 0x10000u) | 1u);
+    }
+  };
+  // the same, but for tokens of -inf
+  const uint32_t apart = uint32_t(reinterpret_cast<char*>(s.left_out + lane) - words);
+  const auto count_some = [&](const Raw<DT>& x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = x.w[0][i];
+      most = pair_signed_max(most, w);
+      const bool lo = (w & 0xFFFFu) == kNone, hi = w >> 16 == kNone;
+      atomicAdd(reinterpret_cast<uint32_t*>(words + (lo ? apart : w << 2 & 0x1FFFCu)), (w << 1 & 0x10000u) | 1u);
+      atomicAdd(reinterpret_cast<uint32_t*>(words + (hi ? apart : w >> 14 & 0x1FFFCu)), (w >> 15 & 0x10000u) | 1u);
+      not_counted += uint32_t(lo) + uint32_t(hi);
+    }
+  };
+  const auto is_none = [&](const Raw<DT>& x) {  // some of the run is -inf (or a negative NaN)
+    const uint32_t u = pair_max(pair_max(x.w[0][0], x.w[0][1]), pair_max(x.w[0][2], x.w[0][3]));
+    return u >= kNone << 16 || (u & 0xFFFFu) >= kNone;
+  };
+  const auto take = [&](Raw<DT>& x, uint32_t valid) {
+    if constexpr (Grammar) {
+      mask(x, valid);
+      if (__any(valid != 0)) count_some(x);
+      else not_counted += kRun;
+    } else {
+      if (__builtin_expect(__any(is_none(x)), 0)) count_some(x);
+      else count(x);
+    }
+  };
+  each<kHeld>([&](auto k) {
+    if (k >= held) return;
+    uint32_t valid = 0;
+    if constexpr (Grammar) valid = bits[k % kAhead];
+    if constexpr (k + kAhead < kHeld) {
+      if (k + kAhead < held) {
+        raw[k + kAhead] = load(k + kAhead);
+        if constexpr (Grammar) bits[k % kAhead] = load_bits(k + kAhead);
+      }
+    }
+    take(raw[k], valid);
+  });
+  const auto again = [&](int32_t k) {  // a run past those held
+    Raw<DT> x = load(k);
+    if constexpr (Grammar) mask(x, load_bits(k));
+    return x;
+  };
+#pragma unroll 1
+  for (int32_t k = held; k < full; ++k) count_some(again(k));
+  Raw<DT> end{};  // the run that is not whole
+  if (tail) {
+    const Run run = run_at(token_of(full), V);
+    end = load_raw<DT>(row, run, V);
+    mask(end, r.vocab ? run_bits(r, run) : 0u);
+    count_some(end);
+  }
+  int32_t top_bits = max(int32_t(most) >> 16, int32_t(most << 16) >> 16);
+  top_bits = -wave_min(-top_bits);
+  const uint32_t added = wave_sum(uint32_t(full + tail) * kRun - not_counted);
+  if (lane == 0) s.added[wave] = added, s.tops[wave] = top_bits;
+  __syncthreads();
+  uint32_t all = 0, counted = 0;
+  for (int k = 0; k < kWaves16; ++k) all += s.added[k], top_bits = max(top_bits, s.tops[k]);
+  float top = value_of<DT>(uint32_t(top_bits));
+  if (top_bits < 0) {  // no value but negative ones (and -0): the smallest magnitude
+    int32_t least = kMagnitudes - 1;
+#pragma unroll 1
+    for (int i = tid; i < kMagnitudes; i += kThreads16)
+      if (s.words[i] != 0) {
+        least = i;
+        break;
+      }
+    least = wave_min(least);
+    __syncthreads();
+    if (lane == 0) s.tops[wave] = least;
+    __syncthreads();
+    for (int k = 0; k < kWaves16; ++k) least = min(least, s.tops[k]);
+    top = 0.0f - value_of<DT>(uint32_t(least));
+  }
+
+  // counts and sums of the chunks; whether all are numbers, and whether all were
+  // counted: a count past 16 bits leaves fewer
+  const Measure m{double(top), want.temp > 0.0 ? kLog2E / want.temp : 0.0, 0.0, scale_of(V)};
+  bool bad = false;
+#pragma unroll 1
+  for (int i0 = 0; i0 < kChunks / 2 / kWaves16; i0 += 4) {
+    uint4 q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = reinterpret_cast<const uint4*>(s.words)[((i0 + i) * kWaves16 + wave) * kWave + lane];
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) {
+      const int32_t c = (i0 + i) * kWaves16 + wave, at = c * kChunk + 4 * lane;
+      const uint32_t w[4] = {q[0].x, q[0].y, q[0].z, q[0].w};
+      q[0] = q[1], q[1] = q[2], q[2] = q[3];
+      if (!__any((w[0] | w[1] | w[2] | w[3]) != 0)) continue;
+      uint32_t n[2] = {0, 0};
+      u64 x[2] = {0, 0};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t below = w[k] >> 16, above = (w[k] & 0xFFFFu) - below;
+        counted += w[k] & 0xFFFFu;
+        n[0] += above, n[1] += below;
+        bad |= at + k >= int32_t(Half<DT>::inf) && (at + k == int32_t(Half<DT>::inf) ? above : w[k]) != 0;
+      }
+#pragma unroll 1
+      for (int e = 0; e < 2; ++e) {
+        if (!__any(n[0] != 0)) {
+          n[0] = n[1];
+          continue;
+        }
+        u64 sum = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float z = value_of<DT>(at + k);
+          const uint32_t below = w[k] >> 16;
+          sum += (e ? below : (w[k] & 0xFFFFu) - below) * m.weight(m.y(e ? -z : z));
+        }
+        const uint32_t tokens = wave_sum(n[0]);
+        sum = wave_sum(sum);
+        if (lane == 0) s.counts[e ? kChunks / 2 + c : kChunks / 2 - 1 - c] = tokens, s.sums[e ? kChunks / 2 + c : kChunks / 2 - 1 - c] = sum;
+        n[0] = n[1];
+      }
     }
   }
-  most = -wave_min(-most), least_below = wave_min(least_below), most_below = -wave_min(-most_below);
   counted = wave_sum(counted);
-  if (lane == 0) s.most[wave] = most, s.least_below[wave] = least_below, s.most_below[wave] = most_below, s.found[wave] = counted;
+  bad = __any(bad);
+  if (lane == 0) s.found[wave] = counted, s.bad[wave] = bad;
   __syncthreads();
-  uint32_t all = 0;
   counted = 0;
-  for (int k = 0; k < kWaves16; ++k) {
-    most = max(most, s.most[k]), least_below = min(least_below, s.least_below[k]), most_below = max(most_below, s.most_below[k]);
-    all += s.added[k], counted += s.found[k];
+  for (int k = 0; k < kWaves16; ++k) counted += s.found[k], bad |= s.bad[k] != 0;
+  if (__builtin_expect(counted != all, 0)) {
+    __syncthreads();
+    general_row<DT, Draw, kThreads16>(a, r, want, b, state, flags, shared.general);
+    return;
   }
-  const bool bad = most >= int32_t(Half<DT>::inf) || most_below > int32_t(Half<DT>::inf);
-  const bool none = bad || (most < 0 && least_below == kMagnitudes);
+  const bool none = bad || all == 0;
   if (bad) flags |= BPD_FLAG_LOGITS;
   int64_t last = -1;
   float border = INFINITY, logprob = -INFINITY;  // what lies above it is kept, and of what equals it all up to `last`
-  if (!none && counted != all) {
-    __syncthreads();
-    Cut cut{0xFFFFFFFFu, 0, 0};
-    bool is_bad;
-    sample_row<DT, kThreads16>(a, r, want, b, Draw, shared.general, &cut, &last, &logprob, &is_bad);
-    if (is_bad) flags |= BPD_FLAG_LOGITS;
-    if (cut.rank) border = logit_of(cut.key);
-    else if (cut.key == 0) border = -INFINITY;
-    else if (cut.key != 0xFFFFFFFFu) border = logit_of(cut.key + 1), last = INT64_MAX;
-  } else if (!none) {
-    const float top = most >= 0 ? value_of<DT>(uint32_t(most)) : -value_of<DT>(uint32_t(least_below));
-    const int32_t first = most >= 0 ? kMagnitudes - 1 - most : kMagnitudes + (least_below == 0 ? -1 : least_below);
-    Measure m{double(top), want.temp > 0.0 ? kLog2E / want.temp : 0.0, 0.0, scale_of(V)};
+  if (!none) {
+    const uint32_t magnitude = DT == BPD_DTYPE_BF16 ? __builtin_bit_cast(uint32_t, fabsf(top)) >> 16
+                                                    : __builtin_bit_cast(uint16_t, _Float16(fabsf(top)));
+    const int32_t first = top < 0.0f ? kMagnitudes + int32_t(magnitude) : kMagnitudes - 1 - int32_t(magnitude);
     const bool whole = want.temp > 0.0 && want.top_k == 0 && want.top_p >= 1.0f && want.min_p <= 0.0;
     if (want.temp > 0.0 && (Draw || !whole)) {
-      // counts and sums of the chunks
-#pragma unroll 1
-      for (int i = 0; i < kChunks / 2 / kWaves16; ++i) {
-        const int32_t c = i * kWaves16 + wave;
-        const uint4 q = reinterpret_cast<const uint4*>(s.words)[c * kWave + lane];
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-        const bool any = __any((q.x | q.y | q.z | q.w) != 0);
-        uint32_t n[2] = {0, 0};
-        u64 x[2] = {0, 0};
-        if (any) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int32_t at = c * kChunk + 4 * lane + k;
-            uint32_t here[2] = {w[k] & 0xFFFFu, w[k] >> 16};
-            if (at == 0) here[0] += here[1], here[1] = 0;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              n[e] += here[e];
-              if (__any(here[e] != 0)) x[e] += here[e] * m.weight(m.y(e ? -value_of<DT>(at) : value_of<DT>(at)));
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 2; ++e) n[e] = wave_sum(n[e]), x[e] = wave_sum(x[e]);
-        }
-        if (lane == 0) {
-          s.counts[kChunks / 2 - 1 - c] = n[0], s.sums[kChunks / 2 - 1 - c] = x[0];
-          s.counts[kChunks / 2 + c] = n[1], s.sums[kChunks / 2 + c] = x[1];
-        }
-      }
-      __syncthreads();
       if (wave == 0) {
         const Chunks<DT> chunks(s, m, lane);
         Place16 cut{kChunks * kChunk - 1, 0, chunks.sum()};
@@ -776,59 +882,56 @@ __global__ __launch_bounds__(kThreads16) void sample16_kernel(SampleArgs a) {
     logprob = s.logprob;
     last = INT64_MAX;
     if (rank > 0) {
-      // the token of that rank among those that equal the border
-      uint32_t n[kHeld], mine = 0;
-      const auto same = [&](const Raw<DT>& x) {
-        float z[kRun];
-        unpack<DT>(x, z);
-        uint32_t e = 0;
-#pragma unroll
-        for (int j = 0; j < kRun; ++j) e |= uint32_t(z[j] == border) << j;
-        return e;
+      // The token of that rank among those that equal the border: halves that
+      // differ from it are counted two at a time.
+      const uint32_t h = uint32_t(s.position < kMagnitudes ? kMagnitudes - 1 - s.position : s.position - kMagnitudes) |
+                         (s.position < kMagnitudes ? 0u : 0x8000u);
+      const bool zero = (h & 0x7FFFu) == 0;
+      const uint32_t both = zero ? 0u : h << 16 | h, sign = zero ? 0x7FFF7FFFu : 0xFFFFFFFFu;
+      const auto other = [&](uint32_t w) {  // 1 in halves that differ
+        return pair_min((w & sign) ^ both, 0x00010001u);
       };
-#pragma unroll
-      for (int k = 0; k < kHeld; ++k) {
-        n[k] = 0;
-        if (k < held) {
-          float z[kRun];
-          unpack<DT>(raw[k], z);
-#pragma unroll
-          for (int j = 0; j < kRun; ++j) n[k] += __popcll(__ballot(z[j] == border));
-        }
-        mine += n[k];
-      }
+      const auto others = [&](const Raw<DT>& x) { return (other(x.w[0][0]) + other(x.w[0][1])) + (other(x.w[0][2]) + other(x.w[0][3])); };
+      uint32_t differ = 0;  // (two sums of 16 bits: at most 4 a run in each)
+      each<kHeld>([&](auto k) {
+        if (k < held) differ += others(raw[k]);
+      });
+      uint32_t same = uint32_t(held) * kRun - (differ & 0xFFFFu) - (differ >> 16);
+      const auto add = [&](const Raw<DT>& x) {
+        const uint32_t d = others(x);
+        same += kRun - (d & 0xFFFFu) - (d >> 16);
+      };
 #pragma unroll 1
-      for (int32_t k = held; k < runs; ++k) {
-        Raw<DT> x = load_raw<DT>(row, run_of(k), V);
-        mask(x, k);
-        mine += wave_sum(uint32_t(__popc(same(x))));
-      }
-      if (lane == 0) s.found[wave] = mine;
+      for (int32_t k = held; k < full; ++k) add(again(k));
+      if (tail) add(end);
+      same = wave_sum(same);
+      if (lane == 0) s.found[wave] = same;
       if (tid == 0) s.last = -1;
       __syncthreads();
       uint32_t before = 0;
       for (int k = 0; k < wave; ++k) before += s.found[k];
-      if (before < rank && rank <= before + mine) {
+      if (before < rank && rank <= before + same) {
         const auto look = [&](const Raw<DT>& x, int32_t k) {
-          uint32_t e = same(x);
+          if (__builtin_expect(before >= rank || !__any(others(x) != 0x00040004u), 1)) return;
+          uint32_t e = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t d = other(x.w[0][i]);
+            e |= (~d & 1u) << (2 * i) | (~(d >> 16) & 1u) << (2 * i + 1);
+          }
           const uint32_t own = __popc(e), upto = before + wave_scan_sum(own);
           if (upto - own < rank && rank <= upto) {
             for (uint32_t i = upto - own + 1; i < rank; ++i) e &= e - 1;
-            s.last = run_of(k).t + __builtin_ctz(e);
+            s.last = run_at(token_of(k), V).t + __builtin_ctz(e);
           }
+          before = of_lane(upto, kWave - 1);
         };
-#pragma unroll
-        for (int k = 0; k < kHeld; ++k) {
-          if (before < rank && rank <= before + n[k]) look(raw[k], k);
-          before += n[k];
-        }
+        each<kHeld>([&](auto k) {
+          if (k < held) look(raw[k], k);
+        });
 #pragma unroll 1
-        for (int32_t k = held; k < runs && before < rank; ++k) {
-          Raw<DT> x = load_raw<DT>(row, run_of(k), V);
-          mask(x, k);
-          look(x, k);
-          before += wave_sum(uint32_t(__popc(same(x))));
-        }
+        for (int32_t k = held; k < full && before < rank; ++k) look(again(k), k);
+        if (tail) look(end, full);
       }
       __syncthreads();
       last = s.last;
@@ -840,41 +943,45 @@ __global__ __launch_bounds__(kThreads16) void sample16_kernel(SampleArgs a) {
     return;
   }
   uint16_t* out = static_cast<uint16_t*>(a.out) + b * a.out_ld;
-  const auto put = [&](Raw<DT> x, int32_t k) {
-    const Run run = run_of(k);
+  const auto cut = [&](Raw<DT>& x, int64_t t) {
     float z[kRun];
     unpack<DT>(x, z);
 #pragma unroll
     for (int j = 0; j < kRun; ++j) {
-      const bool in = z[j] > border || (z[j] == border && run.t + j <= last);
+      const bool in = z[j] > border || (z[j] == border && t + j <= last);
       if (!in) x.w[0][j / 2] = j & 1 ? (x.w[0][j / 2] & 0xFFFFu) | kNone << 16 : (x.w[0][j / 2] & 0xFFFF0000u) | kNone;
     }
-    if (run.own == 0xFFu) {
-      __builtin_memcpy(__builtin_assume_aligned(out + run.t, 2), &x, sizeof(x));
-      return;
-    }
+  };
+  const auto put = [&](Raw<DT> x, int32_t k) {
+    const int64_t t = token_of(k);
+    cut(x, t);
+    __builtin_memcpy(__builtin_assume_aligned(out + t, 2), &x, sizeof(x));
+  };
+  each<kHeld>([&](auto k) {
+    if (k < held) put(raw[k], k);
+  });
+#pragma unroll 1
+  for (int32_t k = held; k < full; ++k) put(again(k), k);
+  if (tail) {
+    const Run run = run_at(token_of(full), V);
+    cut(end, run.t);
 #pragma unroll
     for (int j = 0; j < kRun; ++j)
-      if (run.own >> j & 1) out[run.t + j] = uint16_t(x.w[0][j / 2] >> (16 * (j & 1)));
-  };
-#pragma unroll
-  for (int k = 0; k < kHeld; ++k)
-    if (k < held) put(raw[k], k);
-#pragma unroll 1
-  for (int32_t k = held; k < runs; ++k) {
-    Raw<DT> x = load_raw<DT>(row, run_of(k), V);
-    mask(x, k);
-    put(x, k);
+      if (run.own >> j & 1) out[run.t + j] = uint16_t(end.w[0][j / 2] >> (16 * (j & 1)));
   }
   for (int64_t t = V + tid; t < a.cols; t += kThreads16) out[t] = uint16_t(kNone);
 }
 
 template <int DT, bool Draw>
 int launch_sample_rows(const SampleArgs& a, hipStream_t s) {
-  if constexpr (DT == BPD_DTYPE_F32)
+  if constexpr (DT == BPD_DTYPE_F32) {
     sample_kernel<DT, Draw><<<uint32_t(a.rows), kThreads, 0, s>>>(a);
-  else
-    sample16_kernel<DT, Draw><<<uint32_t(a.rows), kThreads16, 0, s>>>(a);
+  } else {
+    if (a.allow_bits)
+      sample16_kernel<DT, Draw, true><<<uint32_t(a.rows), kThreads16, 0, s>>>(a);
+    else
+      sample16_kernel<DT, Draw, false><<<uint32_t(a.rows), kThreads16, 0, s>>>(a);
+  }
   BPD_LAUNCHED();
   return BPD_OK;
 }
