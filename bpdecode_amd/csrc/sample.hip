@@ -95,8 +95,7 @@ constexpr int kMostScale = 50;  // a weight is read off the bits of its sum with
 
 // Bits of a weight: the sum of a row's fits 63.
 __host__ __device__ __forceinline__ int scale_of(int64_t vocab) {
-  int bits = 0;
-  while ((int64_t(1) << bits) < vocab) ++bits;
+  const int bits = vocab > 1 ? 64 - __builtin_clzll(uint64_t(vocab) - 1) : 0;
   return 62 - bits < kMostScale ? 62 - bits : kMostScale;
 }
 
@@ -581,14 +580,19 @@ struct Chunks {
   __device__ __forceinline__ Place16 find(u64 target) const {
     const u64 from = ByCount ? count_before : sum_before, own = ByCount ? count_mine : sum_mine;
     const int l = __builtin_ctzll(__ballot(from <= target && target < from + own) | u64(1) << 63);
+    const uint4 four = *reinterpret_cast<const uint4*>(s.counts + 4 * l);
+    const ulonglong2 two[2] = {reinterpret_cast<const ulonglong2*>(s.sums + 4 * l)[0],
+                               reinterpret_cast<const ulonglong2*>(s.sums + 4 * l)[1]};
+    const uint32_t fc[3] = {four.x, four.y, four.z};
+    const u64 fs[3] = {two[0].x, two[0].y, two[1].x};
     int c = 4 * l;
-    uint32_t cb;
-    u64 sb;
-    before(c, &cb, &sb);
+    uint32_t cb = of_lane(count_before, l);
+    u64 sb = of_lane(sum_before, l);
+#pragma unroll
     for (int k = 0; k < 3; ++k) {
-      const uint32_t nc = cb + s.counts[c];
-      const u64 ns = sb + s.sums[c];
-      if (target < (ByCount ? nc : ns)) break;
+      const uint32_t nc = cb + fc[k];
+      const u64 ns = sb + fs[k];
+      if (c != 4 * l + k || target < (ByCount ? nc : ns)) continue;
       cb = nc, sb = ns, ++c;
     }
     uint32_t n[4];
@@ -610,7 +614,13 @@ struct Chunks {
       const u64 kw = of_lane(w[k], hit), end_s = sb + kn * kw;
       if (kn && target < (ByCount ? u64(cb + kn) : end_s)) {
         p.position += k;
-        p.rank = uint32_t(ByCount ? target - cb : (target - sb) / kw) + 1;
+        if (ByCount) {
+          p.rank = uint32_t(target) - cb + 1;
+        } else {  // the quotient, by its nearest float of 64 bits
+          p.rank = uint32_t(double(target - sb) / double(kw));
+          p.rank += (p.rank + u64(1)) * kw <= target - sb ? 1u : p.rank * kw > target - sb ? -1u : 0u;
+          ++p.rank;
+        }
         p.sum = sb + p.rank * kw;
         // zeros of both signs are equal: those of the first position count too
         if (p.position == kMagnitudes) p.rank += (s.words[0] & 0xFFFFu) - (s.words[0] >> 16);
@@ -678,6 +688,7 @@ __global__ __launch_bounds__(kThreads16) void sample16_kernel(SampleArgs a) {
       if (k < held) bits[k] = load_bits(k);
     });
   const Asked want = asked_of(a, b);
+  Measure m{0.0, want.temp > 0.0 ? kLog2E / want.temp : 0.0, 0.0, scale_of(V)};
   for (int i = tid; i < kMagnitudes / 4; i += kThreads16) reinterpret_cast<uint4*>(s.words)[i] = uint4{0, 0, 0, 0};
   if (tid < kChunks) s.counts[tid] = 0, s.sums[tid] = 0;
   __syncthreads();
@@ -784,46 +795,47 @@ __global__ __launch_bounds__(kThreads16) void sample16_kernel(SampleArgs a) {
 
   // counts and sums of the chunks; whether all are numbers, and whether all were
   // counted: a count past 16 bits leaves fewer
-  const Measure m{double(top), want.temp > 0.0 ? kLog2E / want.temp : 0.0, 0.0, scale_of(V)};
+  m.top = double(top);
   bool bad = false;
-#pragma unroll 1
-  for (int i0 = 0; i0 < kChunks / 2 / kWaves16; i0 += 4) {
-    uint4 q[4];
+  constexpr int kMine = kChunks / 2 / kWaves16;  // of a wave, every kWaves16-th
+  uint32_t some = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] = reinterpret_cast<const uint4*>(s.words)[((i0 + i) * kWaves16 + wave) * kWave + lane];
-#pragma unroll 1
-    for (int i = 0; i < 4; ++i) {
-      const int32_t c = (i0 + i) * kWaves16 + wave, at = c * kChunk + 4 * lane;
-      const uint32_t w[4] = {q[0].x, q[0].y, q[0].z, q[0].w};
-      q[0] = q[1], q[1] = q[2], q[2] = q[3];
-      if (!__any((w[0] | w[1] | w[2] | w[3]) != 0)) continue;
-      uint32_t n[2] = {0, 0};
-      u64 x[2] = {0, 0};
+  for (int i = 0; i < kMine; ++i) {
+    const uint4 q = reinterpret_cast<const uint4*>(s.words)[(i * kWaves16 + wave) * kWave + lane];
+    some |= uint32_t(__any((q.x | q.y | q.z | q.w) != 0)) << i;
+  }
+  while (some) {
+    const int32_t c = __builtin_ctz(some) * kWaves16 + wave, at = c * kChunk + 4 * lane;
+    some &= some - 1;
+    const uint4 q = reinterpret_cast<const uint4*>(s.words)[c * kWave + lane];
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    uint32_t n[2] = {0, 0};
+    u64 x[2];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t below = w[k] >> 16, above = (w[k] & 0xFFFFu) - below;
-        counted += w[k] & 0xFFFFu;
-        n[0] += above, n[1] += below;
-        bad |= at + k >= int32_t(Half<DT>::inf) && (at + k == int32_t(Half<DT>::inf) ? above : w[k]) != 0;
-      }
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t below = w[k] >> 16, above = (w[k] & 0xFFFFu) - below;
+      counted += w[k] & 0xFFFFu;
+      n[0] += above, n[1] += below;
+      bad |= at + k >= int32_t(Half<DT>::inf) && (at + k == int32_t(Half<DT>::inf) ? above : w[k]) != 0;
+    }
 #pragma unroll 1
-      for (int e = 0; e < 2; ++e) {
-        if (!__any(n[0] != 0)) {
-          n[0] = n[1];
-          continue;
-        }
-        u64 sum = 0;
+    for (int e = 0; e < 2; ++e) {
+      u64 sum = 0;
+      if (__any(n[e] != 0)) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const float z = value_of<DT>(at + k);
           const uint32_t below = w[k] >> 16;
           sum += (e ? below : (w[k] & 0xFFFFu) - below) * m.weight(m.y(e ? -z : z));
         }
-        const uint32_t tokens = wave_sum(n[0]);
-        sum = wave_sum(sum);
-        if (lane == 0) s.counts[e ? kChunks / 2 + c : kChunks / 2 - 1 - c] = tokens, s.sums[e ? kChunks / 2 + c : kChunks / 2 - 1 - c] = sum;
-        n[0] = n[1];
       }
+      x[e] = sum;
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) n[e] = wave_scan_sum(n[e]), x[e] = wave_scan_sum(x[e]);
+    if (lane == kWave - 1) {
+      s.counts[kChunks / 2 - 1 - c] = n[0], s.sums[kChunks / 2 - 1 - c] = x[0];
+      s.counts[kChunks / 2 + c] = n[1], s.sums[kChunks / 2 + c] = x[1];
     }
   }
   counted = wave_sum(counted);
@@ -892,27 +904,35 @@ __global__ __launch_bounds__(kThreads16) void sample16_kernel(SampleArgs a) {
         return pair_min((w & sign) ^ both, 0x00010001u);
       };
       const auto others = [&](const Raw<DT>& x) { return (other(x.w[0][0]) + other(x.w[0][1])) + (other(x.w[0][2]) + other(x.w[0][3])); };
-      uint32_t differ = 0;  // (two sums of 16 bits: at most 4 a run in each)
-      each<kHeld>([&](auto k) {
-        if (k < held) differ += others(raw[k]);
-      });
-      uint32_t same = uint32_t(held) * kRun - (differ & 0xFFFFu) - (differ >> 16);
-      const auto add = [&](const Raw<DT>& x) {
+      const auto none_of = [&](const Raw<DT>& x) {  // no token equals the border
+        const uint32_t least = pair_min(pair_min((x.w[0][0] & sign) ^ both, (x.w[0][1] & sign) ^ both),
+                                        pair_min((x.w[0][2] & sign) ^ both, (x.w[0][3] & sign) ^ both));
+        return pair_min(least, 0x00010001u) == 0x00010001u;
+      };
+      uint32_t same = 0;
+      uint64_t equal = 0;  // held runs in which some token does
+      const auto add_some = [&](const Raw<DT>& x) {
         const uint32_t d = others(x);
         same += kRun - (d & 0xFFFFu) - (d >> 16);
       };
+      each<kHeld>([&](auto k) {
+        if (k >= held || !__any(!none_of(raw[k]))) return;
+        equal |= uint64_t(1) << k;
+        add_some(raw[k]);
+      });
 #pragma unroll 1
-      for (int32_t k = held; k < full; ++k) add(again(k));
-      if (tail) add(end);
+      for (int32_t k = held; k < full; ++k) add_some(again(k));
+      if (tail) add_some(end);
       same = wave_sum(same);
       if (lane == 0) s.found[wave] = same;
       if (tid == 0) s.last = -1;
       __syncthreads();
       uint32_t before = 0;
-      for (int k = 0; k < wave; ++k) before += s.found[k];
+#pragma unroll
+      for (int k = 0; k < kWaves16; ++k) before += k < wave ? s.found[k] : 0;
       if (before < rank && rank <= before + same) {
         const auto look = [&](const Raw<DT>& x, int32_t k) {
-          if (__builtin_expect(before >= rank || !__any(others(x) != 0x00040004u), 1)) return;
+          if (before >= rank) return;
           uint32_t e = 0;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -926,8 +946,11 @@ __global__ __launch_bounds__(kThreads16) void sample16_kernel(SampleArgs a) {
           }
           before = of_lane(upto, kWave - 1);
         };
-        each<kHeld>([&](auto k) {
-          if (k < held) look(raw[k], k);
+        each<kHeld / 8>([&](auto k8) {
+          if ((equal >> (8 * k8) & 0xFF) == 0) return;
+          each<8>([&](auto k) {
+            if (__builtin_expect(equal >> (8 * k8 + k) & 1, 0)) look(raw[8 * k8 + k], 8 * k8 + k);
+          });
         });
 #pragma unroll 1
         for (int32_t k = held; k < full && before < rank; ++k) look(again(k), k);
