@@ -541,6 +541,21 @@ struct Place16 {
   u64 sum;
 };
 
+// A lane's four positions of chunk `c`: counts, and weights of one each.
+template <int DT>
+__device__ __forceinline__ void chunk_positions(const Counted& s, const Measure& m, int c, int lane, uint32_t (&n)[4],
+                                                u64 (&w)[4]) {
+  const int32_t at = c * kChunk + 4 * lane;
+  const bool below = c >= kChunks / 2;
+  const uint4 q = *reinterpret_cast<const uint4*>(s.words + (below ? at - kMagnitudes : kMagnitudes - 4 - at));
+  const uint32_t x[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    n[k] = below ? x[k] >> 16 : (x[3 - k] & 0xFFFFu) - (x[3 - k] >> 16);
+    w[k] = m.weight(m.y(value_at<DT>(at + k)));
+  }
+}
+
 // The first wave's view of the chunks: each lane has four of them.
 template <int DT>
 struct Chunks {
@@ -562,18 +577,6 @@ struct Chunks {
   __device__ __forceinline__ void before(int c, uint32_t* count, u64* sum) const {
     *count = of_lane(count_before, c / 4), *sum = of_lane(sum_before, c / 4);
     for (int k = c / 4 * 4; k < c; ++k) *count += s.counts[k], *sum += s.sums[k];
-  }
-  // the lane's four positions of chunk `c`: counts, and weights of one each
-  __device__ __forceinline__ void positions(int c, uint32_t (&n)[4], u64 (&w)[4]) const {
-    const int32_t at = c * kChunk + 4 * lane;
-    const bool below = c >= kChunks / 2;
-    const uint4 q = *reinterpret_cast<const uint4*>(s.words + (below ? at - kMagnitudes : kMagnitudes - 4 - at));
-    const uint32_t x[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      n[k] = below ? x[k] >> 16 : (x[3 - k] & 0xFFFFu) - (x[3 - k] >> 16);
-      w[k] = m.weight(m.y(value_at<DT>(at + k)));
-    }
   }
   // where the running count (of tokens) or sum (of weights) passes `target`
   template <bool ByCount>
@@ -597,7 +600,7 @@ struct Chunks {
     }
     uint32_t n[4];
     u64 w[4];
-    positions(c, n, w);
+    chunk_positions<DT>(s, m, c, lane, n, w);
     uint32_t nc = 0;
     u64 ns = 0;
 #pragma unroll
@@ -636,7 +639,7 @@ struct Chunks {
     uint32_t cb, n[4];
     u64 sb, w[4], x = 0;
     before(c, &cb, &sb);
-    positions(c, n, w);
+    chunk_positions<DT>(s, m, c, lane, n, w);
 #pragma unroll
     for (int k = 0; k < 4; ++k) x += c * kChunk + 4 * lane + k <= position ? n[k] * w[k] : 0;
     return sb + wave_sum(x);
@@ -793,8 +796,8 @@ __global__ __launch_bounds__(kThreads16) void sample16_kernel(SampleArgs a) {
     top = 0.0f - value_of<DT>(uint32_t(least));
   }
 
-  // counts and sums of the chunks; whether all are numbers, and whether all were
-  // counted: a count past 16 bits leaves fewer
+  // counts of the chunks; whether all are numbers, and whether all were counted: a
+  // count past 16 bits leaves fewer
   m.top = double(top);
   bool bad = false;
   constexpr int kMine = kChunks / 2 / kWaves16;  // of a wave, every kWaves16-th
@@ -810,7 +813,6 @@ __global__ __launch_bounds__(kThreads16) void sample16_kernel(SampleArgs a) {
     const uint4 q = reinterpret_cast<const uint4*>(s.words)[c * kWave + lane];
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
     uint32_t n[2] = {0, 0};
-    u64 x[2];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const uint32_t below = w[k] >> 16, above = (w[k] & 0xFFFFu) - below;
@@ -818,25 +820,9 @@ __global__ __launch_bounds__(kThreads16) void sample16_kernel(SampleArgs a) {
       n[0] += above, n[1] += below;
       bad |= at + k >= int32_t(Half<DT>::inf) && (at + k == int32_t(Half<DT>::inf) ? above : w[k]) != 0;
     }
-#pragma unroll 1
-    for (int e = 0; e < 2; ++e) {
-      u64 sum = 0;
-      if (__any(n[e] != 0)) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float z = value_of<DT>(at + k);
-          const uint32_t below = w[k] >> 16;
-          sum += (e ? below : (w[k] & 0xFFFFu) - below) * m.weight(m.y(e ? -z : z));
-        }
-      }
-      x[e] = sum;
-    }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) n[e] = wave_scan_sum(n[e]), x[e] = wave_scan_sum(x[e]);
-    if (lane == kWave - 1) {
-      s.counts[kChunks / 2 - 1 - c] = n[0], s.sums[kChunks / 2 - 1 - c] = x[0];
-      s.counts[kChunks / 2 + c] = n[1], s.sums[kChunks / 2 + c] = x[1];
-    }
+    for (int e = 0; e < 2; ++e) n[e] = wave_scan_sum(n[e]);
+    if (lane == kWave - 1) s.counts[kChunks / 2 - 1 - c] = n[0], s.counts[kChunks / 2 + c] = n[1];
   }
   counted = wave_sum(counted);
   bad = __any(bad);
@@ -859,21 +845,51 @@ __global__ __launch_bounds__(kThreads16) void sample16_kernel(SampleArgs a) {
     const int32_t first = top < 0.0f ? kMagnitudes + int32_t(magnitude) : kMagnitudes - 1 - int32_t(magnitude);
     const bool whole = want.temp > 0.0 && want.top_k == 0 && want.top_p >= 1.0f && want.min_p <= 0.0;
     if (want.temp > 0.0 && (Draw || !whole)) {
+      // the last position that min-p keeps
+      int32_t likely = kChunks * kChunk - 1;
+      if (want.min_p > 0.0) {
+        const double least = want.temp * log(want.min_p);
+        int32_t out = kMagnitudes + int32_t(Half<DT>::inf);
+        likely = first;
+        while (out - likely > 1) {
+          const int32_t mid = (likely + out) / 2;
+          if (double(value_at<DT>(mid)) - m.top >= least) likely = mid;
+          else out = mid;
+        }
+      }
+      // Sums of the chunks, dealt to the waves in turn: of those that hold the
+      // first top_k tokens, or what min-p keeps (top-p is a share of more than that).
+      const uint4 four = *reinterpret_cast<const uint4*>(s.counts + 4 * lane);
+      const uint32_t here[4] = {four.x, four.y, four.z, four.w};
+      int32_t last_chunk = want.top_p < 1.0f ? kChunks - 1 : likely / kChunk;
+      if (want.top_k > 0) {
+        const uint32_t own = (here[0] + here[1]) + (here[2] + here[3]), upto = wave_scan_sum(own);
+        const uint64_t past = __ballot(int64_t(upto) >= want.top_k);
+        if (past) last_chunk = min(last_chunk, 4 * __builtin_ctzll(past) + 3);
+      }
+      uint32_t turn = 0;
+#pragma unroll 1
+      for (int k = 0; k < 4; ++k) {
+        uint64_t chunks = __ballot((k == 0 ? here[0] : k == 1 ? here[1] : k == 2 ? here[2] : here[3]) != 0);
+        while (chunks) {
+          const int32_t o = 4 * __builtin_ctzll(chunks) + k;
+          chunks &= chunks - 1;
+          if (o > last_chunk) break;
+          if (turn++ % kWaves16 != uint32_t(wave)) continue;
+          uint32_t n[4];
+          u64 w[4];
+          chunk_positions<DT>(s, m, o, lane, n, w);
+          const u64 sum = wave_scan_sum((n[0] * w[0] + n[1] * w[1]) + (n[2] * w[2] + n[3] * w[3]));
+          if (lane == kWave - 1) s.sums[o] = sum;
+        }
+      }
+      __syncthreads();
       if (wave == 0) {
         const Chunks<DT> chunks(s, m, lane);
         Place16 cut{kChunks * kChunk - 1, 0, chunks.sum()};
         if (want.top_k > 0 && want.top_k < int64_t(chunks.count())) cut = chunks.template find<true>(u64(want.top_k) - 1);
         if (want.top_p < 1.0f) cut = chunks.template find<false>(share_of(cut.sum, want.top_p, true));
-        if (want.min_p > 0.0) {
-          const double least = want.temp * log(want.min_p);
-          int32_t in = first, out = kMagnitudes + int32_t(Half<DT>::inf);
-          while (out - in > 1) {
-            const int32_t mid = (in + out) / 2;
-            if (double(value_at<DT>(mid)) - m.top >= least) in = mid;
-            else out = mid;
-          }
-          if (in < cut.position) cut = Place16{in, 0, chunks.sum_upto(in)};
-        }
+        if (likely < cut.position) cut = Place16{likely, 0, chunks.sum_upto(likely)};
         if (Draw) {
           const float u = a.uniforms[b];
           u64 target = u < 1.0f ? share_of(cut.sum, u, false) : cut.sum;
