@@ -41,22 +41,23 @@ struct AppendArgs {
 
 // A token's rows of the rotation's tables, by axis.
 struct Turns {
-  int32_t at[BPD_MAX_AXES];
+  int32_t first, second, third, fourth;
 };
-__host__ __device__ __forceinline__ int32_t turn_on(const Turns& t, int32_t axis) {
-  int32_t x = t.at[0];
-  for (int k = 1; k < BPD_MAX_AXES; ++k) x = axis >= k ? t.at[k] : x;  // an axis past the last is read as it
-  return x;
+static_assert(BPD_MAX_AXES == 4, "as many as Turns holds");
+// (an axis past the last is read as it, one below 0 as the first)
+__host__ __device__ __forceinline__ int32_t turn_on(Turns t, int32_t axis) {
+  // (sums: a choice between places to read from would put them into memory)
+  return t.first + (axis > 0 ? t.second - t.first : 0) + (axis > 1 ? t.third - t.second : 0) +
+         (axis > 2 ? t.fourth - t.third : 0);
 }
 // False where one lies outside the tables.
 __host__ __device__ __forceinline__ bool turns_of(const AppendArgs& a, int64_t b, int32_t i, Turns* t) {
-  bool ok = true;
-  for (int k = 0; k < BPD_MAX_AXES; ++k) {
-    const int32_t last = a.num_axes - 1, axis = k < last ? k : last;
-    t->at[k] = a.places[axis * a.place_axis + b * a.place_row + i * a.place_token];
-    ok = ok && t->at[k] >= 0 && t->at[k] < a.positions;
-  }
-  return ok;
+  const int32_t* place = a.places + b * a.place_row + i * a.place_token;
+  const int32_t last = a.num_axes - 1;
+  const auto at = [&](int32_t k) { return place[(k < last ? k : last) * a.place_axis]; };
+  *t = Turns{at(0), at(1), at(2), at(3)};
+  const auto in = [&](int32_t x) { return x >= 0 && x < a.positions; };
+  return bool(int(in(t->first)) & int(in(t->second)) & int(in(t->third)) & int(in(t->fourth)));
 }
 
 // The axis of a pair; one that is not there is flagged.
@@ -74,15 +75,14 @@ __host__ __device__ __forceinline__ int32_t axis_of(const AppendArgs& a, int32_t
 
 // Whether token i of request b is appended, and where; sets *bad where it
 // should be and cannot.  *turn: its row of the rotation's tables (without axes
-// of its own), or -1.
-__host__ __device__ __forceinline__ int64_t append_place(const AppendArgs& a, int64_t b, int32_t i, int64_t* pos,
-                                                         int64_t* turn, bool* bad) {
+// of its own), or -1.  on_axes: whether the positions on axes are in the tables.
+__host__ __device__ __forceinline__ int64_t append_place(const AppendArgs& a, int64_t b, int32_t i, int32_t start,
+                                                         bool on_axes, int64_t* pos, int64_t* turn, bool* bad) {
   *bad = false;
   *turn = -1;
   if (a.counts && i >= a.counts[b]) return -1;
-  *pos = int64_t(a.starts[b]) + i;
-  Turns t;
-  if (*pos < 0 || (a.num_axes > 0 ? !turns_of(a, b, i, &t) : a.rotary > 0 && *pos >= a.positions)) {
+  *pos = int64_t(start) + i;
+  if (*pos < 0 || (a.num_axes > 0 ? !on_axes : a.rotary > 0 && *pos >= a.positions)) {
     *bad = true;
     return -1;
   }
@@ -142,6 +142,17 @@ __global__ __launch_bounds__(kKvThreads) void kv_append_kernel(AppendArgs a, uin
   const bool rotated = d0 < a.rotary;
   const bool upper = rotated && d0 >= half;
 
+  // the axes of the thread's pairs, on their way first
+  constexpr int kPairs = Mode == kHalves ? kKvWidth : kKvWidth / 2;
+  const int32_t pair = Mode == kNeighbours ? d0 / 2 : upper ? d0 - half : d0;
+  Turns own{};
+  bool on_axes = false;
+  int32_t axis[kPairs] = {};
+  if constexpr (Axes) {
+    if (Mode != kAnywhere && rotated && a.axes)
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) axis[j] = a.axes[pair + j];
+  }
   const uint16_t* qs = a.q + b * a.qs.row + i * a.qs.token;
   const uint16_t* ks = a.k + b * a.ks.row + i * a.ks.token;
   const uint16_t* vs = a.v + b * a.vs.row + i * a.vs.token;
@@ -160,24 +171,23 @@ __global__ __launch_bounds__(kKvThreads) void kv_append_kernel(AppendArgs a, uin
     if (Mode == kHalves && rotated && kind[p] != 2)
       partner[p] = *reinterpret_cast<const words4*>(upper ? from - half : from + half);
   }
+  const int32_t start = a.starts[b];
+  if constexpr (Axes) on_axes = turns_of(a, b, i, &own);
   int64_t pos, turn;
   bool bad;
-  const int64_t page = append_place(a, b, i, &pos, &turn, &bad);
+  const int64_t page = append_place(a, b, i, start, on_axes, &pos, &turn, &bad);
   if (bad && a.err && tid == 0 && part == 0) atomicOr(a.err, BPD_FLAG_PAGE_RANGE);
   const bool turns = rotated && turn >= 0;
   float c[kKvWidth], sn[kKvWidth];
-  Turns own{};
-  if (Axes && turns) turns_of(a, b, i, &own);
   bool apart = false;  // the pairs lie on several axes
   if (Axes && Mode != kAnywhere && turns) {
-    constexpr int kPairs = Mode == kHalves ? kKvWidth : kKvWidth / 2;
-    const int32_t pair = Mode == kNeighbours ? d0 / 2 : upper ? d0 - half : d0;
-    int32_t axis[kPairs];
+    bool outside = false;
 #pragma unroll
     for (int j = 0; j < kPairs; ++j) {
-      axis[j] = axis_of(a, pair + j);
       apart |= axis[j] != axis[0];
+      outside |= axis[j] < 0 || axis[j] >= a.num_axes;
     }
+    if (outside && a.err) atomicOr(a.err, BPD_FLAG_PAGE_RANGE);
     turn = turn_on(own, axis[0]);
     if (apart) {
 #pragma unroll
@@ -188,7 +198,7 @@ __global__ __launch_bounds__(kKvThreads) void kv_append_kernel(AppendArgs a, uin
     }
   }
   if (Mode != kAnywhere && turns && !apart) {
-    const int64_t at = turn * half + (Mode == kNeighbours ? d0 / 2 : upper ? d0 - half : d0);
+    const int64_t at = turn * half + pair;
 #pragma unroll
     for (int k = 0; k < (Mode == kHalves ? 2 : 1); ++k) {
       const floats4 y = *reinterpret_cast<const floats4*>(a.cos + at + 4 * k), z = *reinterpret_cast<const floats4*>(a.sin + at + 4 * k);
@@ -263,10 +273,10 @@ void host_append(const AppendArgs& a) {
     for (int32_t i = 0; i < a.tokens; ++i) {
       int64_t pos, turn;
       bool bad;
-      const int64_t page = append_place(a, b, i, &pos, &turn, &bad);
-      if (bad && a.err) *a.err |= BPD_FLAG_PAGE_RANGE;
       Turns own{};
-      if (turn >= 0 && a.num_axes > 0) turns_of(a, b, i, &own);
+      const bool on_axes = a.num_axes > 0 && turns_of(a, b, i, &own);
+      const int64_t page = append_place(a, b, i, a.starts[b], on_axes, &pos, &turn, &bad);
+      if (bad && a.err) *a.err |= BPD_FLAG_PAGE_RANGE;
       const auto angle = [&](int32_t pair, float* c, float* s) {
         const int64_t at = (a.num_axes > 0 ? turn_on(own, axis_of(a, pair)) : turn) * (a.rotary / 2) + pair;
         *c = a.cos[at], *s = a.sin[at];
