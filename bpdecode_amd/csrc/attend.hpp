@@ -221,37 +221,29 @@ __device__ __forceinline__ void store_columns(uint16_t* out, int v, int g, const
     }
 }
 
-// The prefix's part of a column (at `column` of key head `kvh`) into N of its
-// value tiles from v on, its exponent and its sum.
-template <int D, int N>
-__device__ __forceinline__ void take_prefix(const Prefix& px, const AttendArgs& a, int32_t kvh, int64_t column, int v, int g,
-                                            float* top, float* sum, f32x4* x) {
+// A chunk of the prefix's sums for a lane's column (at `at`; in: there is one)
+// into what the lane has accumulated: its value tiles as a product leaves them,
+// the sum of weights on the first of the column's four lanes.
+template <int D>
+__device__ __forceinline__ void take_chunk(const Prefix& px, int64_t at, bool in, int g, float* top, float* sum, f32x4* acc) {
   constexpr int VT = D / 16;
-  const int64_t step = int64_t(a.kv_heads) * px.columns, at = int64_t(kvh) * px.columns + column;
-  float now = *top;
-  for (int32_t s = 0; s < px.chunks; ++s) now = fmaxf(now, px.stats[s * step + at].x);
-  const float keep = __builtin_amdgcn_exp2f(*top - now);
-  *top = now;
-  *sum *= keep;
+  float2 st = {-3e38f, 0.0f};
+  f32x4 y[VT];
+  if (in) {
+    st = px.stats[at];
+    const f32x4* from = reinterpret_cast<const f32x4*>(px.values + at * D) + g * VT;
 #pragma unroll
-  for (int k = 0; k < N; ++k)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[k][i] *= keep;
-#pragma unroll 4
-  for (int32_t s = 0; s < px.chunks; ++s) {
-    const float2 st = px.stats[s * step + at];
-    if (st.y == 0.0f) continue;  // no token: nothing was written
-    const float f = __builtin_amdgcn_exp2f(st.x - now);
-    *sum += st.y * f;
-    const f32x4* from = reinterpret_cast<const f32x4*>(px.values + (s * step + at) * D) + g * VT + v;
-#pragma unroll
-    for (int k = 0; k < N; ++k)
-      if (v + k < VT) {
-        const f32x4 y = from[k];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[k][i] += y[i] * f;
-      }
+    for (int v = 0; v < VT; ++v) y[v] = from[v];
   }
+  const bool some = in && st.y != 0.0f;  // else nothing was written
+  const float now = some ? fmaxf(*top, st.x) : *top;
+  const float keep = __builtin_amdgcn_exp2f(*top - now), f = some ? __builtin_amdgcn_exp2f(st.x - now) : 0.0f;
+  *top = now;
+  *sum = *sum * keep + (some && g == 0 ? st.y * f : 0.0f);
+#pragma unroll
+  for (int v = 0; v < VT; ++v)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[v][i] = acc[v][i] * keep + (some ? y[v][i] * f : 0.0f);
 }
 
 // Blocks that a CU is to hold, by registers (a block puts one wave on each SIMD).
@@ -466,6 +458,20 @@ __global__ __launch_bounds__(W* kWave, W == kWaves ? attend_blocks(D, NT) : 1) v
 #pragma unroll
       for (int v = 0; v < VT; ++v) acc[t][v] = f32x4{0, 0, 0, 0};
     }
+    // the prefix's chunks, dealt to the waves of the block that begins the unit
+    if constexpr (kShared) {
+      if (base > 0 && tile0 == 0) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const int32_t c = group * plan.cols + t * 16 + qm;
+          const bool in = t * 16 + qm < plan.cols && c / share < n_q;
+          const int64_t step = int64_t(a.kv_heads) * px.columns;
+          const int64_t at = int64_t(kvh) * px.columns + b * (a.tokens * share) + c;
+#pragma unroll 1
+          for (int32_t k = wave; k < px.chunks; k += W) take_chunk<D>(px, k * step + at, in, g, &top[t], &sum[t], acc[t]);
+        }
+      }
+    }
     int32_t nan_at[Pt::count];  // first token of the tail whose value group is bad, as a value lane
 #pragma unroll
     for (int p = 0; p < Pt::count; ++p) nan_at[p] = kNever;
@@ -676,9 +682,6 @@ __global__ __launch_bounds__(W* kWave, W == kWaves ? attend_blocks(D, NT) : 1) v
           const int32_t c = group * plan.cols + column;
           const int32_t i = c / share, h = kvh * share + c % share;
           if (column >= plan.cols || i >= a.tokens) continue;
-          if constexpr (kShared) {
-            if (base > 0) take_prefix<D, kMine>(px, a, kvh, b * (a.tokens * share) + c, v, el >> 4, &now, &whole, mine);
-          }
           // a row past the request's queries has summed what no mask kept out
           if (i >= n_q)
 #pragma unroll
@@ -788,10 +791,6 @@ __global__ __launch_bounds__(W* kWave) void kv_attend_join_kernel(AttendArgs a, 
   const int32_t c = unit % plan.groups * plan.cols + column;
   const int32_t i = c / share, h = unit / plan.groups * share + c % share;
   if (column >= plan.cols || i >= a.tokens) return;
-  if constexpr (std::is_same<Px, Prefix>::value) {
-    if (begin_of(a, sp, b) > 0)
-      take_prefix<D, 2>(px, a, unit / plan.groups, b * (a.tokens * share) + c, v0, lane >> 4, &now, &sum, acc);
-  }
   const bool none = i >= queries_of(a, b);
   if (none) acc[0] = acc[1] = f32x4{0, 0, 0, 0};
   store_columns<DT, D, 2>(a.out + ((b * a.tokens + i) * a.heads + h) * D, v0, lane >> 4, acc,
