@@ -90,7 +90,8 @@ __host__ __device__ __forceinline__ void store_drawn(const SampleArgs& a, int64_
 // where a row's 10^5 borders want 10^-12 of its sum.
 typedef unsigned long long u64;
 
-constexpr int kBins = 4096;
+constexpr int kBins = 8192, kSubBins = 2048;  // of the first table, and of a part of one bin of it
+constexpr int kListed = 512;                  // tokens of a bin that are put in order
 constexpr int kMostScale = 50;  // a weight is read off the bits of its sum with 2^52
 
 // Bits of a weight: the sum of a row's fits 63.
@@ -134,20 +135,32 @@ struct Measure {
 };
 
 // A first part of the order: all tokens with larger keys, and the first `rank`
-// of those with this one.
+// of those with this one, the last of them at `last` (-1: not yet known).
 struct Cut {
   uint32_t key;
   u64 rank, sum;  // sum: of its weights
+  int64_t last;
 };
 
+template <int Bins>
 struct Table {
-  u64 sums[kBins];
-  uint32_t counts[kBins];
+  u64 sums[Bins];
+  uint32_t counts[Bins];
+};
+struct Listed {
+  u64 place;  // larger for one that stands before: its key and its index, the other way round
+  u64 weight;
 };
 template <int N>  // threads
 struct Scratch {
-  static constexpr int waves = N / kWave, step = N * kRun;  // tokens that a block reads at a time
-  Table first, sub;  // by weight, and of a part of one bin of it by key
+  static constexpr int waves = N / kWave;
+  Table<kBins> first;  // by weight
+  union {
+    Table<kSubBins> sub;  // by key
+    Listed list[kListed];
+  };
+  uint32_t listed;
+  Cut hit;
   u64 sums[waves], counts[waves];
   u64 hit_count, hit_sum;
   int64_t found;
@@ -155,23 +168,24 @@ struct Scratch {
   int32_t bad[waves], hit_bin;
 };
 
-template <int N>
-__device__ __forceinline__ void clear(Table& t) {
-  for (int i = threadIdx.x; i < kBins; i += N) t.sums[i] = 0, t.counts[i] = 0;
+template <int N, int Bins>
+__device__ __forceinline__ void clear(Table<Bins>& t) {
+  for (int i = threadIdx.x; i < Bins; i += N) t.sums[i] = 0, t.counts[i] = 0;
 }
 
 // The bin in which the running count or sum passes `target` (less than the
 // whole); *count and *sum become what lies before it.
-template <int N>
-__device__ __forceinline__ int32_t find_bin(const Table& t, u64 target, bool by_count, u64* count, u64* sum, Scratch<N>& s) {
-  constexpr int kMine = kBins / N;
+template <int N, int Bins>
+__device__ __forceinline__ int32_t find_bin(const Table<Bins>& t, u64 target, bool by_count, u64* count, u64* sum,
+                                            Scratch<N>& s) {
+  constexpr int kMine = Bins / N;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   u64 c = 0, x = 0;
 #pragma unroll
   for (int k = 0; k < kMine; ++k) c += t.counts[tid * kMine + k], x += t.sums[tid * kMine + k];
   u64 upto_c = wave_scan_sum(c), upto_x = wave_scan_sum(x);
   if (lane == kWave - 1) s.counts[wave] = upto_c, s.sums[wave] = upto_x;
-  if (tid == 0) s.hit_bin = kBins - 1, s.hit_count = s.hit_sum = 0;
+  if (tid == 0) s.hit_bin = Bins - 1, s.hit_count = s.hit_sum = 0;
   __syncthreads();
   for (int k = 0; k < wave; ++k) upto_c += s.counts[k], upto_x += s.sums[k];
   c = upto_c - c, x = upto_x - x;
@@ -198,16 +212,29 @@ __device__ __forceinline__ int32_t find_bin(const Table& t, u64 target, bool by_
 // are the thread's own, allowed and not -inf.
 template <int DT, class F>
 __device__ __forceinline__ void each_run(const Row& r, int64_t first, int64_t end, int64_t step, F f) {
+  constexpr int kAtOnce = 2;  // runs on their way together
 #pragma unroll 1
-  for (int64_t t = first; t < end; t += step) {
-    const Run run = run_at(t, r.vocab);
-    uint32_t valid = run_bits(r, run);
-    float z[kRun];
-    load_run<DT>(r.logits, run, r.vocab, z);
+  for (int64_t t0 = first; t0 < end; t0 += kAtOnce * step) {
+    Raw<DT> raw[kAtOnce];
+    uint32_t valid[kAtOnce];
+    int64_t at[kAtOnce];
 #pragma unroll
-    for (int j = 0; j < kRun; ++j)
-      if (z[j] == -INFINITY) valid &= ~(1u << j);
-    f(z, valid, run.t);
+    for (int k = 0; k < kAtOnce; ++k) {
+      const Run run = run_at(t0 + k * step, r.vocab);  // (past the row: none of its own)
+      const bool in = t0 + k * step < end;
+      raw[k] = load_raw<DT>(r.logits, run, r.vocab);
+      valid[k] = in ? run_bits(r, run) : 0u;
+      at[k] = run.t;
+    }
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      float z[kRun];
+      unpack<DT>(raw[k], z);
+#pragma unroll
+      for (int j = 0; j < kRun; ++j)
+        if (z[j] == -INFINITY) valid[k] &= ~(1u << j);
+      f(z, valid[k], at[k]);
+    }
   }
 }
 
@@ -237,10 +264,11 @@ __device__ __forceinline__ int64_t nth_token(const Row& r, uint32_t key, u64 ran
   for (; hit < kWaves - 1 && before + s.counts[hit] < rank; ++hit) before += s.counts[hit];
   if (wave == hit) {
     for (int64_t t0 = begin; t0 < end; t0 += kWave * kRun) {
-      uint32_t m = 0;
-      int64_t at = 0;
-      each_run<DT>(r, t0 + lane * kRun, t0 + lane * kRun + 1 < end ? t0 + lane * kRun + 1 : end, kWave * kRun,
-                   [&](const float(&z)[kRun], uint32_t valid, int64_t t) { m = same(z, valid), at = t; });
+      const Run run = run_at(t0 + lane * kRun, r.vocab);
+      const int64_t at = run.t;
+      float z[kRun];
+      load_run<DT>(r.logits, run, r.vocab, z);
+      uint32_t m = t0 + lane * kRun < end ? same(z, run_bits(r, run)) : 0u;
       const u64 upto = before + wave_scan_sum(u64(__popc(m)));
       if (upto >= rank && upto - __popc(m) < rank) {
         for (u64 k = upto - __popc(m) + 1; k < rank; ++k) m &= m - 1;
@@ -286,6 +314,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const Row& r, co
       top = fmaxf(top, z[j]);
     }
   });
+  const float own = top;  // the thread's
   top = wave_max(top);
   bad = __any(bad);
   if (lane == 0) s.tops[wave] = top, s.bad[wave] = bad;
@@ -297,27 +326,67 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const Row& r, co
   *logprob = -INFINITY;
   if (bad || top == -INFINITY) return;
   const uint32_t top_key = key_of(top);
-  Cut cut{top_key, 1, 1};
+  Cut cut{top_key, 1, 1, -1};
   Measure m{double(top), want.temp > 0.0 ? kLog2E / want.temp : 0.0, 0.0, scale_of(r.vocab)};
   m.bins = double(kBins) / (m.scale + 2);
   const bool whole = want.temp > 0.0 && want.top_k == 0 && want.top_p >= 1.0f && want.min_p <= 0.0;
   if (!draw && whole) {
     cut.key = cut.rank = 0;
   } else if (want.temp > 0.0) {
+    // keys that bin i can hold, generously
+    const auto keys_of = [&](int32_t i, uint32_t* lo, uint32_t* hi) {
+      const double per = m.bins * m.to_log2;
+      const double from = m.top - i / per, to = m.top - (i + 1) / per;
+      const double off = fabs(m.top) * 0x1p-50 + (m.top - to) * 0x1p-50;
+      *hi = top_key, *lo = key_of(-3.402823466e38f);
+      if (from + off < m.top) *hi = min(*hi, key_of(float(from + off)) + 2);
+      if (i < kBins - 1 && to - off > -3.4e38) *lo = max(*lo, key_of(float(to - off)) - 2);
+    };
+    // the least key that min-p keeps
+    uint32_t likely = 0;
+    if (want.min_p > 0.0) {
+      const double least = want.temp * log(want.min_p);
+      uint32_t out = 0;
+      likely = top_key;
+      while (likely - out > 1) {
+        const uint32_t mid = out + (likely - out) / 2;
+        if (mid > 0x007FFFFFu && double(logit_of(mid)) - m.top >= least) likely = mid;
+        else out = mid;
+      }
+    }
+    // What lies below `from` is not needed: min-p's border, where top-p does not
+    // want the sum of more, and the bin that holds the k-th of the threads'
+    // largest logits, which is not before that of the k-th of all.
+    uint32_t from = want.top_p < 1.0f ? 0 : likely;
     clear<N>(s.first);
     __syncthreads();
+    if (want.top_k > 0 && want.top_k <= N) {
+      if (own > -INFINITY) atomicAdd(&s.first.counts[m.bin(m.y(own))], 1u);
+      __syncthreads();
+      u64 c, x;
+      const int32_t i = find_bin(s.first, u64(want.top_k) - 1, true, &c, &x, s);
+      if (c < u64(want.top_k) && c + s.first.counts[i] >= u64(want.top_k)) {
+        uint32_t lo, hi;
+        keys_of(i, &lo, &hi);
+        from = max(from, lo);
+      }
+      __syncthreads();
+      clear<N>(s.first);
+      __syncthreads();
+    }
+    const float floor_z = from > 0x007FFFFFu ? logit_of(from) : -INFINITY;
     each_run<DT>(r, tid * kRun, r.vocab, kStep, [&](const float(&z)[kRun], uint32_t valid, int64_t) {
 #pragma unroll
       for (int j = 0; j < kRun; ++j) {
-        if (!(valid >> j & 1)) continue;
+        if (!(valid >> j & 1) || z[j] < floor_z) continue;
         const double y = m.y(z[j]);
         const int32_t i = m.bin(y);
-        atomicAdd(&s.first.counts[i], 1u);
+        if (want.top_k > 0) atomicAdd(&s.first.counts[i], 1u);
         atomicAdd(&s.first.sums[i], m.weight(y));
       }
     });
     __syncthreads();
-    // all of the row
+    // all of them
     u64 count = 0, sum = 0;
     {
       u64 c = 0, x = 0;
@@ -328,21 +397,56 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const Row& r, co
       for (int k = 0; k < kWaves; ++k) count += s.counts[k], sum += s.sums[k];
       __syncthreads();
     }
-    cut = Cut{0, 0, sum};
+    // (all that min-p keeps, or all of the row)
+    cut = want.top_p < 1.0f || likely == 0 ? Cut{0, 0, sum, -1} : Cut{likely - 1, 0, sum, -1};
     // the first part of the order that ends where the running count or sum passes `target`
     const auto select = [&](u64 target, bool by_count) {
       u64 c, x;
       const int32_t bin = find_bin(s.first, target, by_count, &c, &x, s);
-      // keys that the bin can hold, generously
-      const double per = m.bins * m.to_log2, slack = fabs(m.top) * 0x1p-50;
-      const double from = m.top - bin / per, to = m.top - (bin + 1) / per;
-      const double off = slack + (m.top - to) * 0x1p-50;
-      uint32_t hi = top_key, lo = key_of(-3.402823466e38f);
-      if (from + off < m.top) hi = min(hi, key_of(float(from + off)) + 2);
-      if (bin < kBins - 1 && to - off > -3.4e38) lo = max(lo, key_of(float(to - off)) - 2);
+      uint32_t lo, hi;
+      keys_of(bin, &lo, &hi);
+      lo = max(lo, from);
+      // the bin's tokens, put in order where they are few
+      const float least = logit_of(lo), most = logit_of(hi);
+      if (tid == 0) s.listed = 0;
+      __syncthreads();
+      each_run<DT>(r, tid * kRun, r.vocab, kStep, [&](const float(&z)[kRun], uint32_t valid, int64_t t) {
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) {
+          if (!(valid >> j & 1) || !(z[j] >= least && z[j] <= most)) continue;
+          const double y = m.y(z[j]);
+          if (m.bin(y) != bin) continue;
+          const uint32_t at = atomicAdd(&s.listed, 1u);
+          if (at < kListed) s.list[at] = Listed{u64(key_of(z[j])) << 32 | uint32_t(~uint32_t(t + j)), m.weight(y)};
+        }
+      });
+      __syncthreads();
+      const uint32_t listed = s.listed;
+      if (listed <= uint32_t(kListed)) {
+        if (tid == 0) s.hit = Cut{hi, 1, x + 1, -1};
+        __syncthreads();
+        for (uint32_t i = tid; i < listed; i += N) {
+          const Listed mine = s.list[i];
+          u64 bc = c, bx = x, rank = 1;
+#pragma unroll 4
+          for (uint32_t e = 0; e < listed; ++e) {
+            const Listed other = s.list[e];
+            const bool before = other.place > mine.place;
+            bc += before, bx += before ? other.weight : 0;
+            rank += before && (other.place ^ mine.place) >> 32 == 0;
+          }
+          if (by_count ? bc == target : bx <= target && target < bx + mine.weight)
+            s.hit = Cut{uint32_t(mine.place >> 32), rank, bx + mine.weight, int64_t(uint32_t(~uint32_t(mine.place)))};
+        }
+        __syncthreads();
+        const Cut found = s.hit;
+        __syncthreads();
+        return found;
+      }
       for (;;) {
         const uint32_t range = hi - lo;
-        const int shift = range < uint32_t(kBins) ? 0 : 32 - __builtin_clz(range) - __builtin_ctz(uint32_t(kBins));
+        const int shift = range < uint32_t(kSubBins) ? 0 : 32 - __builtin_clz(range) - __builtin_ctz(uint32_t(kSubBins));
+        __syncthreads();
         clear<N>(s.sub);
         __syncthreads();
         each_run<DT>(r, tid * kRun, r.vocab, kStep, [&](const float(&z)[kRun], uint32_t valid, int64_t) {
@@ -366,33 +470,24 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const Row& r, co
       }
       const u64 w = m.weight(m.y(logit_of(hi)));
       const u64 rank = by_count ? target - c + 1 : (target - x) / w + 1;
-      return Cut{hi, rank, x + rank * w};
+      return Cut{hi, rank, x + rank * w, -1};
     };
-    if (want.top_k > 0 && u64(want.top_k) < count) cut = select(u64(want.top_k) - 1, true);
+    if (want.top_k > 0 && u64(want.top_k) <= count) cut = select(u64(want.top_k) - 1, true);
     if (want.top_p < 1.0f) cut = select(share_of(cut.sum, want.top_p, true), false);
-    if (want.min_p > 0.0) {
-      // the least key that min-p keeps
-      const double least = want.temp * log(want.min_p);
-      uint32_t lo = 0, hi = top_key;  // lo is not kept, hi is
-      while (hi - lo > 1) {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        if (mid > 0x007FFFFFu && double(logit_of(mid)) - m.top >= least) hi = mid;
-        else lo = mid;
-      }
-      if (hi > cut.key) {
-        u64 x = 0;
-        each_run<DT>(r, tid * kRun, r.vocab, kStep, [&](const float(&z)[kRun], uint32_t valid, int64_t) {
+    if (likely > cut.key && !(cut.rank == 0 && cut.key == likely - 1)) {
+      // (behind top-p: its sum is not known yet)
+      u64 x = 0;
+      each_run<DT>(r, tid * kRun, r.vocab, kStep, [&](const float(&z)[kRun], uint32_t valid, int64_t) {
 #pragma unroll
-          for (int j = 0; j < kRun; ++j)
-            if ((valid >> j & 1) && key_of(z[j]) >= hi) x += m.weight(m.y(z[j]));
-        });
-        x = wave_sum(x);
-        if (lane == 0) s.sums[wave] = x;
-        __syncthreads();
-        cut = Cut{hi - 1, 0, 0};
-        for (int k = 0; k < kWaves; ++k) cut.sum += s.sums[k];
-        __syncthreads();
-      }
+        for (int j = 0; j < kRun; ++j)
+          if ((valid >> j & 1) && key_of(z[j]) >= likely) x += m.weight(m.y(z[j]));
+      });
+      x = wave_sum(x);
+      if (lane == 0) s.sums[wave] = x;
+      __syncthreads();
+      cut = Cut{likely - 1, 0, 0, -1};
+      for (int k = 0; k < kWaves; ++k) cut.sum += s.sums[k];
+      __syncthreads();
     }
     if (draw) {
       const float u = a.uniforms[b];
@@ -406,7 +501,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const Row& r, co
     *logprob = 0.0f;
   }
   *cut_out = cut;
-  if (cut.rank > 0) *last_out = nth_token<DT, N>(r, cut.key, cut.rank, s);
+  if (cut.rank > 0) *last_out = cut.last >= 0 ? cut.last : nth_token<DT, N>(r, cut.key, cut.rank, s);
 }
 
 __device__ __forceinline__ Row row_of(const SampleArgs& a, int64_t b, int32_t* state, int32_t* flags) {
@@ -422,7 +517,7 @@ __device__ __forceinline__ Row row_of(const SampleArgs& a, int64_t b, int32_t* s
 template <int DT, bool Draw, int N>
 __device__ __forceinline__ void general_row(const SampleArgs& a, const Row& r, const Asked& want, int64_t b, int32_t state, int32_t flags,
                             Scratch<N>& s) {
-  Cut cut{0xFFFFFFFFu, 0, 0};
+  Cut cut{0xFFFFFFFFu, 0, 0, -1};
   int64_t last = -1;
   float logprob = -INFINITY;
   bool bad = false;
