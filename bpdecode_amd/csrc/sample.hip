@@ -173,23 +173,42 @@ __device__ __forceinline__ void clear(Table<Bins>& t) {
   for (int i = threadIdx.x; i < Bins; i += N) t.sums[i] = 0, t.counts[i] = 0;
 }
 
-// The bin in which the running count or sum passes `target` (less than the
-// whole); *count and *sum become what lies before it.
+// A thread's neighbouring bins: what lies before them, and with them.
+struct Span {
+  u64 count, count_end, sum, sum_end;
+};
+// *count and *sum become those of the whole table.
 template <int N, int Bins>
-__device__ __forceinline__ int32_t find_bin(const Table<Bins>& t, u64 target, bool by_count, u64* count, u64* sum,
-                                            Scratch<N>& s) {
-  constexpr int kMine = Bins / N;
+__device__ __forceinline__ Span span_of(const Table<Bins>& t, u64* count, u64* sum, Scratch<N>& s) {
+  constexpr int kMine = Bins / N, kWaves = N / kWave;
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   u64 c = 0, x = 0;
 #pragma unroll
   for (int k = 0; k < kMine; ++k) c += t.counts[tid * kMine + k], x += t.sums[tid * kMine + k];
-  u64 upto_c = wave_scan_sum(c), upto_x = wave_scan_sum(x);
-  if (lane == kWave - 1) s.counts[wave] = upto_c, s.sums[wave] = upto_x;
+  Span p{0, wave_scan_sum(c), 0, wave_scan_sum(x)};
+  if (lane == kWave - 1) s.counts[wave] = p.count_end, s.sums[wave] = p.sum_end;
+  __syncthreads();
+  *count = *sum = 0;
+#pragma unroll
+  for (int k = 0; k < kWaves; ++k) {
+    if (k == wave) p.count_end += *count, p.sum_end += *sum;
+    *count += s.counts[k], *sum += s.sums[k];
+  }
+  p.count = p.count_end - c, p.sum = p.sum_end - x;
+  __syncthreads();
+  return p;
+}
+// The bin in which the running count or sum passes `target` (less than the
+// whole); *count and *sum become what lies before it.
+template <int N, int Bins>
+__device__ __forceinline__ int32_t find_bin(const Table<Bins>& t, const Span& p, u64 target, bool by_count, u64* count,
+                                            u64* sum, Scratch<N>& s) {
+  constexpr int kMine = Bins / N;
+  const int tid = threadIdx.x;
   if (tid == 0) s.hit_bin = Bins - 1, s.hit_count = s.hit_sum = 0;
   __syncthreads();
-  for (int k = 0; k < wave; ++k) upto_c += s.counts[k], upto_x += s.sums[k];
-  c = upto_c - c, x = upto_x - x;
-  if ((by_count ? c <= target && target < upto_c : x <= target && target < upto_x)) {
+  if (by_count ? p.count <= target && target < p.count_end : p.sum <= target && target < p.sum_end) {
+    u64 c = p.count, x = p.sum;
 #pragma unroll 1
     for (int k = tid * kMine;; ++k) {
       const u64 nc = c + t.counts[k], nx = x + t.sums[k];
@@ -209,10 +228,9 @@ __device__ __forceinline__ int32_t find_bin(const Table<Bins>& t, u64 target, bo
 
 // f(z, valid, t) for the runs of tokens [begin, end) that threads take from
 // `first` on, `step` tokens apart: t is the token of z[0], `valid` says which
-// are the thread's own, allowed and not -inf.
-template <int DT, class F>
+// are the thread's own and allowed.
+template <int DT, int kAtOnce, class F>  // runs on their way together
 __device__ __forceinline__ void each_run(const Row& r, int64_t first, int64_t end, int64_t step, F f) {
-  constexpr int kAtOnce = 2;  // runs on their way together
 #pragma unroll 1
   for (int64_t t0 = first; t0 < end; t0 += kAtOnce * step) {
     Raw<DT> raw[kAtOnce];
@@ -230,9 +248,6 @@ __device__ __forceinline__ void each_run(const Row& r, int64_t first, int64_t en
     for (int k = 0; k < kAtOnce; ++k) {
       float z[kRun];
       unpack<DT>(raw[k], z);
-#pragma unroll
-      for (int j = 0; j < kRun; ++j)
-        if (z[j] == -INFINITY) valid[k] &= ~(1u << j);
       f(z, valid[k], at[k]);
     }
   }
@@ -253,7 +268,7 @@ __device__ __forceinline__ int64_t nth_token(const Row& r, uint32_t key, u64 ran
     return m & valid;
   };
   u64 n = 0;
-  each_run<DT>(r, begin + lane * kRun, end, kWave * kRun,
+  each_run<DT, 4>(r, begin + lane * kRun, end, kWave * kRun,
                [&](const float(&z)[kRun], uint32_t valid, int64_t) { n += __popc(same(z, valid)); });
   n = wave_sum(n);
   if (lane == 0) s.counts[wave] = n;
@@ -306,12 +321,16 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const Row& r, co
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   float top = -INFINITY;
   bool bad = false;
-  each_run<DT>(r, tid * kRun, r.vocab, kStep, [&](const float(&z)[kRun], uint32_t valid, int64_t) {
+  each_run<DT, 4>(r, tid * kRun, r.vocab, kStep, [&](const float(&z)[kRun], uint32_t valid, int64_t) {
+    if (__all(valid == 0xFFu)) {
 #pragma unroll
-    for (int j = 0; j < kRun; ++j) {
-      if (!(valid >> j & 1)) continue;
-      bad |= !(z[j] < INFINITY);
-      top = fmaxf(top, z[j]);
+      for (int j = 0; j < kRun; ++j) bad |= !(z[j] < INFINITY), top = fmaxf(top, z[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kRun; ++j) {
+        const float x = valid >> j & 1 ? z[j] : -INFINITY;
+        bad |= !(x < INFINITY), top = fmaxf(top, x);
+      }
     }
   });
   const float own = top;  // the thread's
@@ -364,7 +383,8 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const Row& r, co
       if (own > -INFINITY) atomicAdd(&s.first.counts[m.bin(m.y(own))], 1u);
       __syncthreads();
       u64 c, x;
-      const int32_t i = find_bin(s.first, u64(want.top_k) - 1, true, &c, &x, s);
+      const Span span = span_of(s.first, &c, &x, s);
+      const int32_t i = find_bin(s.first, span, u64(want.top_k) - 1, true, &c, &x, s);
       if (c < u64(want.top_k) && c + s.first.counts[i] >= u64(want.top_k)) {
         uint32_t lo, hi;
         keys_of(i, &lo, &hi);
@@ -374,50 +394,58 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const Row& r, co
       clear<N>(s.first);
       __syncthreads();
     }
-    const float floor_z = from > 0x007FFFFFu ? logit_of(from) : -INFINITY;
-    each_run<DT>(r, tid * kRun, r.vocab, kStep, [&](const float(&z)[kRun], uint32_t valid, int64_t) {
-#pragma unroll
-      for (int j = 0; j < kRun; ++j) {
-        if (!(valid >> j & 1) || z[j] < floor_z) continue;
-        const double y = m.y(z[j]);
+    const float floor_z = from > 0x007FFFFFu ? logit_of(from) : -3.402823466e38f;  // (-inf lies below)
+    const bool counts = want.top_k > 0;
+    each_run<DT, 2>(r, tid * kRun, r.vocab, kStep, [&](const float(&z)[kRun], uint32_t valid, int64_t) {
+      const auto add = [&](float x) {
+        const double y = m.y(x);
         const int32_t i = m.bin(y);
-        if (want.top_k > 0) atomicAdd(&s.first.counts[i], 1u);
+        if (counts) atomicAdd(&s.first.counts[i], 1u);
         atomicAdd(&s.first.sums[i], m.weight(y));
+      };
+#pragma unroll
+      for (int j = 0; j < kRun; ++j)
+        if (z[j] < floor_z) valid &= ~(1u << j);
+      if (__all(valid == 0xFFu)) {  // (no branches: the exponentials of eight tokens interleave)
+#pragma unroll
+        for (int j = 0; j < kRun; ++j) add(z[j]);
+      } else if (__any(valid != 0)) {
+#pragma unroll
+        for (int j = 0; j < kRun; ++j)
+          if (valid >> j & 1) add(z[j]);
       }
     });
     __syncthreads();
-    // all of them
-    u64 count = 0, sum = 0;
-    {
-      u64 c = 0, x = 0;
-      for (int i = tid; i < kBins; i += N) c += s.first.counts[i], x += s.first.sums[i];
-      c = wave_sum(c), x = wave_sum(x);
-      if (lane == 0) s.counts[wave] = c, s.sums[wave] = x;
-      __syncthreads();
-      for (int k = 0; k < kWaves; ++k) count += s.counts[k], sum += s.sums[k];
-      __syncthreads();
-    }
+    u64 count, sum;
+    const Span span = span_of(s.first, &count, &sum, s);
     // (all that min-p keeps, or all of the row)
     cut = want.top_p < 1.0f || likely == 0 ? Cut{0, 0, sum, -1} : Cut{likely - 1, 0, sum, -1};
     // the first part of the order that ends where the running count or sum passes `target`
     const auto select = [&](u64 target, bool by_count) {
       u64 c, x;
-      const int32_t bin = find_bin(s.first, target, by_count, &c, &x, s);
+      const int32_t bin = find_bin(s.first, span, target, by_count, &c, &x, s);
       uint32_t lo, hi;
       keys_of(bin, &lo, &hi);
       lo = max(lo, from);
       // the bin's tokens, put in order where they are few
       const float least = logit_of(lo), most = logit_of(hi);
+      const float middle = 0.5f * least + 0.5f * most, half = (0.5f * most - 0.5f * least) * (1.0f + 0x1p-20f) + fabsf(middle) * 0x1p-20f + 1e-38f;
       if (tid == 0) s.listed = 0;
       __syncthreads();
-      each_run<DT>(r, tid * kRun, r.vocab, kStep, [&](const float(&z)[kRun], uint32_t valid, int64_t t) {
+      each_run<DT, 4>(r, tid * kRun, r.vocab, kStep, [&](const float(&z)[kRun], uint32_t valid, int64_t t) {
+        uint32_t near = 0;
 #pragma unroll
-        for (int j = 0; j < kRun; ++j) {
-          if (!(valid >> j & 1) || !(z[j] >= least && z[j] <= most)) continue;
-          const double y = m.y(z[j]);
-          if (m.bin(y) != bin) continue;
+        for (int j = 0; j < kRun; ++j) near |= fabsf(z[j] - middle) <= half ? 1u << j : 0u;
+        near &= valid;
+        while (__any(near != 0)) {  // few: read again one by one
+          if (near == 0) continue;
+          const int64_t i = t + __builtin_ctz(near);
+          near &= near - 1;
+          const float x = load_elem(r.logits, DT, i);
+          const double y = m.y(x);
+          if (!(x >= least && x <= most) || m.bin(y) != bin) continue;
           const uint32_t at = atomicAdd(&s.listed, 1u);
-          if (at < kListed) s.list[at] = Listed{u64(key_of(z[j])) << 32 | uint32_t(~uint32_t(t + j)), m.weight(y)};
+          if (at < kListed) s.list[at] = Listed{u64(key_of(x)) << 32 | uint32_t(~uint32_t(i)), m.weight(y)};
         }
       });
       __syncthreads();
@@ -449,7 +477,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const Row& r, co
         __syncthreads();
         clear<N>(s.sub);
         __syncthreads();
-        each_run<DT>(r, tid * kRun, r.vocab, kStep, [&](const float(&z)[kRun], uint32_t valid, int64_t) {
+        each_run<DT, 4>(r, tid * kRun, r.vocab, kStep, [&](const float(&z)[kRun], uint32_t valid, int64_t) {
 #pragma unroll
           for (int j = 0; j < kRun; ++j) {
             const uint32_t key = key_of(z[j]);
@@ -462,7 +490,8 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const Row& r, co
         });
         __syncthreads();
         u64 dc, dx;
-        const uint32_t i = uint32_t(find_bin(s.sub, target - (by_count ? c : x), by_count, &dc, &dx, s));
+        const Span part = span_of(s.sub, &dc, &dx, s);
+        const uint32_t i = uint32_t(find_bin(s.sub, part, target - (by_count ? c : x), by_count, &dc, &dx, s));
         c += dc, x += dx;
         hi -= i << shift;
         if (shift == 0 || hi <= lo) break;
@@ -477,7 +506,7 @@ __device__ __forceinline__ void sample_row(const SampleArgs& a, const Row& r, co
     if (likely > cut.key && !(cut.rank == 0 && cut.key == likely - 1)) {
       // (behind top-p: its sum is not known yet)
       u64 x = 0;
-      each_run<DT>(r, tid * kRun, r.vocab, kStep, [&](const float(&z)[kRun], uint32_t valid, int64_t) {
+      each_run<DT, 4>(r, tid * kRun, r.vocab, kStep, [&](const float(&z)[kRun], uint32_t valid, int64_t) {
 #pragma unroll
         for (int j = 0; j < kRun; ++j)
           if ((valid >> j & 1) && key_of(z[j]) >= likely) x += m.weight(m.y(z[j]));
