@@ -996,6 +996,10 @@ def _asked(value, name: str, rows: int, dtype: torch.dtype, what) -> tuple[torch
     if isinstance(value, torch.Tensor):
         if value.shape != (rows,):
             raise RuntimeError(f"one {name} per row, or one number")
+        if dtype == torch.int32 and value.dtype != dtype:
+            if value.is_floating_point():
+                raise RuntimeError(f"{name} must be whole numbers, got {value.dtype}")
+            value = value.clamp(-1, 2 ** 31 - 1)
         return value.to(dtype).contiguous(), what(0)
     return None, what(value)
 

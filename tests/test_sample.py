@@ -409,6 +409,18 @@ def test_exactly_as_many_as_16_bits_count(dtype, device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_numbers_of_other_types(device):
+    """top_k past 32 bits keeps all; 64-bit tensors are rounded as numbers are."""
+    g = torch.Generator().manual_seed(13)
+    z, u = torch.randn(3, 500, generator=g).to(device), torch.rand(3, generator=g).to(device)
+    k = torch.tensor([2 ** 32 + 5, 7, -(2 ** 40)], device=device)
+    want = ops.sample(z, u, top_k=torch.tensor([0, 7, 0], dtype=torch.int32, device=device), temperature=0.7)
+    got = ops.sample(z, u, top_k=k, temperature=torch.full((3,), 0.7, dtype=torch.float64, device=device))
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+    assert torch.equal(ops.sample(z, u, top_k=2 ** 40)[0], ops.sample(z, u)[0])
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_refusals(device):
     z, u = torch.zeros(2, 40, device=device), torch.zeros(2, device=device)
     bits, at = torch.zeros(3, 2, dtype=torch.int32, device=device), torch.zeros(2, dtype=torch.int32, device=device)
@@ -422,7 +434,7 @@ def test_refusals(device):
         (dict(vocab=0), "columns"), (dict(allow_bits=bits), "bit_rows"), (dict(bit_rows=at), "allow_bits"),
         (dict(allow_bits=bits[:, :1], bit_rows=at), "allow_bits must be"), (dict(allow_bits=bits.long(), bit_rows=at), "allow_bits must be"),
         (dict(allow_bits=bits, bit_rows=at[:1]), "one state per row"), (dict(err=torch.zeros(1, device=device)), "err must be int32"),
-        (dict(min_p=other), "same device"),
+        (dict(min_p=other), "same device"), (dict(top_k=torch.ones(2, device=device)), "whole numbers"),
     ]
     for kw, match in bad:
         with pytest.raises(RuntimeError, match=match):
