@@ -61,11 +61,15 @@ __global__ __launch_bounds__(kWaves* kWave, D <= 128 ? 2 : 1) void kv_prefix_ker
         q[t][Pt::begin(p) / 32 + k] = f;
       }
   }
-  f32x4 acc[NT][VT];
-  float top[NT], sum[NT];
+  // The sums of weights are a product with ones, of the rounded weights that the
+  // values are weighted by: four products of 16 cycles for 32 additions.
+  constexpr uint32_t kOnes = DT == BPD_DTYPE_BF16 ? 0x3F803F80u : 0x3C003C00u;
+  const Frag ones = {{kOnes, kOnes, kOnes, kOnes}};
+  f32x4 acc[NT][VT], sum[NT];  // (rows of sum are equal)
+  float top[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    top[t] = -3e38f, sum[t] = 0.0f;
+    top[t] = -3e38f, sum[t] = f32x4{0, 0, 0, 0};
 #pragma unroll
     for (int v = 0; v < VT; ++v) acc[t][v] = f32x4{0, 0, 0, 0};
   }
@@ -187,16 +191,12 @@ __global__ __launch_bounds__(kWaves* kWave, D <= 128 ? 2 : 1) void kv_prefix_ker
     if (first >= px.columns) continue;
     f32x4 s[NT][4];
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s[t][j] = f32x4{0, 0, 0, 0};
-#pragma unroll
     for (int k = 0; k < KW; ++k)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const Frag f = keys[now_at][j * KW + k][lane];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) s[t][j] = mfma<DT>(f, q[t][k], s[t][j]);
+        for (int t = 0; t < NT; ++t) s[t][j] = mfma<DT>(f, q[t][k], k == 0 ? f32x4{0, 0, 0, 0} : s[t][j]);
       }
     if (__any(!here_valid)) {
 #pragma unroll
@@ -222,7 +222,8 @@ __global__ __launch_bounds__(kWaves* kWave, D <= 128 ? 2 : 1) void kv_prefix_ker
         now = fmaxf(now, __shfl_xor(now, 32));
         const float keep = __builtin_amdgcn_exp2f(top[t] - now);
         top[t] = now;
-        sum[t] *= keep;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[t][i] *= keep;
 #pragma unroll
         for (int v = 0; v < VT; ++v)
 #pragma unroll
@@ -231,16 +232,17 @@ __global__ __launch_bounds__(kWaves* kWave, D <= 128 ? 2 : 1) void kv_prefix_ker
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[t][j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][i], to_log2, -top[t]));
-          sum[t] += s[t][j][i];
-        }
+        for (int i = 0; i < 4; ++i) s[t][j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][i], to_log2, -top[t]));
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           w[t][h].u[k] = two_rounded<DT>(s[t][2 * (k & 1)][2 * h + (k >> 1)], s[t][2 * (k & 1) + 1][2 * h + (k >> 1)]);
     }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) sum[t] = mfma<DT>(ones, w[t][h], sum[t]);
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -253,10 +255,8 @@ __global__ __launch_bounds__(kWaves* kWave, D <= 128 ? 2 : 1) void kv_prefix_ker
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int64_t c = first + t * 16 + m;
-    sum[t] += __shfl_xor(sum[t], 16);
-    sum[t] += __shfl_xor(sum[t], 32);
     if (c >= px.columns) continue;
-    if (g == 0) px.stats[at + c] = float2{top[t], sum[t]};
+    if (g == 0) px.stats[at + c] = float2{top[t], sum[t][0]};
     if (tile0 >= tile1) continue;
     f32x4* to = reinterpret_cast<f32x4*>(px.values + (at + c) * D) + g * VT;
 #pragma unroll
