@@ -628,7 +628,9 @@ class ConstraintBatch:
         (:func:`~bpdecode_amd.ops.sample`; the logits need no mask before, and
         the tokens no commit after).  Returns (int32 tokens, float32
         log-probabilities); a sequence whose grammar allows nothing yields -1
-        and is ``BROKEN``."""
+        and is ``BROKEN``.  No sequence twice in a call."""
+        if len(set(seq_ids)) < len(seq_ids):
+            raise RuntimeError("a sequence twice in one draw")
         slots = self._slots(seq_ids)
         pool = self._state
         kw = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p, "err": self._err}

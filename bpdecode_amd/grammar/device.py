@@ -618,7 +618,9 @@ class CFGConstraintBatch:
         under the grammar and advance each sequence by it
         (:func:`~bpdecode_amd.ops.sample`).  Returns (int32 tokens, float32
         log-probabilities); a sequence that is broken or allows nothing yields
-        -1 and is broken."""
+        -1 and is broken.  No sequence twice in a call."""
+        if len(set(seq_ids)) < len(seq_ids):
+            raise RuntimeError("a sequence twice in one draw")
         slots = self._slots(seq_ids)
         self._flush()
         rows = torch.arange(len(seq_ids), dtype=torch.int32, device=self.device)

@@ -1016,7 +1016,7 @@ def _cut_args(logits, temperature, top_k, top_p, min_p, vocab, allow_bits, state
         raise RuntimeError(f"logits have {columns} columns for a vocabulary of {V} tokens")
     code = _lib.dtype_code(logits.dtype)
     t, t_all = _asked(temperature, "temperature", B, torch.float32, float)
-    k, k_all = _asked(top_k, "top_k", B, torch.int32, lambda x: min(operator.index(x), 2 ** 31 - 1))
+    k, k_all = _asked(top_k, "top_k", B, torch.int32, lambda x: max(-1, min(operator.index(x), 2 ** 31 - 1)))
     p, p_all = _asked(top_p, "top_p", B, torch.float32, float)
     m, m_all = _asked(min_p, "min_p", B, torch.float32, float)
     dev = _same_device(logits, t, k, p, m, allow_bits, states, slots, *others)
@@ -1048,11 +1048,11 @@ def dense_sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p
                  allow_bits=None, bit_rows=None, states=None, slots=None, write_back=False, err=None):
     """:func:`sample` over the tables themselves: ``allow_bits`` (packed, one
     row per state) with ``tok_next`` and ``states`` (the state of row b is
-    ``states[slots[b]]`` with ``slots``, and ``write_back`` updates it there) or
-    with ``bit_rows`` int32 [batch], the row of ``allow_bits`` of each (-1:
-    allows nothing).  ``vocab``: columns that are tokens (all of ``logits``, or
-    of ``tok_next``, without it); ``err``: int32 [1] on the logits' device, flags
-    are OR-ed into it.  (token, logprob), and with ``tok_next`` the state."""
+    ``states[slots[b]]`` with ``slots``, and ``write_back`` updates it there; no
+    slot twice then) or with ``bit_rows`` int32 [batch], the row of
+    ``allow_bits`` of each (-1: allows nothing).  ``vocab``: columns that are
+    tokens (all of ``logits``, or of ``tok_next``, without it); ``err``: int32
+    [1] on the logits' device, flags are OR-ed into it.  (token, logprob), and with ``tok_next`` the state."""
     if tok_next is not None:
         if vocab is None:
             vocab = tok_next.shape[-1]
@@ -1089,6 +1089,14 @@ def dense_sample(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0, min_p
     return (token, logprob) if tok_next is None else (token, logprob, state)
 
 
+def _span(x: torch.Tensor) -> tuple[int, int]:
+    """First address of a tensor's elements, and the one past its last."""
+    begin = x.data_ptr()
+    if x.numel() == 0:
+        return begin, begin
+    return begin, begin + (sum((n - 1) * s for n, s in zip(x.shape, x.stride())) + 1) * x.element_size()
+
+
 def dense_truncate(logits, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, vocab=None, allow_bits=None, bit_rows=None,
                    slots=None, out=None, err=None):
     """:func:`truncate` over the tables themselves: ``bit_rows`` int32, the row
@@ -1102,9 +1110,10 @@ def dense_truncate(logits, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, vo
         out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     elif out.shape != logits.shape or out.dtype != logits.dtype:
         raise RuntimeError(f"out must be {logits.dtype} {list(logits.shape)}")
-    elif out is not logits and out.untyped_storage().data_ptr() == logits.untyped_storage().data_ptr() \
-            and (out.data_ptr() != logits.data_ptr() or out.stride() != logits.stride()):
-        raise RuntimeError("out must be logits itself or share no memory with it")
+    elif out is not logits and (out.data_ptr() != logits.data_ptr() or out.stride() != logits.stride()):
+        (x0, x1), (y0, y1) = _span(out), _span(logits)
+        if x0 < y1 and y0 < x1:
+            raise RuntimeError("out must be logits itself or share no memory with it")
     to, copied = _unit_stride_rows(out)
     args = (*head, to.data_ptr(), out.shape[1], to.stride(0) if B > 1 else out.shape[1], *cuts, ptr(at), sl, word)
     if dev.type == "cuda":

@@ -717,8 +717,8 @@ int bpd_host_verify(const void* logits, int dtype, int64_t rows, int32_t drafts,
  * allows none, is negative or, BPD_FLAG_STATE_RANGE, not below num_states;
  * every allowed logit -inf; one +inf or NaN, BPD_FLAG_LOGITS): token -1,
  * logprob -inf.  With tok_next, next_state[b] (may be NULL) and, with
- * write_back, the pool entry become the state after the token, -1 where there
- * is none.  Sums that decide are held in 64 bits.
+ * write_back, the pool entry (of one row at most) become the state after the
+ * token, -1 where there is none.  Sums that decide are held in 64 bits.
  * bpd_truncate: out [rows, cols >= vocab] (row stride out_ld) = the logits
  * that bpd_sample would draw from, -inf elsewhere; out may be logits itself
  * (the same rows), and overlaps them in no other way.  bpd_verify on

@@ -475,3 +475,31 @@ def test_refusals(device):
     with pytest.raises(RuntimeError, match="share no memory"):
         ops.dense_truncate(wide[:, :40], out=wide[:, 10:])
     assert ops.dense_sample(z[:0], u[:0])[0].shape == (0,) and ops.truncate(z[:0]).shape == (0, 40)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_out_beside_the_logits_in_one_allocation(device):
+    g = torch.Generator().manual_seed(14)
+    both = torch.randn(2, 3, 77, generator=g).to(device)
+    want = ops.truncate(both[0].clone(), top_k=5)
+    got = ops.truncate(both[0], top_k=5, out=both[1])
+    assert got.data_ptr() == both[1].data_ptr() and torch.equal(got, want)
+    with pytest.raises(RuntimeError, match="share no memory"):
+        ops.truncate(both[0], top_k=5, out=both.view(-1)[77:77 * 4].view(3, 77))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_sequence_twice_and_a_count_below_32_bits(device):
+    """Two rows of one sequence would read and advance one state at once."""
+    z, u = torch.zeros(2, TOY_VOCAB.size, device=device), torch.zeros(2, device=device)
+    batch = ConstraintBatch(FsaTensors.build("a+b*", TOY_VOCAB, dense=True), capacity=2, device=device)
+    batch.add("x")
+    with pytest.raises(RuntimeError, match="twice"):
+        batch.sample(["x", "x"], z, u)
+    g = build_pda_tensors(CompiledGrammar.build(parse_gbnf(synth.JSON_GBNF)), PDA_VOCAB)
+    batch = CFGConstraintBatch(g, capacity=2, device=device)
+    batch.add("x")
+    with pytest.raises(RuntimeError, match="twice"):
+        batch.sample(["x", "x"], torch.zeros(2, PDA_VOCAB.size, device=device), u)
+    with pytest.raises(RuntimeError, match="top_k"):  # not the 5 that its lower 32 bits are
+        ops.sample(z, u, top_k=5 - 2 ** 32)
