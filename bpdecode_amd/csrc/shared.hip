@@ -20,13 +20,14 @@ namespace {
 // one is multiplied.  Every column sees every token: a request with a query
 // that does not is left to kv_attend_kernel, and what its columns come to here
 // is not read.
-template <int DT, int D, int NT>
-__global__ __launch_bounds__(kWaves* kWave, D <= 128 ? 2 : 1) void kv_prefix_kernel(AttendArgs a, Prefix px,
-                                                                                   uint32_t groups) {
+template <int DT, int D, int NT, int W>
+__global__ __launch_bounds__(W* kWave, D <= 128 ? 2 : 1) void kv_prefix_kernel(AttendArgs a, Prefix px, uint32_t groups) {
   using Pt = Parts<D>;
-  constexpr int G = D / kKvGroup, KW = D / 32, VT = D / 16;
-  __shared__ Frag keys[2][4 * KW][kWave], values[2][2 * VT][kWave];
-  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  constexpr int G = D / kKvGroup, KW = D / 32, VT = D / 16, kStep = W / 4;
+  __shared__ Frag keys[2][kStep][4 * KW][kWave], values[2][kStep][2 * VT][kWave];
+  __shared__ int32_t pages_there[2][kStep][4];
+  const int lane = threadIdx.x % kWave, number = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int wave = number % 4, part = number / 4;  // its share of a tile, and which tile of a step
   const int m = lane & 15, g = lane >> 4;
   const uint32_t group = blockIdx.x % groups, kvh = blockIdx.x / groups % uint32_t(a.kv_heads);
   const int32_t chunk = int32_t(blockIdx.x / groups / uint32_t(a.kv_heads));
@@ -37,7 +38,7 @@ __global__ __launch_bounds__(kWaves* kWave, D <= 128 ? 2 : 1) void kv_prefix_ker
   const int32_t tile0 = chunk * per, tile1 = tile0 + per < tiles ? tile0 + per : tiles;
 
   const int32_t share = a.heads / a.kv_heads, per_request = a.tokens * share;
-  const int64_t first = (int64_t(group) * kWaves + wave) * (NT * 16);  // of the wave's columns
+  const int64_t first = (int64_t(group) * W + number) * (NT * 16);  // of the wave's columns
   const int64_t at = (int64_t(chunk) * a.kv_heads + kvh) * px.columns;
   const float to_log2 = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * 1.44269504088896340736f;
   Frag q[NT][KW];
@@ -82,8 +83,10 @@ __global__ __launch_bounds__(kWaves* kWave, D <= 128 ? 2 : 1) void kv_prefix_ker
   // a wave's share of a tile: keys of tokens 4 m + wave, values of tokens 16 g + 4 wave + 0..3
   uint32_t kc[KW], ks[Pt::count], vc[4][Pt::count], vs[G];
   int32_t kpage = -1, vpage = -1;  // of the tile to be loaded next
+  // (a wave whose tile lies past the last converts that once more, for nobody)
+  const auto first_of = [&](int32_t tile) { return (tile + part < tile1 ? tile + part : tile1 - 1) * kTile; };
   const auto load_pages = [&](int32_t tile) {
-    const int32_t t0 = tile * kTile;
+    const int32_t t0 = first_of(tile);
     kpage = px.table[(t0 + (m >> 2) * 16) >> shift];
     vpage = px.table[(t0 + g * 16) >> shift];
   };
@@ -92,7 +95,7 @@ __global__ __launch_bounds__(kWaves* kWave, D <= 128 ? 2 : 1) void kv_prefix_ker
     return a.pages + (int64_t(is_page(page) ? page : 0) * a.kv_heads + kvh) * int64_t(a.page.bytes());
   };
   const auto load = [&](int32_t tile) {
-    const int32_t t0 = tile * kTile;
+    const int32_t t0 = first_of(tile);
     const uint8_t* block = block_at(kpage);
     int32_t slot = ((t0 + 4 * m) & (P - 1)) + wave;
 #pragma unroll
@@ -125,10 +128,11 @@ __global__ __launch_bounds__(kWaves* kWave, D <= 128 ? 2 : 1) void kv_prefix_ker
 #pragma unroll
       for (int k = 0; k < Pt::width(p) / 32; ++k) {
         const uint32_t w = kc[Pt::begin(p) / 32 + k];
-        keys[to][wave * KW + Pt::begin(p) / 32 + k][lane] =
+        keys[to][part][wave * KW + Pt::begin(p) / 32 + k][lane] =
             Frag{{two_values<DT, 0>(w, sc), two_values<DT, 1>(w, sc), two_values<DT, 2>(w, sc), two_values<DT, 3>(w, sc)}};
       }
     }
+    if (wave == 0 && m == 0) pages_there[to][part][g] = there;
     if (!there) {  // no page: zeros, at a scale of one
 #pragma unroll
       for (int k = 0; k < G; ++k) vs[k] = 0x7F7F7F7Fu;
@@ -156,45 +160,46 @@ __global__ __launch_bounds__(kWaves* kWave, D <= 128 ? 2 : 1) void kv_prefix_ker
       }
 #pragma unroll
       for (int v = 0; v < Pt::width(p) / 16; ++v)
-        *reinterpret_cast<uint2*>(&values[to][(wave >> 1) * VT + Pt::begin(p) / 16 + v][lane].u[2 * (wave & 1)]) =
+        *reinterpret_cast<uint2*>(&values[to][part][(wave >> 1) * VT + Pt::begin(p) / 16 + v][lane].u[2 * (wave & 1)]) =
             uint2{x[v][0], x[v][1]};
     }
   };
 
-  bool there = false, there_next = false;  // this lane's 16 tokens: of the tile multiplied, of the one loaded
+  bool there_next = false;  // this lane's 16 tokens of the tile loaded
   if (tile0 < tile1) {
     load_pages(tile0);
     load(tile0);
-    there = is_page(vpage);
-    if (tile0 + 1 < tile1) load_pages(tile0 + 1);
+    const bool there = is_page(vpage);
+    if (tile0 + kStep < tile1) load_pages(tile0 + kStep);
     convert(0, there);
-    if (tile0 + 1 < tile1) {
-      load(tile0 + 1);
+    if (tile0 + kStep < tile1) {
+      load(tile0 + kStep);
       there_next = is_page(vpage);
-      if (tile0 + 2 < tile1) load_pages(tile0 + 2);
+      if (tile0 + 2 * kStep < tile1) load_pages(tile0 + 2 * kStep);
     }
   }
   int now_at = 0;
-  for (int32_t tile = tile0; tile < tile1; ++tile, now_at ^= 1) {
-    __syncthreads();  // this tile is converted, and the other buffer has been read
-    const bool here_valid = there;
-    if (!here_valid && a.err) atomicOr(a.err, BPD_FLAG_PAGE_RANGE);
-    if (tile + 1 < tile1) {
+  for (int32_t tile = tile0; tile < tile1; tile += kStep, now_at ^= 1) {
+    __syncthreads();  // these tiles are converted, and the other buffer has been read
+    if (tile + kStep < tile1) {
       convert(now_at ^ 1, there_next);
-      there = there_next;
-      if (tile + 2 < tile1) {
-        load(tile + 2);
+      if (tile + 2 * kStep < tile1) {
+        load(tile + 2 * kStep);
         there_next = is_page(vpage);
-        if (tile + 3 < tile1) load_pages(tile + 3);
+        if (tile + 3 * kStep < tile1) load_pages(tile + 3 * kStep);
       }
     }
     if (first >= px.columns) continue;
+#pragma unroll 1
+    for (int e = 0; e < kStep && tile + e < tile1; ++e) {
+    const bool here_valid = pages_there[now_at][e][g] != 0;
+    if (!here_valid && a.err) atomicOr(a.err, BPD_FLAG_PAGE_RANGE);
     f32x4 s[NT][4];
 #pragma unroll
     for (int k = 0; k < KW; ++k)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const Frag f = keys[now_at][j * KW + k][lane];
+        const Frag f = keys[now_at][e][j * KW + k][lane];
 #pragma unroll
         for (int t = 0; t < NT; ++t) s[t][j] = mfma<DT>(f, q[t][k], k == 0 ? f32x4{0, 0, 0, 0} : s[t][j]);
       }
@@ -247,10 +252,11 @@ __global__ __launch_bounds__(kWaves* kWave, D <= 128 ? 2 : 1) void kv_prefix_ker
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int v = 0; v < VT; ++v) {
-        const Frag f = values[now_at][h * VT + v][lane];
+        const Frag f = values[now_at][e][h * VT + v][lane];
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[t][v] = mfma<DT>(f, w[t][h], acc[t][v]);
       }
+  }
   }
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
@@ -266,7 +272,7 @@ __global__ __launch_bounds__(kWaves* kWave, D <= 128 ? 2 : 1) void kv_prefix_ker
 
 struct SharedSizes {
   AttendSizes own;
-  int32_t nt, chunks;
+  int32_t nt, waves, chunks;
   int64_t columns, groups;
   size_t partials, stats, bytes;
 };
@@ -279,9 +285,10 @@ SharedSizes shared_sizes(int64_t rows, int32_t tokens, int32_t heads, int32_t kv
   z.own = attend_sizes(rows, tokens, heads, kv_heads, dim, longest, longest > prefix ? longest - prefix : longest);
   z.columns = rows * tokens * (heads / kv_heads);
   z.nt = z.columns > kWaves * 16 ? 2 : 1;
-  z.groups = (z.columns + kWaves * 16 * z.nt - 1) / (kWaves * 16 * z.nt);
+  z.waves = dim <= 128 && z.columns > kWaves * 32 ? 8 : 4;
+  z.groups = (z.columns + z.waves * 16 * z.nt - 1) / (z.waves * 16 * z.nt);
   const int64_t tiles = std::min<int64_t>(prefix, 0x7FFFFFFF) / kTile;
-  z.chunks = int32_t(std::max<int64_t>(1, std::min<int64_t>(kPrefixBlocks / (z.groups * kv_heads), (tiles + 3) / 4)));
+  z.chunks = int32_t(std::max<int64_t>(1, std::min<int64_t>(kPrefixBlocks * 4 / z.waves / (z.groups * kv_heads), (tiles + 3) / 4)));
   z.partials = (2 * size_t(attend_runs(z.own, rows)) * z.own.piece * sizeof(float) + 15) / 16 * 16;
   const size_t all = size_t(z.chunks) * kv_heads * size_t(z.columns);
   z.stats = (all * sizeof(float2) + 15) / 16 * 16;
@@ -293,10 +300,16 @@ template <int DT, int D>
 int launch_prefix(const AttendArgs& a, const SharedSizes& z, const Prefix& px, hipStream_t s) {
   const int64_t blocks = z.groups * a.kv_heads * z.chunks;
   BPD_REQUIRE(blocks < (int64_t(1) << 31), "too many queries in one call");
+  if constexpr (D <= 128)
+    if (z.waves == 8) {
+      kv_prefix_kernel<DT, D, 2, 8><<<uint32_t(blocks), 8 * kWave, 0, s>>>(a, px, uint32_t(z.groups));
+      BPD_LAUNCHED();
+      return BPD_OK;
+    }
   if (z.nt == 1)
-    kv_prefix_kernel<DT, D, 1><<<uint32_t(blocks), kWaves * kWave, 0, s>>>(a, px, uint32_t(z.groups));
+    kv_prefix_kernel<DT, D, 1, 4><<<uint32_t(blocks), 4 * kWave, 0, s>>>(a, px, uint32_t(z.groups));
   else
-    kv_prefix_kernel<DT, D, 2><<<uint32_t(blocks), kWaves * kWave, 0, s>>>(a, px, uint32_t(z.groups));
+    kv_prefix_kernel<DT, D, 2, 4><<<uint32_t(blocks), 4 * kWave, 0, s>>>(a, px, uint32_t(z.groups));
   BPD_LAUNCHED();
   return BPD_OK;
 }
