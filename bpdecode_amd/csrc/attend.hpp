@@ -1,5 +1,5 @@
 // The attention kernels over the 4-bit paged cache (kv4.hpp) and the cut of a
-// call's work: for requests by themselves (attend.hip) and, with Shared, for
+// call's work: for requests by themselves (attend.hip) and, with Prefix, for
 // what follows a prefix that a batch shares (shared.hip).
 #pragma once
 

@@ -12,14 +12,24 @@ namespace bpd {
 namespace {
 
 // The prefix's whole tiles for all requests.  A block takes one key head, a
-// chunk of the tiles and kWaves * NT * 16 columns (request, query, head that
-// shares the key head), a wave NT tiles of 16 columns.  The codes of a tile are
-// converted once for the block, a fourth by each wave, into operands as the
-// products' lanes take them (attend.hpp's order, which keeps the weights in
-// their lane), and read from LDS by all four; the next tile is converted while
-// one is multiplied.  Every column sees every token: a request with a query
-// that does not is left to kv_attend_kernel, and what its columns come to here
-// is not read.
+// chunk of the tiles and W * NT * 16 columns (request, query, head that shares
+// the key head), a wave NT tiles of 16 columns.  The codes of a tile are
+// converted once for the block, a fourth by each of four waves, into operands
+// as the products' lanes take them (attend.hpp's order, which keeps the weights
+// in their lane), and read from LDS by all; the next W / 4 tiles are converted
+// while as many are multiplied.  Every column sees every token: a request with
+// a query that does not is left to kv_attend_kernel, and what its columns come
+// to here is not read.
+//
+// What bounds it: a SIMD's time goes to vector instructions (conversions, the
+// exponentials and roundings of weights) and products in about equal parts, which
+// two waves overlap in part.  128 requests of 32 heads, 8 key heads of 128,
+// behind 32,768 tokens: 69 GFLOP in 90 us, 760 of the 1,197 TFLOP/s that a large
+// product reaches (each request by itself would read 16 GB of cache).  A block's
+// conversions shared by eight waves instead of four took it from 99 us to 90;
+// scores formed a tile ahead of their exponentials, for 248 registers, from 99
+// to 110; loads that go around the registers do not fit codes that have to be
+// converted.
 template <int DT, int D, int NT, int W>
 __global__ __launch_bounds__(W* kWave, D <= 128 ? 2 : 1) void kv_prefix_kernel(AttendArgs a, Prefix px, uint32_t groups) {
   using Pt = Parts<D>;
@@ -277,18 +287,36 @@ struct SharedSizes {
   size_t partials, stats, bytes;
 };
 
-constexpr int kPrefixBlocks = 512;  // that the device is to have
+// How many blocks of four waves the device is to have: two a CU, which is what
+// their registers and LDS allow (128 requests behind 32,768 tokens: 99 us, with
+// 256 blocks 128, with 1,024 108; 12 requests: 15.3, 17.7, 15.3).
+constexpr int kPrefixBlocks = 512;
+
+// Wide blocks share what they convert, and narrow ones are more: the widest
+// that still come to a block for each place with chunks of four tiles.  (us of
+// narrow, 128 columns, 256 columns: 128 requests behind 32,768 tokens 128, 99,
+// 90; 48 of four drafts, heads of 64, behind 4,096 15.3, 17.0, 15.0; 40 behind
+// 2,048 13.5, 16.5, 15.7; 6 behind 1,000, which fill one narrow block, 9.1, 11.6.)
+// Heads past 128 have no LDS for the widest.  A chunk has four tiles, as what it
+// leaves is written and read once more, but where that makes fewer than eight
+// chunks, two for each wave that joins them.  (6 requests behind 1,000 tokens,
+// both kernels: 4 chunks 17.6 us, 8 16.0, 15 15.7; 40 behind 2,048: 8 chunks
+// 27.3, 16 30.3, 32 39; with eight tiles a chunk 40 behind 2,048 take 21.2 for
+// 16.5 in this kernel, 48 of four drafts 19.0 for 17.3.)
 
 SharedSizes shared_sizes(int64_t rows, int32_t tokens, int32_t heads, int32_t kv_heads, int32_t dim, int64_t longest,
                          int64_t prefix) {
   SharedSizes z{};
   z.own = attend_sizes(rows, tokens, heads, kv_heads, dim, longest, longest > prefix ? longest - prefix : longest);
   z.columns = rows * tokens * (heads / kv_heads);
-  z.nt = z.columns > kWaves * 16 ? 2 : 1;
-  z.waves = dim <= 128 && z.columns > kWaves * 32 ? 8 : 4;
-  z.groups = (z.columns + z.waves * 16 * z.nt - 1) / (z.waves * 16 * z.nt);
   const int64_t tiles = std::min<int64_t>(prefix, 0x7FFFFFFF) / kTile;
-  z.chunks = int32_t(std::max<int64_t>(1, std::min<int64_t>(kPrefixBlocks * 4 / z.waves / (z.groups * kv_heads), (tiles + 3) / 4)));
+  const auto groups = [&](int64_t of) { return (z.columns + of - 1) / of; };
+  const auto fills = [&](int64_t of) { return groups(of) * kv_heads * ((tiles + 3) / 4) * (of / 64) >= 2 * kPrefixBlocks; };
+  z.waves = dim <= 128 && z.columns > 128 && fills(256) ? 8 : 4;
+  z.nt = z.waves == 8 || (z.columns > 64 && fills(128)) ? 2 : 1;
+  z.groups = groups(z.waves * 16 * z.nt);
+  const int64_t room = kPrefixBlocks * 4 / z.waves / (z.groups * kv_heads);
+  z.chunks = int32_t(std::max<int64_t>(1, std::min<int64_t>(room, std::max<int64_t>((tiles + 3) / 4, std::min<int64_t>(tiles, 8)))));
   z.partials = (2 * size_t(attend_runs(z.own, rows)) * z.own.piece * sizeof(float) + 15) / 16 * 16;
   const size_t all = size_t(z.chunks) * kv_heads * size_t(z.columns);
   z.stats = (all * sizeof(float2) + 15) / 16 * 16;
