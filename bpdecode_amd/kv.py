@@ -6,6 +6,8 @@ the block's keys (and queries) to their positions and appends keys and values
 to the cache, :meth:`PagedKV4.attend` is the block's attention over the cache,
 and :meth:`bpdecode_amd.batch.ConstraintBatch.verify` decides on the drafts.
 A prompt is a long block, a plain decoding step a block of one token.
+:meth:`PagedKV4.attend_shared` is the attention of requests that begin with the
+same prompt, read once for all of them.
 
 An element takes 4.25 bits: an e2m1 code, and one power of two for 32
 neighbouring channels (the OCP microscaling layout of 4-bit floats, scales
