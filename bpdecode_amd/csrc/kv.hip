@@ -128,7 +128,7 @@ enum Partners { kHalves, kNeighbours, kAnywhere };
 // With Axes a pair's row of the tables goes by its axis; 8 pairs of one axis
 // (blocks of them, as models with axes for time, height and width lay them out)
 // are read as without, others one by one.  (12 prompts of 2,900 tokens, 36 heads
-// of 128, three axes in blocks: 147 us, 4.1 TB/s, 128 without axes; 3 blocks of
+// of 128, three axes in blocks: 147 us, 4.0 TB/s, 128 without axes; 3 blocks of
 // 1,533 tokens, 32 heads of 96, the axes of neighbouring pairs in turn: 22.)
 template <int DT, int D, int Passes, int Mode, bool Axes>
 __global__ __launch_bounds__(kKvThreads) void kv_append_kernel(AppendArgs a, uint32_t parts) {
