@@ -30,7 +30,7 @@ import torch
 
 from .. import _lib
 from .._lib import PDA_CONFIG_WORDS, PDA_MAX_CONFIGS, PDA_MAX_DEPTH, check, lib, ptr
-from ..ops import dense_sample
+from ..ops import dense_sample, dense_truncate
 from ..tokenizer import Vocabulary
 from .nfa import RuleNFA
 from .frames import frame_lists
@@ -631,6 +631,18 @@ class CFGConstraintBatch:
         pda_step(self._pool, self.g, token.clamp(min=0), slots, self._flags, self._err)
         self._flags[slots] |= token < 0
         return token, logprob
+
+    def truncate(self, seq_ids, logits, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """In place: ``-inf`` for every logit of ``logits`` [len(seq_ids),
+        columns] that :meth:`sample` would not draw from
+        (:func:`~bpdecode_amd.ops.truncate`).  Sequences stay where they are."""
+        slots = self._slots(seq_ids)
+        self._flush()
+        rows = torch.arange(len(seq_ids), dtype=torch.int32, device=self.device)
+        return dense_truncate(
+            logits, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, vocab=self.g.vocab_size,
+            allow_bits=pda_compute_mask(self.g, self._pool, slots), bit_rows=torch.where(self._flags[slots], -1, rows),
+            out=logits, err=self._err)
 
     def is_complete(self, seq_id: Hashable) -> bool:
         slot = self._slot_of[seq_id]

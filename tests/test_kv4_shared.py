@@ -250,3 +250,36 @@ def test_refusals_and_empty_calls(device):
     assert not none.attend_shared(*good).any()
     with pytest.raises(IndexError):
         none.check_errors()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,KV,H,D,P,dt,shared", [
+    (77, 4, 4, 64, 16, FP16, 8_400), (25, 8, 16, 96, 32, BF16, 8_260), (18, 8, 32, 128, 64, BF16, 4_224), (18, 8, 32, 128, 16, FP16, 4_100),
+    (20, 8, 16, 256, 32, BF16, 8_200), (25, 8, 8, 192, 64, FP16, 16_420)])
+def test_wide_blocks_of_long_prefixes(T, KV, H, D, P, dt, shared, dev):
+    """Enough work for blocks of 128 and 256 columns: odd numbers of tiles, of
+    columns and of tiles in a chunk, and then a page that is not there."""
+    print(f"shared {T} {KV} {H} {D} {shared}", flush=True)
+    B = 4
+    g = torch.Generator().manual_seed(D + T)
+    lengths = [shared + T + 31 * b for b in range(B - 1)] + [shared + T - 1]
+    blocks = max(lengths) // P + 1
+    cache, prefix, table, hidden = shared_cache(g, B, P, KV, D, dt, shared, blocks, dev, T)
+    q = torch.randn(B, T, H, D, generator=g).to(dt).to(dev)
+    lens = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    out = cache.attend_shared(q, prefix.to(dev), shared, hidden.to(dev), lens)
+    k, v = stored(cache, table, max(lengths))
+    plain, tol = R.attend(q.double().cpu().numpy(), k, v, lengths, dt)
+    close(out, plain, tol, v)
+    cache.check_errors()
+    most, eps = float(np.abs(v).max()), torch.finfo(dt).eps / 2
+    gone = 70 * 64 // P if shared > 5_000 else 3
+    prefix[gone] = -1
+    table[:, gone] = -1
+    out = cache.attend_shared(q, prefix.to(dev), shared, hidden.to(dev), lens)
+    with pytest.raises(IndexError):
+        cache.check_errors()
+    want = cache.attend(q, table.to(dev), lens)
+    with pytest.raises(IndexError):
+        cache.check_errors()
+    assert float((out.double() - want.double()).abs().max()) <= 4 * eps * most

@@ -503,3 +503,21 @@ def test_a_sequence_twice_and_a_count_below_32_bits(device):
         batch.sample(["x", "x"], torch.zeros(2, PDA_VOCAB.size, device=device), u)
     with pytest.raises(RuntimeError, match="top_k"):  # not the 5 that its lower 32 bits are
         ops.sample(z, u, top_k=5 - 2 ** 32)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_recursive_grammar_truncates_as_masked_logits_are(device):
+    g = build_pda_tensors(CompiledGrammar.build(parse_gbnf(synth.JSON_GBNF)), PDA_VOCAB)
+    batch = CFGConstraintBatch(g, capacity=3, device=device)
+    for i in range(3):
+        batch.add(i)
+    gen = torch.Generator().manual_seed(15)
+    ids = [2, 0]
+    for step in range(4):
+        logits = torch.randn(2, PDA_VOCAB.size + 3, generator=gen).to(device)
+        masked = batch.apply_mask(ids, logits[:, :PDA_VOCAB.size].clone())
+        got = batch.truncate(ids, logits, top_k=4, temperature=0.7)
+        assert got is logits and got[:, PDA_VOCAB.size:].isneginf().all()
+        assert torch.equal(got[:, :PDA_VOCAB.size], ops.truncate(masked, top_k=4, temperature=0.7))
+        batch.sample(ids, logits, torch.rand(2, generator=gen).to(device))
+        assert not batch.is_broken(2) and not batch.is_broken(0)
