@@ -189,6 +189,7 @@ __global__ __launch_bounds__(W* kWave, D <= 128 ? 2 : 1) void kv_prefix_kernel(A
     }
   }
   int now_at = 0;
+  bool missing = false;
   for (int32_t tile = tile0; tile < tile1; tile += kStep, now_at ^= 1) {
     __syncthreads();  // these tiles are converted, and the other buffer has been read
     if (tile + kStep < tile1) {
@@ -203,7 +204,6 @@ __global__ __launch_bounds__(W* kWave, D <= 128 ? 2 : 1) void kv_prefix_kernel(A
 #pragma unroll 1
     for (int e = 0; e < kStep && tile + e < tile1; ++e) {
     const bool here_valid = pages_there[now_at][e][g] != 0;
-    if (!here_valid && a.err) atomicOr(a.err, BPD_FLAG_PAGE_RANGE);
     f32x4 s[NT][4];
 #pragma unroll
     for (int k = 0; k < KW; ++k)
@@ -214,6 +214,7 @@ __global__ __launch_bounds__(W* kWave, D <= 128 ? 2 : 1) void kv_prefix_kernel(A
         for (int t = 0; t < NT; ++t) s[t][j] = mfma<DT>(f, q[t][k], k == 0 ? f32x4{0, 0, 0, 0} : s[t][j]);
       }
     if (__any(!here_valid)) {
+      missing = true;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -272,6 +273,13 @@ __global__ __launch_bounds__(W* kWave, D <= 128 ? 2 : 1) void kv_prefix_kernel(A
   for (int t = 0; t < NT; ++t) {
     const int64_t c = first + t * 16 + m;
     if (c >= px.columns) continue;
+    if (missing && a.err) {
+      // noted where some query sees it: requests whose queries do not all see the
+      // prefix are looked after by kv_attend_kernel
+      const int64_t b = c / per_request;
+      if (int32_t(c - b * per_request) / share < queries_of(a, b) && begin_of(a, sp, b) > 0)
+        atomicOr(a.err, BPD_FLAG_PAGE_RANGE);
+    }
     if (g == 0) px.stats[at + c] = float2{top[t], sum[t][0]};
     if (tile0 >= tile1) continue;
     f32x4* to = reinterpret_cast<f32x4*>(px.values + (at + c) * D) + g * VT;

@@ -873,9 +873,9 @@ int bpd_host_kv_attend(const uint8_t* pages, int64_t num_pages, int32_t page_siz
  * request; its block table names the pages behind them, at their places in
  * the whole request (entries before those are not read).  Lengths count the
  * shared tokens, and a query sees what it would in bpd_kv_attend over the whole
- * request, also where a request is shorter than the prefix.  More shared
- * tokens than prefix_table has room for count as many as it has
- * (BPD_FLAG_PAGE_RANGE; shared_all is refused).  Sums of the prefix and of the
+ * request, also where a request is shorter than the prefix; a missing page is
+ * flagged where some query sees it.  More shared tokens than prefix_table has
+ * room for count as many as it has (BPD_FLAG_PAGE_RANGE; shared_all is refused).  Sums of the prefix and of the
  * rest are kept apart in float and joined in float.  workspace:
  * bpd_kv_attend_shared_workspace_bytes bytes for `longest` = table_blocks *
  * page_size and `prefix` = prefix_blocks * page_size, 16-byte aligned. */
