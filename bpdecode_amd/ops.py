@@ -999,7 +999,7 @@ def _asked(value, name: str, rows: int, dtype: torch.dtype, what) -> tuple[torch
         if dtype == torch.int32 and value.dtype != dtype:
             if value.is_floating_point():
                 raise RuntimeError(f"{name} must be whole numbers, got {value.dtype}")
-            value = value.clamp(-1, 2 ** 31 - 1)
+            value = value.to(torch.int64).clamp(-1, 2 ** 31 - 1)  # (a narrower type does not hold the bounds)
         return value.to(dtype).contiguous(), what(0)
     return None, what(value)
 
