@@ -1103,9 +1103,12 @@ def dense_truncate(logits, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, vo
     of ``allow_bits`` of each row of logits (of ``bit_rows[slots[b]]`` with
     ``slots``); ``out``: a tensor like ``logits`` to write to, which may be
     ``logits``."""
-    work, dev, B, V, head, cuts, sl, word, kept = _cut_args(logits, temperature, top_k, top_p, min_p, vocab, allow_bits,
-                                                           None if bit_rows is None else _i32(bit_rows), slots, err, out)
+    if torch.is_grad_enabled() and (logits.requires_grad or (out is not None and out.requires_grad)):
+        raise RuntimeError("truncation has no gradient: call it under torch.no_grad(), or on logits.detach()")
     at = None if bit_rows is None else _i32(bit_rows)
+    work, dev, B, V, head, cuts, sl, word, kept = _cut_args(logits, temperature, top_k, top_p, min_p, vocab, allow_bits, at,
+                                                           slots, err, out)
+    given = out is not None
     if out is None:
         out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     elif out.shape != logits.shape or out.dtype != logits.dtype:
@@ -1122,6 +1125,8 @@ def dense_truncate(logits, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, vo
         check(lib().bpd_host_truncate(*args))
     if copied:
         out.copy_(to)
+    elif given and not out.is_inference():  # a backward pass that saved it has to notice
+        torch.autograd.graph.increment_version(out)
     return out
 
 
@@ -1179,7 +1184,9 @@ def truncate(logits: torch.Tensor, fsa: FsaTensors | None = None, states: torch.
     """The logits that :func:`sample` would draw from, ``-inf`` elsewhere (the
     kept ones as they are, not divided by the temperature).  Their softmax at
     the same temperature is the distribution of the draw: what a draft is
-    sampled from, and what :func:`verify_draft` on them verifies against."""
+    sampled from, and what :func:`verify_draft` on them verifies against.  It
+    has no gradient: logits that want one are refused but under
+    ``torch.no_grad()``."""
     kw = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p, "out": out}
     if fsa is None:
         if states is not None:
