@@ -203,71 +203,71 @@ __global__ __launch_bounds__(W* kWave, D <= 128 ? 2 : 1) void kv_prefix_kernel(A
     if (first >= px.columns) continue;
 #pragma unroll 1
     for (int e = 0; e < kStep && tile + e < tile1; ++e) {
-    const bool here_valid = pages_there[now_at][e][g] != 0;
-    f32x4 s[NT][4];
+      const bool here_valid = pages_there[now_at][e][g] != 0;
+      f32x4 s[NT][4];
 #pragma unroll
-    for (int k = 0; k < KW; ++k)
+      for (int k = 0; k < KW; ++k)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const Frag f = keys[now_at][e][j * KW + k][lane];
+        for (int j = 0; j < 4; ++j) {
+          const Frag f = keys[now_at][e][j * KW + k][lane];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) s[t][j] = mfma<DT>(f, q[t][k], k == 0 ? f32x4{0, 0, 0, 0} : s[t][j]);
+          for (int t = 0; t < NT; ++t) s[t][j] = mfma<DT>(f, q[t][k], k == 0 ? f32x4{0, 0, 0, 0} : s[t][j]);
+        }
+      if (__any(!here_valid)) {
+        missing = true;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[t][j][i] = here_valid ? s[t][j][i] : -INFINITY;
       }
-    if (__any(!here_valid)) {
-      missing = true;
+      Frag w[NT][2];
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < NT; ++t) {
+        float most = s[t][0][0];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[t][j][i] = here_valid ? s[t][j][i] : -INFINITY;
-    }
-    Frag w[NT][2];
+          for (int i = 0; i < 4; ++i) most = fmaxf(most, s[t][j][i]);
+        most *= to_log2;
+        // the running maximum is followed loosely, as in kv_attend_kernel
+        if (__any(most > top[t] + (kLift<DT> + 8.0f))) {
+          float now = fmaxf(top[t], most - kLift<DT>);
+          now = fmaxf(now, __shfl_xor(now, 16));
+          now = fmaxf(now, __shfl_xor(now, 32));
+          const float keep = __builtin_amdgcn_exp2f(top[t] - now);
+          top[t] = now;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      float most = s[t][0][0];
+          for (int i = 0; i < 4; ++i) sum[t][i] *= keep;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+          for (int v = 0; v < VT; ++v)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) most = fmaxf(most, s[t][j][i]);
-      most *= to_log2;
-      // the running maximum is followed loosely, as in kv_attend_kernel
-      if (__any(most > top[t] + (kLift<DT> + 8.0f))) {
-        float now = fmaxf(top[t], most - kLift<DT>);
-        now = fmaxf(now, __shfl_xor(now, 16));
-        now = fmaxf(now, __shfl_xor(now, 32));
-        const float keep = __builtin_amdgcn_exp2f(top[t] - now);
-        top[t] = now;
+            for (int i = 0; i < 4; ++i) acc[t][v][i] *= keep;
+        }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum[t][i] *= keep;
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int v = 0; v < VT; ++v)
+          for (int i = 0; i < 4; ++i) s[t][j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][i], to_log2, -top[t]));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[t][v][i] *= keep;
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            w[t][h].u[k] = two_rounded<DT>(s[t][2 * (k & 1)][2 * h + (k >> 1)], s[t][2 * (k & 1) + 1][2 * h + (k >> 1)]);
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[t][j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][i], to_log2, -top[t]));
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          w[t][h].u[k] = two_rounded<DT>(s[t][2 * (k & 1)][2 * h + (k >> 1)], s[t][2 * (k & 1) + 1][2 * h + (k >> 1)]);
+        for (int t = 0; t < NT; ++t) sum[t] = mfma<DT>(ones, w[t][h], sum[t]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int v = 0; v < VT; ++v) {
+          const Frag f = values[now_at][e][h * VT + v][lane];
+#pragma unroll
+          for (int t = 0; t < NT; ++t) acc[t][v] = mfma<DT>(f, w[t][h], acc[t][v]);
+        }
     }
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int t = 0; t < NT; ++t) sum[t] = mfma<DT>(ones, w[t][h], sum[t]);
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int v = 0; v < VT; ++v) {
-        const Frag f = values[now_at][e][h * VT + v][lane];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) acc[t][v] = mfma<DT>(f, w[t][h], acc[t][v]);
-      }
-  }
   }
 #pragma unroll
   for (int t = 0; t < NT; ++t) {

@@ -809,16 +809,6 @@ int bpd_host_kv_append(uint8_t* pages, int64_t num_pages, int32_t page_size, int
                        const float* sin, int64_t positions, int32_t rotary, int interleaved,
                        int32_t* err);
 int bpd_kv_append_axes(uint8_t* pages, int64_t num_pages, int32_t page_size, int32_t kv_heads,
-                  int32_t head_dim, int dtype, const void* k, int64_t k_row, int64_t k_token,
-                  int64_t k_head, const void* v, int64_t v_row, int64_t v_token, int64_t v_head,
-                  const void* q, int64_t q_row, int64_t q_token, int64_t q_head, int32_t heads,
-                  void* q_out, int64_t rows, int32_t tokens, const int32_t* block_table,
-                  int64_t table_ld, int32_t table_blocks, const int32_t* starts,
-                  const int32_t* counts, const float* cos, const float* sin, int64_t positions,
-                  int32_t rotary, int interleaved, const int32_t* places, int64_t place_axis,
-                       int64_t place_row, int64_t place_token, int32_t num_axes,
-                       const int32_t* axes, int32_t* err, void* stream);
-int bpd_host_kv_append_axes(uint8_t* pages, int64_t num_pages, int32_t page_size, int32_t kv_heads,
                        int32_t head_dim, int dtype, const void* k, int64_t k_row, int64_t k_token,
                        int64_t k_head, const void* v, int64_t v_row, int64_t v_token,
                        int64_t v_head, const void* q, int64_t q_row, int64_t q_token,
@@ -826,6 +816,18 @@ int bpd_host_kv_append_axes(uint8_t* pages, int64_t num_pages, int32_t page_size
                        const int32_t* block_table, int64_t table_ld, int32_t table_blocks,
                        const int32_t* starts, const int32_t* counts, const float* cos,
                        const float* sin, int64_t positions, int32_t rotary, int interleaved,
+                       const int32_t* places, int64_t place_axis, int64_t place_row,
+                       int64_t place_token, int32_t num_axes, const int32_t* axes, int32_t* err,
+                       void* stream);
+int bpd_host_kv_append_axes(uint8_t* pages, int64_t num_pages, int32_t page_size, int32_t kv_heads,
+                            int32_t head_dim, int dtype, const void* k, int64_t k_row,
+                            int64_t k_token, int64_t k_head, const void* v, int64_t v_row,
+                            int64_t v_token, int64_t v_head, const void* q, int64_t q_row,
+                            int64_t q_token, int64_t q_head, int32_t heads, void* q_out,
+                            int64_t rows, int32_t tokens, const int32_t* block_table,
+                            int64_t table_ld, int32_t table_blocks, const int32_t* starts,
+                            const int32_t* counts, const float* cos, const float* sin,
+                            int64_t positions, int32_t rotary, int interleaved,
                             const int32_t* places, int64_t place_axis, int64_t place_row,
                             int64_t place_token, int32_t num_axes, const int32_t* axes,
                             int32_t* err);
