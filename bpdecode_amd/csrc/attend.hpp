@@ -275,9 +275,10 @@ __device__ __forceinline__ int here(int x) {
 // maximum, sums and the accumulated values are floats; the weights are rounded
 // to the cache's type, because the second product takes its operands in 16
 // bits (the values themselves are exact in them).  A weight is off by half a
-// step, which the division's unrounded sum does not follow: with bfloat16 an
-// output of 1,000 tokens is off by 0.0020 of itself, the roundings of inputs
-// and output alone make that 0.0016.  (Weights as two terms of 16 bits, for
+// step, which the sum that divides does not follow here, where it is of weights
+// as they were before (a prefix's own sum, shared.hip, is of rounded ones): with
+// bfloat16 an output of 1,000 tokens is off by 0.0020 of itself, the roundings
+// of inputs and output alone make that 0.0016.  (Weights as two terms of 16 bits, for
 // twice the second product: 16 columns of 128 channels 174 -> 200 us, 20 of
 // them 57 -> 66, one short request 10.6 -> 11.9.)  In float16 a row's
 // largest weight lies between kLift and kLift + 8 powers of two, so that

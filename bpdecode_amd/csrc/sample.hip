@@ -591,8 +591,9 @@ __device__ __forceinline__ void general_row(const SampleArgs& a, const Row& r, c
 // pass that sums weights (an exponential and an addition to 64 bits in LDS for
 // each token that the cuts can reach), on the CUs that have a row; a maximum
 // takes 6 us, tables' sums 3, each cut's or the draw's pass over the row 8, from
-// the cache.  The floor of 6.7 us would take rows dealt over several CUs, and
-// counts joined between them at each of the five steps.
+// the cache.  Of the five steps the maximum and the sums, 32 us, would need one
+// join each if a row were dealt over the CUs that have none, the cuts one each;
+// rows are not dealt.
 constexpr int kThreads = 1024;
 template <int DT, bool Draw>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
@@ -617,7 +618,17 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
 // words), 6 the sums of counts and of the weights that the cuts need, 2.6 the cuts
 // themselves, which one wave finds, 5 the search for the token among its equals.
 // Truncation writes the row from its registers (160 rows under a grammar: 49
-// us, a copy takes 20).
+// us, a copy takes 20).  A grammar's row costs what one without does: it is loaded
+// and counted whole, however few tokens the state allows.
+//
+// Rows past the registers take as long for a token (256 of 262,144: 66 us, 0.25 ns
+// for each token of a row, as with 151,936; 48 of 200,064: 38 us).
+// One finite value that most of a row holds is the slowest input: lanes that add
+// to one word take 128 cycles, and past 65,535 tokens the row starts over in the
+// form for 32 bits.  48 rows of 151,936 with 99 of 100 logits at the type's lowest
+// number, as a mask with a finite fill leaves them: 300 us under top-p, 204 with
+// top-k of 50 (50,000 tokens: 55), with -inf in their place 28, unmasked 30; 32-bit
+// rows 161, 57, 63 and 95.
 constexpr int kMagnitudes = 32768;
 // Half the threads that a CU holds, with twice the registers: 40 runs are the
 // row of a vocabulary of 163,840, longer ones are read once more.  (1,024

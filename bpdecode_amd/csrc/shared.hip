@@ -21,11 +21,21 @@ namespace {
 // a query that does not is left to kv_attend_kernel, and what its columns come
 // to here is not read.
 //
-// What bounds it: a SIMD's time goes to vector instructions (conversions, the
-// exponentials and roundings of weights) and products in about equal parts, which
-// two waves overlap in part.  128 requests of 32 heads, 8 key heads of 128,
-// behind 32,768 tokens: 69 GFLOP in 90 us, 760 of the 1,197 TFLOP/s that a large
-// product reaches (each request by itself would read 16 GB of cache).  A block's
+// Scores, maximum, sums and accumulated values are floats; weights are rounded
+// to the cache's type, half a step, as kv_attend_kernel's are and for the same
+// reason (attend.hpp states what other choices cost).  Their sum is of the rounded
+// weights, so numerator and denominator err alike.  With bfloat16 outputs are off
+// by 0.00176 and 0.00177 of themselves (6 requests behind 1,000 tokens, 128 behind
+// 32,768), in float16 by 0.000217 (48 of four drafts), where rounding exact
+// results alone makes 0.00166 and 0.000204.
+//
+// What bounds it: dependent steps.  Products take 70,000 of a SIMD's 217,000
+// cycles, vector instructions (conversions, the exponentials and roundings of
+// weights) about as many, and the two waves of a SIMD cover the waits between
+// them in part.  128 requests of 32 heads, 8 key heads of 128, behind 32,768
+// tokens: 69 GFLOP in 90 us, 760 of the 1,197 TFLOP/s that a large product
+// reaches.  (The whole call takes 114 us where kv_attend_kernel over whole tables,
+// which name the same pages, takes 560.)  A block's
 // conversions shared by eight waves instead of four took it from 99 us to 90;
 // scores formed a tile ahead of their exponentials, for 248 registers, from 99
 // to 110; loads that go around the registers do not fit codes that have to be

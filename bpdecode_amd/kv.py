@@ -17,6 +17,7 @@ float16 magnitudes past 57,344 are, and kept as 49,152).
 run the HIP kernels on torch's current stream, CPU tensors the library's host
 entry points.  The cache keeps no lengths: the caller says where each request
 stands, so a block whose drafts were refused is overwritten by the next one.
+Nothing here has a gradient.
 """
 
 from __future__ import annotations
@@ -240,7 +241,11 @@ class PagedKV4:
         are those of the whole requests, as :meth:`append` and :meth:`attend`
         take them (a table's entries before the shared pages' end are not
         read).  The result is :meth:`attend`'s with the shared pages first in
-        every request's table."""
+        every request's table, and where prompt or batch are small that is the
+        faster call: single tokens of 32 heads, 8 of 128 in the cache, gain from
+        4 requests behind 8,000 tokens (25 us there, 20 here) and 128 behind
+        2,000 (43 and 39; of 128 behind 32,768 508 and 102), and lose behind 500
+        (128 requests 21 and 37); blocks of 100 tokens are even behind 8,000."""
         q, qs = self._block(q, "q")
         B, T, H, D = q.shape
         if H < 1 or H % self.kv_heads:

@@ -1164,8 +1164,10 @@ def sample(logits: torch.Tensor, uniforms: torch.Tensor, fsa: FsaTensors | None 
     vocabulary never count.
 
     Returns int32 tokens and float32 log-probabilities (of the token among
-    what is kept), and with ``fsa`` and ``states`` (one per row) the states after
-    the tokens; a row that allows nothing yields -1, -inf and -1."""
+    what is kept; without a gradient), and with ``fsa`` and ``states`` (one per
+    row) the states after the tokens; a row that allows nothing yields -1, -inf
+    and -1.  Tokens that a mask took out should be -inf, or left to ``fsa``: a
+    finite number that most of a row holds makes a draw several times slower."""
     kw = {"temperature": temperature, "top_k": top_k, "top_p": top_p, "min_p": min_p}
     if fsa is None:
         if states is not None:
